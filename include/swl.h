@@ -399,6 +399,73 @@ int swl_paged_attention_rows_bf16(void* const* qkv_rows, void* const* out_rows, 
                                   const int32_t* cache_seqlens, const int64_t* positions, const void* cos_sin,
                                   int64_t max_pos, int rope, float softmax_scale, void* stream);
 
+/* ------------------------------------------------- 4-bit KV cache ----
+ * No counterpart in the reference (its cache is bf16, paged_attention.py:7-128).
+ * A group of 32 dims of one token's key or value is 32 codes (sign, then 0 .5
+ * 1 1.5 2 3 4 6) times 2^(b - 127) of one byte b; b is the least in [2, 252]
+ * for which the group's largest magnitude is under 7 * 2^(b - 127) (a code is
+ * the nearest, ties to the even code, at most 6), and 255 for a group with an
+ * infinity or a NaN, which is read as NaN.
+ * pages: [num_blocks, hkv, block_size / 16] records of swl_kv4_record_bytes()
+ * (2176) bytes, one per 16 tokens of a head, 16-byte aligned; block_size a
+ * multiple of 16.  Bytes of a record (token t of the 16, dim d of the 128):
+ *   64 t + d / 2                                    key codes, even dims low
+ *   1024 + 256 (t / 4) + 16 (d / 8) + 4 (t % 4) + d % 8 / 2   value codes
+ *   2048 + 16 (d / 32) + t                          key scales
+ *   2112 + 16 (t / 4) + 4 (d / 32) + t % 4          value scales
+ * Zeroed pages hold zeros.
+ * New tokens are packed: sequence s has tokens cu_seqlens[s] ..
+ * cu_seqlens[s + 1] - 1 of the ntok (device int32 [nseq + 1], ascending from
+ * 0; sequences may be empty, tokens from cu_seqlens[nseq] on belong to none and
+ * their outputs are left as they were); cu_seqlens NULL: ntok / nseq tokens
+ * each.  cache_seqlens [nseq] int32: tokens of the sequence before its new
+ * ones; new token i of sequence s is token cache_seqlens[s] + i, in page
+ * block_table[s][that / block_size] (int32 [nseq, max_blocks]).  A token whose
+ * page is outside the table, or outside 0 .. num_blocks - 1, has no place: it
+ * is not stored, read as zeros, and not attended to.
+ * d must be 128.  All calls can be captured into a graph; they use no library
+ * scratch. */
+int64_t swl_kv4_record_bytes(void);
+
+/* Stores the new tokens' k and v (rows of hkv heads, token strides in
+ * elements), the keys rotated (NeoX halves, as swl_paged_attention_bf16) at
+ * positions[ntok] from cos_sin [max_pos, 128] (both NULL: no rotation; a
+ * position outside 0 .. max_pos - 1: that token is not rotated) and rounded
+ * once, from fp32.  k and v are left as they are.  With q (rows of hq heads),
+ * q_out [ntok, hq * 128] gets the rotated queries (q_out may be q when its
+ * stride is hq * 128); q and q_out may both be NULL. */
+int swl_kv4_append_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, void* q_out, int nseq, int64_t ntok, const int32_t* cu_seqlens, int hq,
+                        int hkv, int d, void* pages, int64_t num_blocks, int block_size, const int32_t* block_table,
+                        int64_t max_blocks, const int32_t* cache_seqlens, const int64_t* positions,
+                        const void* cos_sin, int64_t max_pos, void* stream);
+
+/* The held values of tokens starts[s] + i as bf16 (exact), k_out and v_out
+ * [ntok, hkv, 128]; cu_seqlens and starts as cu_seqlens and cache_seqlens
+ * above. */
+int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, const int32_t* block_table,
+                      int64_t max_blocks, const int32_t* starts, int nseq, int64_t ntok, const int32_t* cu_seqlens,
+                      int hkv, int d, void* k_out, void* v_out, void* stream);
+
+/* Causal attention of the new tokens (already appended) over the cache: query
+ * i of sequence s sees tokens 0 .. cache_seqlens[s] + i; query head j reads kv
+ * head j / (hq / hkv), any hq that is a multiple of hkv.  out [ntok, hq *
+ * 128].  Sums and softmax in fp32.  A query that sees no token gets zeros, one
+ * with an infinity or a NaN, or that sees a NaN key, NaN; a NaN value group
+ * reaches the queries that see it.  Values must leave room for their sum (under
+ * 2^118 / tokens).
+ * max_q_len: the most new tokens of a sequence (a hint for speed alone: it
+ * chooses between kernels, any value >= 1 gives a right result).
+ * workspace: swl_kv4_attention_workspace(nseq, ntok, max_q_len, hq, hkv,
+ * max_blocks * block_size) bytes of device memory, 16-byte aligned, owned by
+ * the call until its kernels have run; its contents do not matter. */
+int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int64_t max_q_len, int hq, int hkv, int64_t max_keys);
+int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t ntok, const int32_t* cu_seqlens,
+                           int64_t max_q_len, int hq, int hkv, int d, const void* pages, int64_t num_blocks,
+                           int block_size, const int32_t* block_table, int64_t max_blocks,
+                           const int32_t* cache_seqlens, float softmax_scale, void* out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

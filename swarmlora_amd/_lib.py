@@ -128,6 +128,14 @@ _SIGS = {
     "swl_silu_mul_bf16": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp]),
     "swl_paged_attention_rows_bf16": (c_int, [P_vp, P_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_i64,
                                               c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_f32, c_vp]),
+    "swl_kv4_record_bytes": (c_i64, []),
+    "swl_kv4_append_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_int,
+                                    c_int, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "swl_kv4_read_bf16": (c_int, [c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_vp, c_vp,
+                                  c_vp]),
+    "swl_kv4_attention_workspace": (c_i64, [c_int, c_i64, c_i64, c_int, c_int, c_i64]),
+    "swl_kv4_attention_bf16": (c_int, [c_vp, c_i64, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_i64,
+                                       c_int, c_vp, c_i64, c_vp, c_f32, c_vp, c_vp, c_i64, c_vp]),
 }
 
 _RUNTIME_SIGS = {}

@@ -1,0 +1,884 @@
+// The KV cache held in 4 bits: append with RoPE, read back, attention.
+//
+// A group of 32 dims of one token's key or value of one head is 32 codes
+// (sign and 0 .5 1 1.5 2 3 4 6, e2m1) times 2^(b - 127), b one byte; these are
+// the operands that gfx950's conversions and scaled MFMA take.  The cache is
+// [num_blocks, hkv, block_size / 16] records of 16 tokens of one head (a
+// "tile"), each laid out as the attention's MFMA operands read it:
+//   0     key codes    64 t + d / 2 (token t of the tile, even dims low)
+//   1024  value codes  256 (t / 4) + 16 (d / 8) + 4 (t % 4) + d % 8 / 2
+//   2048  key scales   16 (d / 32) + t
+//   2112  value scales 16 (t / 4) + 4 (d / 32) + t % 4
+// Keys: lane (t, g) of a wave's 16-byte load holds token t's dims 32 g .. + 31,
+// the A operand of the 16x16x128 MFMA with one scale per lane.  Values: lane
+// (g, c) holds 8 dims 8 c .. + 7 of the four tokens 4 g .. + 3, which is what
+// V^T as the A operand of a 16x16x32 MFMA needs of them, a token's scale per
+// dword.  A tile is 2176 contiguous bytes, 17 lines of 128: one head's cache is
+// read without its neighbours' (3.8 times fewer bytes than bf16).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <algorithm>
+#include <cmath>
+
+#include "dev_util.h"
+#include "swl.h"
+#include "swl_common.h"
+
+namespace {
+
+constexpr int kD = 128;          // head dim
+constexpr int kTile = 16;        // tokens of a record
+constexpr int kRec = 17 * kD;    // bytes of a record
+constexpr int kRecV = 1024, kRecKs = 2048, kRecVs = 2112;
+
+struct Kv4Args {
+  const bf16* q;            // [T, hq, 128], token stride qs
+  const bf16* k;            // append: [T, hkv, 128]
+  const bf16* v;
+  int64_t qs, ks, vs;
+  uint8_t* pages;
+  const int32_t* bt;        // [nseq, max_blocks]
+  const int32_t* seqlens;   // tokens before the new ones
+  const int32_t* cu;        // [nseq + 1] token offsets, null: L tokens each
+  const int64_t* pos;
+  const bf16* cs;           // [max_pos, 128]
+  bf16* out;                // append: rotated q; attention: [T, hq * 128]
+  bf16* out2;               // read: values
+  int64_t num_blocks, max_blocks, max_pos;
+  int64_t T;
+  int32_t nseq, L, hq, hkv, G;
+  int32_t tpp;              // tiles of a page
+  float scale;
+  // attention: records of parts, and how many parts are wanted
+  float* part;
+  int32_t target, min_spp, row_lo, row_hi;
+  int64_t max_rec;
+};
+
+// The sequence of packed token t (the same for the whole wave): how many
+// sequences end at or before it; nseq for a token behind the last one.
+__device__ __forceinline__ int seq_of(const Kv4Args& a, int64_t t, int lane) {
+  if (!a.cu) return (int)(t / a.L);
+  int s = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+    const int i = i0 + lane;
+    s += __popcll(__ballot(i < a.nseq && a.cu[i + 1] <= t));
+  }
+  return s;
+}
+
+// Record of the tile that holds token p of sequence s, head h; null where it
+// has no page.
+__device__ __forceinline__ uint8_t* tile_of(const Kv4Args& a, int s, int h, int64_t p) {
+  if (p < 0) return nullptr;
+  const int64_t tile = p / kTile, bi = tile / a.tpp;
+  if (bi >= a.max_blocks) return nullptr;
+  const int32_t blk = a.bt[(int64_t)s * a.max_blocks + bi];
+  if (blk < 0 || blk >= a.num_blocks) return nullptr;
+  return a.pages + (((int64_t)blk * a.hkv + h) * a.tpp + (tile - bi * a.tpp)) * kRec;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false);
+}
+
+// Scale byte of a group from the largest magnitude bits of its four lanes' 8
+// dims: the largest / 2^(b - 127) in [4, 7), so that it rounds as if the grid
+// went on to 8 (5 % less of its error than with [4, 8), where up to 8 would be
+// cut to 6); [2, 252], so that every value held is a normal, finite bf16;
+// 255 (read as NaN) for a group with an infinity or a NaN.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  top = max(top, dpp_u<0xB1>(top));  // quad_perm [1, 0, 3, 2]
+  top = max(top, dpp_u<0x4E>(top));  // quad_perm [2, 3, 0, 1]
+  const int b = (int)((top + 0x200000u) >> 23) - 2;
+  return top >= 0x7f800000u ? 255u : (uint32_t)min(max(b, 2), 252);
+}
+
+// Eight dims as codes under 2^(b - 127), dim i in bits 4 i.
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], uint32_t b) {
+  const float s = __uint_as_float(min(b, 252u) << 23);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+}
+
+__device__ __forceinline__ uint32_t top8(const float (&x)[8]) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t = max(t, __float_as_uint(x[e]) & 0x7fffffffu);
+  return t;
+}
+
+// NeoX rotation of q and k at their positions; q to its output rows, k and v
+// as 4-bit groups to the pages.  A 128-thread workgroup per (token, 16 heads),
+// eight threads a head with 16-byte accesses: thread c has dims 8 c .. + 7 and
+// the same of the other half, so that a quad of threads holds two whole groups
+// of 32.  Keys are rounded once, from the fp32 rotation.
+__global__ __launch_bounds__(128) void kv4_append_kernel(Kv4Args a) {
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int nq = a.out ? a.hq : 0;
+  const int h = blockIdx.y * 16 + (threadIdx.x >> 3);  // [0, nq): q, then k, then v heads
+  const int s = seq_of(a, t, lane);
+  if (s >= a.nseq || h >= nq + 2 * a.hkv) return;
+  const int c = threadIdx.x & 7, d = 8 * c;
+  const bool is_q = h < nq, is_k = !is_q && h < nq + a.hkv;
+  const int kvh = is_k ? h - nq : h - nq - a.hkv;
+  const bf16* row = (is_q ? a.q + t * a.qs + h * kD : is_k ? a.k + t * a.ks + kvh * kD : a.v + t * a.vs + kvh * kD) + d;
+  const u32x4 w1 = ldg16(row), w2 = ldg16(row + 64);
+  const int64_t pos = a.pos ? a.pos[t] : -1;
+  const int64_t i = t - (a.cu ? (int64_t)a.cu[s] : (int64_t)s * a.L);
+  const int64_t p = (int64_t)a.seqlens[s] + i;
+  float x1[8], x2[8];
+  unpack8(w1, x1);
+  unpack8(w2, x2);
+  if ((is_q || is_k) && pos >= 0 && pos < a.max_pos) {
+    const bf16* cs = a.cs + pos * kD + d;
+    float co[8], sn[8];
+    unpack8(ldg16(cs), co);
+    unpack8(ldg16(cs + 64), sn);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // (products of two bf16 are exact: one rounding each)
+      const float y1 = x1[e] * co[e] - x2[e] * sn[e];
+      x2[e] = x2[e] * co[e] + x1[e] * sn[e];
+      x1[e] = y1;
+    }
+  }
+  if (is_q) {
+    bf16x8 o1, o2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o1[e] = f2bf(x1[e]);
+      o2[e] = f2bf(x2[e]);
+    }
+    bf16* dst = a.out + (t * a.hq + h) * kD + d;
+    *reinterpret_cast<u32x4*>(dst) = __builtin_bit_cast(u32x4, o1);
+    *reinterpret_cast<u32x4*>(dst + 64) = __builtin_bit_cast(u32x4, o2);
+    return;
+  }
+  const uint32_t b1 = scale_byte(top8(x1)), b2 = scale_byte(top8(x2));
+  const uint32_t q1 = codes8(x1, b1), q2 = codes8(x2, b2);
+  uint8_t* rec = tile_of(a, s, kvh, p);
+  if (!rec) return;
+  const int tk = (int)(p & 15);
+  uint8_t* dst = rec + (is_k ? 64 * tk + 4 * c : kRecV + 256 * (tk >> 2) + 4 * (tk & 3) + 16 * c);
+  *reinterpret_cast<uint32_t*>(dst) = q1;
+  *reinterpret_cast<uint32_t*>(dst + (is_k ? 32 : 128)) = q2;
+  if ((c & 3) == 0) {
+    uint8_t* sc = rec + (is_k ? kRecKs + 16 * (c >> 2) + tk : kRecVs + 16 * (tk >> 2) + 4 * (c >> 2) + (tk & 3));
+    sc[0] = (uint8_t)b1;
+    sc[is_k ? 32 : 8] = (uint8_t)b2;
+  }
+}
+
+template <int J>
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t codes, float s) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, J));
+}
+__device__ __forceinline__ u32x4 values8(uint32_t codes, uint32_t b) {
+  const float s = __uint_as_float(b << 23);  // (exponent 255: the conversion gives NaN)
+  return u32x4{pair_bf16<0>(codes, s), pair_bf16<1>(codes, s), pair_bf16<2>(codes, s), pair_bf16<3>(codes, s)};
+}
+
+// Cached tokens as bf16: sixteen threads a (token, head) row of keys and of
+// values, a wave four tokens of a head.  Tokens without a page are zeros.
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
+  const int lane = threadIdx.x & 63, c = lane & 15;
+  const int h = blockIdx.y;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4;
+  for (int u = 0; u < 4; ++u) {
+    const int64_t tu = t0 + u;  // the sequence is found for a token at a time by the whole wave
+    if (tu >= a.T) return;
+    const int s = seq_of(a, tu, lane);
+    if (s >= a.nseq || (lane >> 4) != u) continue;
+    const int64_t p = (int64_t)a.seqlens[s] + tu - (a.cu ? (int64_t)a.cu[s] : (int64_t)s * a.L);
+    const uint8_t* rec = tile_of(a, s, h, p);
+    u32x4 k = u32x4{0u, 0u, 0u, 0u}, v = k;
+    if (rec) {
+      const int tk = (int)(p & 15);
+      k = values8(*reinterpret_cast<const uint32_t*>(rec + 64 * tk + 4 * c), rec[kRecKs + 16 * (c >> 2) + tk]);
+      v = values8(*reinterpret_cast<const uint32_t*>(rec + kRecV + 256 * (tk >> 2) + 16 * c + 4 * (tk & 3)),
+                  rec[kRecVs + 16 * (tk >> 2) + 4 * (c >> 2) + (tk & 3)]);
+    }
+    const int64_t at = (tu * a.hkv + h) * kD + 8 * c;
+    *reinterpret_cast<u32x4*>(a.out + at) = k;
+    *reinterpret_cast<u32x4*>(a.out2 + at) = v;
+  }
+}
+
+// ------------------------------------------------------------- attention ---
+// Rows are (new token, query head) pairs of one kv head, row = token * G +
+// head; a row sees the keys before its token and its own.  Work is cut into
+// units (sequence, kv head, block of RB rows, part of the keys); every wave
+// finds its unit by itself from the lengths (a scan over the sequences, 64 at
+// a time), so that the host knows none of them and a captured call follows
+// them.  A part is `spp` steps of KS keys, as many as make about `target`
+// units of the whole call, so that units are equally long whatever the
+// lengths are.  A block of one part writes its rows; others leave a record per
+// part, merged by kv4_combine_kernel.
+struct SeqInfo {
+  int t0, n, rb;
+  int64_t len, steps;  // steps of the longest row
+};
+
+template <int RB, int KS>
+__device__ __forceinline__ SeqInfo seq_info(const Kv4Args& a, int i) {
+  SeqInfo r{0, 0, 0, 0, 0};
+  if (i >= a.nseq) return r;
+  r.t0 = a.cu ? a.cu[i] : i * a.L;
+  r.n = a.cu ? a.cu[i + 1] - r.t0 : a.L;
+  r.len = a.seqlens[i];
+  if (r.t0 < 0 || r.n < 0 || (int64_t)r.t0 + r.n > a.T) r.n = 0;  // offsets that are none
+  const int64_t rows = (int64_t)r.n * a.G;
+  if (rows <= a.row_lo || rows > a.row_hi) return r;
+  r.rb = (int)((rows + RB - 1) / RB);
+  const int64_t kend = min<int64_t>(max<int64_t>(r.len + r.n, 0), a.max_blocks * a.tpp * kTile);
+  r.steps = max<int64_t>((kend + KS - 1) / KS, 1);
+  return r;
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((long long)v, o, 64);
+  return v;
+}
+
+// Steps of a part: as many as cut all blocks' steps into `target` parts (the
+// last one of a block may be shorter), so that there are at most `target` full
+// parts, `target` + blocks units, and 2 `target` records, whatever the lengths.
+template <int RB, int KS>
+__device__ __forceinline__ int steps_per_part(const Kv4Args& a, int lane) {
+  int64_t sum = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+    const SeqInfo r = seq_info<RB, KS>(a, i0 + lane);
+    sum += r.rb * r.steps;
+  }
+  sum = wave_sum(sum) * a.hkv;
+  return (int)max<int64_t>(a.min_spp, (sum + a.target - 1) / a.target);
+}
+
+struct Unit {
+  int s, h, b, p, parts, t0, n;
+  int64_t len, rec;  // rec: the block's first record (where parts > 1)
+};
+
+// COUNT_PARTS: u counts (block, part) pairs, else blocks.
+template <int RB, int KS, bool COUNT_PARTS>
+__device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int spp, int lane, Unit& o) {
+  o.h = (int)(u % a.hkv);
+  const int64_t want = u / a.hkv;
+  int64_t before = 0, rec = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+    const SeqInfo r = seq_info<RB, KS>(a, i0 + lane);
+    const int parts = (int)((r.steps + spp - 1) / spp);
+    const int units = r.rb * parts, mine = COUNT_PARTS ? units : r.rb;
+    const int recs = parts > 1 ? units : 0;
+    int inc = mine, rinc = recs;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(inc, d, 64), z = __shfl_up(rinc, d, 64);
+      if (lane >= d) {
+        inc += y;
+        rinc += z;
+      }
+    }
+    const uint64_t hit = __ballot(before + inc > want);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      o.s = i0 + l;
+      o.parts = __shfl(parts, l, 64);
+      o.t0 = __shfl(r.t0, l, 64);
+      o.n = __shfl(r.n, l, 64);
+      o.len = __shfl((long long)r.len, l, 64);
+      const int rb = __shfl(r.rb, l, 64);
+      const int local = (int)(want - before) - (__shfl(inc, l, 64) - __shfl(mine, l, 64));
+      const int per = COUNT_PARTS ? o.parts : 1;
+      o.b = rb - 1 - local / per;  // the blocks with the most keys first
+      o.p = local % per;
+      if (local < 0 || o.b < 0 || o.p < 0) return false;  // (counts past 32 bits: offsets that are none)
+      o.rec = ((rec + __shfl(rinc - recs, l, 64)) + (int64_t)o.b * o.parts) * a.hkv + o.h;
+      return true;
+    }
+    before += __shfl(inc, 63, 64);
+    rec += __shfl(rinc, 63, 64);
+  }
+  return false;
+}
+
+// A record: 16 rows as [dim % 8][row-dim slot 256] sums, then the rows' maxima
+// and sums of probabilities; slot (g * 16 + row) * 4 + i holds dim 32 g + 8 i +
+// e in piece e.
+constexpr int kRecF = 2048 + 32;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// 16 rows of q as the B operand of the scaled MFMA: fp8 twice, the nearest and
+// what is left of it, both exact but for elements under 2^-13 of their row's
+// largest (off by 2^-22 of that): a bf16 has 8 significant bits, e4m3 4.  The
+// lane has dims 16 g .. + 15 and 64 + 16 g .. + 15, as the operand counts them.
+struct QFrag {
+  i32x8 hi, lo;
+  int sb;  // scale byte of hi; lo's is 4 less
+};
+__device__ __forceinline__ QFrag q_frag(const bf16* row, int g) {
+  float x[4][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unpack8(ldg16(row + 64 * (j >> 1) + 16 * g + 8 * (j & 1)), x[j]);
+    top = max(top, top8(x[j]));
+  }
+  top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+  QFrag f;
+  const int e = (int)(top >> 23);  // the largest / 2^(sb - 127) in [128, 256)
+  f.sb = e == 255 ? 255 : max(e - 7, 5);
+  const float s = __uint_as_float((uint32_t)min(f.sb, 250) << 23), s2 = s * 0.0625f;
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float* y = &x[j][4 * w];
+      s16x2 h = {0, 0}, l = {0, 0};
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, y[0], y[1], s, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, y[2], y[3], s, true);
+      const int hw = __builtin_bit_cast(int, h);
+      const f32x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, s, false);
+      const f32x2 a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hw, s, true);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, y[0] - a0[0], y[1] - a0[1], s2, false);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, y[2] - a1[0], y[3] - a1[1], s2, true);
+      f.hi[2 * j + w] = hw;
+      f.lo[2 * j + w] = __builtin_bit_cast(int, l);
+    }
+  return f;
+}
+
+// scores of a 16-key tile (key 4 (lane / 16) + i) with 16 rows (lane % 16)
+__device__ __forceinline__ f32x4 scores(u32x4 k, int ks, const QFrag& q) {
+  const i32x8 A = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+  c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, q.hi, c, 4, 0, 0, ks, 0, q.sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, q.lo, c, 4, 0, 0, ks, 0, q.sb - 4);
+}
+
+// A lane's dwords of a tile's values (8 dims of four tokens) as pairs of
+// tokens: f[e][0], f[e][1] = tokens (0, 1), (2, 3) of dim e.
+__device__ __forceinline__ void v_pairs(u32x4 v, uint32_t vs, uint32_t (&f)[8][2]) {
+  const float s0 = __uint_as_float((vs & 0xffu) << 23), s1 = __uint_as_float((vs >> 8 & 0xffu) << 23);
+  const float s2 = __uint_as_float((vs >> 16 & 0xffu) << 23), s3 = __uint_as_float((vs >> 24) << 23);
+  auto put = [&](int e, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    f[e][0] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+    f[e][1] = __builtin_amdgcn_perm(w3, w2, 0x05040100u);
+    f[e + 1][0] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+    f[e + 1][1] = __builtin_amdgcn_perm(w3, w2, 0x07060302u);
+  };
+  put(0, pair_bf16<0>(v[0], s0), pair_bf16<0>(v[1], s1), pair_bf16<0>(v[2], s2), pair_bf16<0>(v[3], s3));
+  put(2, pair_bf16<1>(v[0], s0), pair_bf16<1>(v[1], s1), pair_bf16<1>(v[2], s2), pair_bf16<1>(v[3], s3));
+  put(4, pair_bf16<2>(v[0], s0), pair_bf16<2>(v[1], s1), pair_bf16<2>(v[2], s2), pair_bf16<2>(v[3], s3));
+  put(6, pair_bf16<3>(v[0], s0), pair_bf16<3>(v[1], s1), pair_bf16<3>(v[2], s2), pair_bf16<3>(v[3], s3));
+}
+
+__device__ __forceinline__ uint32_t ldg_u8(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) uint8_t*)(p);
+}
+__device__ __forceinline__ uint32_t ldg_u32(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) uint32_t*)(p);
+}
+
+// Takes the NaN groups out of a tile's values where some row does not see
+// their token (0 times a NaN is one); flags gets 0xff in the bytes of theirs.
+__device__ __forceinline__ void take_nan(u32x4& v, uint32_t& vs, uint32_t& flags) {
+  flags = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if ((vs >> (8 * k) & 0xffu) > 252u) {
+      v[k] = 0;
+      vs = (vs & ~(0xffu << (8 * k))) | 127u << (8 * k);
+      flags |= 0xffu << (8 * k);
+    }
+}
+// Whether the lane's row, which sees the first `see` keys of the step, sees one
+// whose values of dims 32 g .. + 31 (the lane's) are a NaN group.  By the whole
+// wave.
+__device__ __forceinline__ bool sees_nan(const uint32_t (&flags)[2], int see, int g) {
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int qd = 0; qd < 4; ++qd) {
+      const uint32_t f = (uint32_t)__shfl((int)flags[t], 16 * qd + 4 * g, 64);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad |= (f >> (8 * k) & 1u) != 0 && 16 * t + 4 * qd + k < see;
+    }
+  return bad;
+}
+
+// e^(m - M) in powers of two; a side without a key (-inf) counts for nothing,
+// one that has the maximum wholly (an infinite or NaN one too)
+__device__ __forceinline__ float merge_factor(float m, float M) {
+  return m == M ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M);
+}
+
+// dims 32 g + 8 i .. + 7 of a row; slot = (16 g + row % 16) * 4 + i
+__device__ __forceinline__ void write_row(const Kv4Args& a, const Unit& u, int r, int slot, float L,
+                                          const float (&o)[8]) {
+  const int tok = r / a.G, head = u.h * a.G + r - tok * a.G;
+  // (L is 0 where the row sees no key, NaN where a score is)
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16x8 y;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) y[d] = f2bf(L == 0.f ? 0.f : o[d] * inv);
+  bf16* dst = a.out + ((int64_t)(u.t0 + tok) * a.hq + head) * kD + 32 * (slot >> 6) + 8 * (slot & 3);
+  *(__attribute__((address_space(1))) u32x4*)dst = __builtin_bit_cast(u32x4, y);
+}
+
+// Few rows, many keys (single and drafted tokens): a workgroup of four waves
+// per unit of 16 SETS rows; wave w takes the part's steps of 32 keys (two
+// tiles) w, w + 4, ... on its own, loading each step's operands straight from
+// the pages into registers one step ahead; the waves' results meet in LDS.
+// S^T = K Q^T (scaled MFMA, keys as stored) leaves in a lane the keys 4 g .. +
+// 3 of both tiles of its row, which is the B operand of O^T = V^T P^T as it
+// is.  The probabilities enter as two bf16 (2^-17 of them unaccounted): the
+// matrix units idle here, the cache's bytes are the bound.
+constexpr int kSplitWaves = 4;
+
+template <int SETS>
+__global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split_kernel(Kv4Args a) {
+  constexpr int RB = 16 * SETS, KS = 32, W = kSplitWaves;
+  __shared__ __attribute__((aligned(16))) float mg[W][kRecF];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int spp = steps_per_part<RB, KS>(a, lane);
+  Unit u;
+  if (!find_unit<RB, KS, true>(a, blockIdx.x, spp, lane, u)) return;  // the same for the whole workgroup
+  const int rows = u.n * a.G, r0 = u.b * RB;
+  const int64_t kmax = a.max_blocks * a.tpp * kTile;
+  const int64_t ctx_lo = u.len + r0 / a.G + 1;                                 // of the block's first row
+  const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
+  const int64_t st0 = (int64_t)u.p * spp;                                      // the part's first step
+  const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
+  const int nst = (int)max<int64_t>(0, min<int64_t>(spp, steps - st0));
+  if (nst == 0 && u.p > 0) return;  // (the longest row's part; this block's end before it)
+  const int nw = nst > w ? (nst - w + W - 1) / W : 0;  // this wave's steps: st0 + w + j W
+
+  QFrag q[SETS];
+  int64_t ctx[SETS];
+#pragma unroll
+  for (int e = 0; e < SETS; ++e) {
+    const int r = min(r0 + e * 16 + col, rows - 1), tok = r / a.G;
+    q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
+    ctx[e] = u.len + tok + 1;
+  }
+
+  // lane 2 i + t: offset of the record of tile t of this wave's step j0 + i
+  // (-1: past the keys, or no page), a table of 32 steps
+  const int32_t* bt = a.bt + (int64_t)u.s * a.max_blocks;
+  int64_t table = -1;
+  auto look = [&](int j) {
+    const int64_t tile = (st0 + w + (int64_t)(j + (lane >> 1)) * W) * 2 + (lane & 1);
+    table = -1;
+    if (tile * kTile < kend) {
+      const int64_t bi = tile / a.tpp;
+      const int32_t blk = bt[bi];
+      if (blk >= 0 && blk < a.num_blocks)
+        table = (((int64_t)blk * a.hkv + u.h) * a.tpp + (tile - bi * a.tpp)) * kRec;
+    }
+  };
+  auto from_lane = [&](int l) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(table & 0xffffffff), l) |
+           ((int64_t)__builtin_amdgcn_readlane((int)(table >> 32), l) << 32);
+  };
+  struct Step {
+    u32x4 k[2], v[2];
+    uint32_t ks[2], vs[2];
+    uint32_t none;  // bit t: tile t is not there
+  };
+  auto load = [&](int j) {
+    Step x;
+    if ((j & 31) == 0) look(j);
+    x.none = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t at = from_lane(2 * (j & 31) + t);
+      x.none |= at < 0 ? 1u << t : 0u;
+      const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
+      x.k[t] = ldg16_nt(rec + 64 * col + 16 * g);
+      x.v[t] = ldg16_nt(rec + kRecV + 16 * lane);
+      x.ks[t] = ldg_u8(rec + kRecKs + lane);
+      x.vs[t] = ldg_u32(rec + kRecVs + 16 * g + (col & 12));
+    }
+    return x;
+  };
+
+  const float c2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
+  float m[SETS], l[SETS];
+  f32x4 acc[SETS][8];
+#pragma unroll
+  for (int e = 0; e < SETS; ++e) {
+    m[e] = -INFINITY;
+    l[e] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  Step x;
+  if (nw > 0) x = load(0);
+  for (int j = 0; j < nw; ++j) {
+    Step nx;
+    if (j + 1 < nw) nx = load(j + 1);
+    const int64_t k0 = (st0 + w + (int64_t)j * W) * KS;
+    f32x4 sv[SETS][2];
+#pragma unroll
+    for (int e = 0; e < SETS; ++e)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sv[e][t] = scores(x.k[t], (int)x.ks[t], q[e]);
+    // a row of the block ends inside the step, or a tile is missing
+    uint32_t nan_v[2] = {0, 0};  // scales of NaN groups, taken out of the values
+    if (k0 + KS > ctx_lo || x.none) {
+      const int live = (int)min<int64_t>(KS, kend - k0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const bool gone = x.none >> t & 1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (gone || 16 * t + 4 * g + k >= live) {  // what is stored there is anything: 0 times a NaN is one
+            x.v[t][k] = 0;
+            x.vs[t] = (x.vs[t] & ~(0xffu << (8 * k))) | 127u << (8 * k);
+          }
+        take_nan(x.v[t], x.vs[t], nan_v[t]);
+#pragma unroll
+        for (int e = 0; e < SETS; ++e) {
+          const int see = (int)min<int64_t>(KS, ctx[e] - k0);  // keys of the step that the row sees
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (gone || 16 * t + 4 * g + k >= see) sv[e][t][k] = -INFINITY;
+        }
+      }
+    }
+    uint32_t vf[2][8][2];
+    v_pairs(x.v[0], x.vs[0], vf[0]);
+    v_pairs(x.v[1], x.vs[1], vf[1]);
+#pragma unroll
+    for (int e = 0; e < SETS; ++e) {
+      float mx = fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
+                       fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
+      // the reference the exponents are taken from moves only when the maximum
+      // has grown by 2^8 since: any reference gives the same quotient
+      if (__ballot(mx > m[e] + 8.f) != 0) {
+        const float mn = fmaxf(m[e], mx);
+        const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
+        m[e] = mn;
+        l[e] *= corr;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
+      }
+      const float mr = m[e] == -INFINITY ? 0.f : m[e];
+      u32x4 ph, pl;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // tokens in pairs: one conversion for both
+        const f32x4& y = sv[e][k >> 1];
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1)], c2, -mr));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr));
+        l[e] += p0;
+        l[e] += p1;
+        const uint32_t hi = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0), f2bf(p1)});
+        ph[k] = hi;
+        pl[k] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0 - __uint_as_float(hi << 16)),
+                                                      f2bf(p1 - __uint_as_float(hi & 0xffff0000u))});
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const u32x4 f = u32x4{vf[0][d][0], vf[0][d][1], vf[1][d][0], vf[1][d][1]};
+        acc[e][d] = mfma16(f, ph, acc[e][d]);
+        acc[e][d] = mfma16(f, pl, acc[e][d]);
+      }
+    }
+    if (__ballot((nan_v[0] | nan_v[1]) != 0) != 0) {
+#pragma unroll
+      for (int e = 0; e < SETS; ++e)
+        if (sees_nan(nan_v, (int)min<int64_t>(KS, ctx[e] - k0), g))
+#pragma unroll
+          for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
+    }
+    x = nx;
+  }
+
+  // the row sums over the four lane groups, then the waves' results in LDS;
+  // thread = (g, row, i): dims 32 g + 8 i .. + 7
+  const int row = threadIdx.x >> 2 & 15;
+#pragma unroll
+  for (int e = 0; e < SETS; ++e) {
+    l[e] += __shfl_xor(l[e], 16, 64);
+    l[e] += __shfl_xor(l[e], 32, 64);
+    if (e > 0) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(&mg[w][d * 256 + lane * 4]) = acc[e][d];
+    if (g == 0) {
+      mg[w][2048 + col] = m[e];
+      mg[w][2064 + col] = l[e];
+    }
+    __syncthreads();
+    const int r = r0 + e * 16 + row;
+    float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < W; ++v) M = fmaxf(M, mg[v][2048 + row]);
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const float f = merge_factor(mg[v][2048 + row], M);
+      L += mg[v][2064 + row] * f;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] += mg[v][d * 256 + threadIdx.x] * f;
+    }
+    if (r >= rows) continue;
+    if (u.parts == 1) {
+      write_row(a, u, r, threadIdx.x, L, o);
+    } else {
+      const int64_t at = u.rec + (int64_t)u.p * a.hkv;
+      if (at >= a.max_rec) continue;  // (only where offsets overlap)
+      float* rec = a.part + (at * SETS + e) * kRecF;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) rec[d * 256 + threadIdx.x] = o[d];
+      if ((threadIdx.x & 0xc3) == 0) {
+        rec[2048 + row] = M;
+        rec[2064 + row] = L;
+      }
+    }
+  }
+}
+
+// Merges the parts of 16 rows of a block that was cut: a workgroup per (block,
+// kv head, set of 16 rows), thread (g, row, i) as above, parts in order.
+template <int RB, int KS>
+__global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
+  constexpr int SETS = RB / 16;
+  const int lane = threadIdx.x & 63;
+  const int spp = steps_per_part<RB, KS>(a, lane);
+  const int e = blockIdx.x % SETS;
+  Unit u;
+  if (!find_unit<RB, KS, false>(a, blockIdx.x / SETS, spp, lane, u) || u.parts == 1) return;
+  const int rows = u.n * a.G, row = threadIdx.x >> 2 & 15, r = u.b * RB + e * 16 + row;
+  // the block's own parts: its last row may see fewer keys than the sequence's
+  const int64_t kend = min<int64_t>(u.len + (min((u.b + 1) * RB, rows) - 1) / a.G + 1, a.max_blocks * a.tpp * kTile);
+  const int parts = (int)max<int64_t>(1, (max<int64_t>(kend, 0) + (int64_t)spp * KS - 1) / ((int64_t)spp * KS));
+  if (r >= rows || u.rec + (int64_t)(parts - 1) * a.hkv >= a.max_rec) return;
+  const float* rec = a.part + (u.rec * SETS + e) * kRecF;
+  const int64_t next = (int64_t)a.hkv * SETS * kRecF;
+  float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  constexpr int B = 4;  // records in flight together
+  for (int p0 = 0; p0 < parts; p0 += B) {
+    float pm[B], pl[B], po[B][8];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const float* rp = rec + min(p0 + b, parts - 1) * next;
+      pm[b] = rp[2048 + row];
+      pl[b] = rp[2064 + row];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) po[b][d] = rp[d * 256 + threadIdx.x];
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (p0 + b >= parts) break;
+      const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
+      L = L * fa + pl[b] * fb;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] = o[d] * fa + po[b][d] * fb;
+      M = mn;
+    }
+  }
+  write_row(a, u, r, threadIdx.x, L, o);
+}
+
+// ------------------------------------------------------------- launchers ---
+// Geometry of one attention call, from shapes alone: bounds that hold for
+// every set of lengths (steps_per_part).
+struct Kv4Plan {
+  int sets, rb, target, min_spp;
+  int64_t blocks, units, recs;
+};
+constexpr int kMinSteps = 8;  // steps of 32 keys of a part, at least
+
+Kv4Plan kv4_plan(int64_t nseq, int64_t T, int64_t max_q_len, int hq, int hkv, int64_t max_keys) {
+  Kv4Plan p{};
+  const int G = hq / hkv;
+  p.sets = max_q_len * G <= 16 ? 1 : 2;
+  p.rb = 16 * p.sets;
+  p.target = 1024;
+  p.min_spp = kMinSteps;
+  p.blocks = std::min<int64_t>(T * G, T * G / p.rb + nseq) * hkv;
+  const int64_t most = std::max<int64_t>(1, ((max_keys + 31) / 32 + p.min_spp - 1) / p.min_spp);
+  p.units = std::min<int64_t>(p.blocks * most, p.blocks + p.target);
+  p.recs = most > 1 ? std::min<int64_t>(p.blocks * most, 2 * p.target) : 0;
+  return p;
+}
+
+int kv4_check_pages(const char* what, const void* pages, int64_t num_blocks, int block_size,
+                    const int32_t* block_table, int64_t max_blocks, const int32_t* cache_seqlens, int nseq, int64_t T,
+                    const int32_t* cu, int hkv) {
+  auto bad = [&](const char* m) { return swl::fail(SWL_ERR_INVALID, std::string(what) + ": " + m); };
+  if (nseq < 0 || T < 0 || T >= ((int64_t)1 << 31)) return bad("bad sequence or token count");
+  if (hkv < 1 || hkv > 4096) return bad("bad head counts");
+  if (block_size < 16 || block_size % 16 != 0 || block_size > (1 << 20))
+    return bad("block_size must be a multiple of 16");
+  if (num_blocks < 1 || num_blocks >= ((int64_t)1 << 31) || max_blocks < 1 ||
+      max_blocks > ((int64_t)1 << 31) / block_size)
+    return bad("bad page geometry");
+  if (nseq == 0 || T == 0) return SWL_OK;
+  if (!pages || !block_table || !cache_seqlens) return bad("null argument");
+  if (reinterpret_cast<uintptr_t>(pages) & 15) return bad("pages must be 16-byte aligned");
+  if (!cu && T % nseq != 0) return bad("without cu_seqlens every sequence has as many tokens");
+  return SWL_OK;
+}
+
+Kv4Args kv4_args(void* pages, int64_t num_blocks, int block_size, const int32_t* block_table, int64_t max_blocks,
+                 const int32_t* cache_seqlens, int nseq, int64_t T, const int32_t* cu, int hkv) {
+  Kv4Args a{};
+  a.pages = reinterpret_cast<uint8_t*>(pages);
+  a.num_blocks = num_blocks;
+  a.tpp = block_size / kTile;
+  a.bt = block_table;
+  a.max_blocks = max_blocks;
+  a.seqlens = cache_seqlens;
+  a.nseq = nseq;
+  a.T = T;
+  a.cu = cu;
+  a.L = (int32_t)(nseq > 0 ? T / nseq : 0);
+  a.hkv = hkv;
+  return a;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+extern "C" int64_t swl_kv4_record_bytes(void) { return kRec; }
+
+extern "C" int swl_kv4_append_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                   int64_t v_stride, void* q_out, int nseq, int64_t ntok, const int32_t* cu_seqlens,
+                                   int hq, int hkv, int d, void* pages, int64_t num_blocks, int block_size,
+                                   const int32_t* block_table, int64_t max_blocks, const int32_t* cache_seqlens,
+                                   const int64_t* positions, const void* cos_sin, int64_t max_pos, void* stream) {
+  const char* what = "swl_kv4_append_bf16";
+  int rc = kv4_check_pages(what, pages, num_blocks, block_size, block_table, max_blocks, cache_seqlens, nseq, ntok,
+                           cu_seqlens, hkv);
+  if (rc) return rc;
+  SWL_CHECK(d == kD, SWL_ERR_INVALID, "swl_kv4_append_bf16: head_dim must be 128");
+  SWL_CHECK((q == nullptr) == (q_out == nullptr), SWL_ERR_INVALID, "swl_kv4_append_bf16: q and q_out go together");
+  SWL_CHECK(!q || (hq > 0 && hq <= 65536), SWL_ERR_INVALID, "swl_kv4_append_bf16: bad head counts");
+  SWL_CHECK((positions == nullptr) == (cos_sin == nullptr) && (!positions || max_pos > 0), SWL_ERR_INVALID,
+            "swl_kv4_append_bf16: positions and cos_sin go together");
+  if (nseq == 0 || ntok == 0) return SWL_OK;
+  SWL_CHECK(k && v, SWL_ERR_INVALID, "swl_kv4_append_bf16: null argument");
+  SWL_CHECK((!q || q_stride >= (int64_t)hq * d) && k_stride >= (int64_t)hkv * d && v_stride >= (int64_t)hkv * d,
+            SWL_ERR_INVALID, "swl_kv4_append_bf16: token strides smaller than a token row");
+  SWL_CHECK(aligned16(k) && aligned16(v) && (k_stride & 7) == 0 && (v_stride & 7) == 0 &&
+                (!q || (aligned16(q) && aligned16(q_out) && (q_stride & 7) == 0)) && aligned16(cos_sin),
+            SWL_ERR_INVALID, "swl_kv4_append_bf16: q, k, v rows and cos_sin must be 16-byte aligned");
+  Kv4Args a = kv4_args(pages, num_blocks, block_size, block_table, max_blocks, cache_seqlens, nseq, ntok, cu_seqlens,
+                       hkv);
+  a.q = reinterpret_cast<const bf16*>(q);
+  a.k = reinterpret_cast<const bf16*>(k);
+  a.v = reinterpret_cast<const bf16*>(v);
+  a.qs = q_stride;
+  a.ks = k_stride;
+  a.vs = v_stride;
+  a.out = reinterpret_cast<bf16*>(q_out);
+  a.hq = hq;
+  a.pos = positions;
+  a.cs = reinterpret_cast<const bf16*>(cos_sin);
+  a.max_pos = max_pos;
+  const int heads = (q ? hq : 0) + 2 * hkv;
+  hipLaunchKernelGGL(kv4_append_kernel, dim3((unsigned)ntok, (unsigned)((heads + 15) / 16)), dim3(128), 0,
+                     (hipStream_t)stream, a);
+  SWL_LAUNCH_CHECK("kv4_append_kernel launch");
+  return SWL_OK;
+}
+
+extern "C" int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, const int32_t* block_table,
+                                 int64_t max_blocks, const int32_t* starts, int nseq, int64_t ntok,
+                                 const int32_t* cu_seqlens, int hkv, int d, void* k_out, void* v_out, void* stream) {
+  int rc = kv4_check_pages("swl_kv4_read_bf16", pages, num_blocks, block_size, block_table, max_blocks, starts, nseq,
+                           ntok, cu_seqlens, hkv);
+  if (rc) return rc;
+  SWL_CHECK(d == kD, SWL_ERR_INVALID, "swl_kv4_read_bf16: head_dim must be 128");
+  if (nseq == 0 || ntok == 0) return SWL_OK;
+  SWL_CHECK(k_out && v_out && aligned16(k_out) && aligned16(v_out), SWL_ERR_INVALID,
+            "swl_kv4_read_bf16: k_out and v_out must be 16-byte aligned");
+  Kv4Args a = kv4_args(const_cast<void*>(pages), num_blocks, block_size, block_table, max_blocks, starts, nseq, ntok,
+                       cu_seqlens, hkv);
+  a.out = reinterpret_cast<bf16*>(k_out);
+  a.out2 = reinterpret_cast<bf16*>(v_out);
+  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((ntok + 15) / 16), (unsigned)hkv), dim3(256), 0,
+                     (hipStream_t)stream, a);
+  SWL_LAUNCH_CHECK("kv4_read_kernel launch");
+  return SWL_OK;
+}
+
+extern "C" int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int64_t max_q_len, int hq, int hkv,
+                                               int64_t max_keys) {
+  if (nseq <= 0 || ntok <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 0;
+  const Kv4Plan p = kv4_plan(nseq, ntok, std::min(max_q_len, ntok), hq, hkv, max_keys);
+  return p.recs * p.sets * kRecF * (int64_t)sizeof(float);
+}
+
+extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t ntok,
+                                      const int32_t* cu_seqlens, int64_t max_q_len, int hq, int hkv, int d,
+                                      const void* pages, int64_t num_blocks, int block_size,
+                                      const int32_t* block_table, int64_t max_blocks, const int32_t* cache_seqlens,
+                                      float softmax_scale, void* out, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+  int rc = kv4_check_pages("swl_kv4_attention_bf16", pages, num_blocks, block_size, block_table, max_blocks,
+                           cache_seqlens, nseq, ntok, cu_seqlens, hkv);
+  if (rc) return rc;
+  SWL_CHECK(d == kD, SWL_ERR_INVALID, "swl_kv4_attention_bf16: head_dim must be 128");
+  SWL_CHECK(hq > 0 && hq <= 65536 && hq % hkv == 0, SWL_ERR_INVALID, "swl_kv4_attention_bf16: bad head counts");
+  SWL_CHECK(softmax_scale > 0.f && std::isfinite(softmax_scale), SWL_ERR_INVALID,
+            "swl_kv4_attention_bf16: softmax_scale must be positive and finite");
+  SWL_CHECK(max_q_len >= 1, SWL_ERR_INVALID, "swl_kv4_attention_bf16: max_q_len must be at least 1");
+  if (nseq == 0 || ntok == 0) return SWL_OK;
+  SWL_CHECK(ntok * (int64_t)(hq / hkv) < ((int64_t)1 << 31), SWL_ERR_INVALID,
+            "swl_kv4_attention_bf16: too many rows");
+  SWL_CHECK(q && out, SWL_ERR_INVALID, "swl_kv4_attention_bf16: null argument");
+  SWL_CHECK(q_stride >= (int64_t)hq * d && (q_stride & 7) == 0 && aligned16(q) && aligned16(out), SWL_ERR_INVALID,
+            "swl_kv4_attention_bf16: q and out rows must be 16-byte aligned, a token's heads together");
+  Kv4Args a = kv4_args(const_cast<void*>(pages), num_blocks, block_size, block_table, max_blocks, cache_seqlens, nseq,
+                       ntok, cu_seqlens, hkv);
+  a.q = reinterpret_cast<const bf16*>(q);
+  a.qs = q_stride;
+  a.hq = hq;
+  a.G = hq / hkv;
+  a.scale = softmax_scale;
+  a.out = reinterpret_cast<bf16*>(out);
+  const Kv4Plan p = kv4_plan(nseq, ntok, std::min(max_q_len, ntok), hq, hkv, max_blocks * block_size);
+  SWL_CHECK(p.units < ((int64_t)1 << 31), SWL_ERR_INVALID, "swl_kv4_attention_bf16: too many rows");
+  SWL_CHECK(p.recs == 0 || (workspace && aligned16(workspace) &&
+                            workspace_bytes >= p.recs * p.sets * kRecF * (int64_t)sizeof(float)),
+            SWL_ERR_INVALID, "swl_kv4_attention_bf16: workspace smaller than swl_kv4_attention_workspace");
+  a.part = reinterpret_cast<float*>(workspace);
+  a.max_rec = p.recs;
+  a.target = p.target;
+  a.min_spp = p.min_spp;
+  a.row_lo = 0;
+  a.row_hi = 0x7fffffff;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.sets == 1)
+    hipLaunchKernelGGL(kv4_split_kernel<1>, dim3((unsigned)p.units), dim3(64 * kSplitWaves), 0, st, a);
+  else
+    hipLaunchKernelGGL(kv4_split_kernel<2>, dim3((unsigned)p.units), dim3(64 * kSplitWaves), 0, st, a);
+  SWL_LAUNCH_CHECK("kv4_split_kernel launch");
+  if (p.recs == 0) return SWL_OK;
+  const dim3 grid((unsigned)(p.blocks * p.sets));
+  if (p.sets == 1)
+    hipLaunchKernelGGL((kv4_combine_kernel<16, 32>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_combine_kernel<32, 32>), grid, dim3(256), 0, st, a);
+  SWL_LAUNCH_CHECK("kv4_combine_kernel launch");
+  return SWL_OK;
+}

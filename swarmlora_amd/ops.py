@@ -793,6 +793,174 @@ def paged_attention_rows(qkv_rows, out_rows, q_len: int, hq: int, hkv: int, d: i
         _ptr(cos_sin if rp else None), max_pos, rope, float(softmax_scale), _stream()))
 
 
+# ---------------------------------------------------- 4-bit KV cache ---
+KV4_RECORD = 2176  # bytes of 16 tokens of one head (swl_kv4_record_bytes)
+
+
+def kv4_pages(num_blocks: int, block_size: int, hkv: int, device) -> torch.Tensor:
+    """Empty pages of a cache held in 4 bits: uint8 [num_blocks, hkv,
+    block_size / 16, 2176] zeros (heads of 128 dims; swl.h documents the
+    record)."""
+    if block_size < 16 or block_size % 16:
+        raise ValueError("block_size must be a multiple of 16")
+    return torch.zeros(num_blocks, hkv, block_size // 16, KV4_RECORD, dtype=torch.uint8, device=device)
+
+
+def _kv4_cache(pages, block_table, lens, name, nseq, cu):
+    """Checks of what the kv4 calls share; nseq None: as many as cu says."""
+    _need(pages, "pages", torch.uint8)
+    if pages.dim() != 4 or pages.shape[3] != KV4_RECORD or not pages.is_contiguous():
+        raise ValueError(f"pages must be contiguous [num_blocks, hkv, block_size / 16, {KV4_RECORD}]")
+    _need(block_table, "block_table", torch.int32)
+    _need(lens, name, torch.int32)
+    if cu is not None:
+        _need(cu, "cu_seqlens", torch.int32)
+        if cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+            raise ValueError("cu_seqlens must be contiguous [nseq + 1]")
+        nseq = cu.numel() - 1
+    if block_table.dim() != 2 or block_table.shape[0] < nseq or not block_table.is_contiguous():
+        raise ValueError("block_table must be contiguous [nseq, max_blocks]")
+    if lens.dim() != 1 or lens.numel() < nseq or not lens.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with nseq entries")
+    _same_device(pages, block_table, lens, cu)
+    return nseq
+
+
+def _same_device(*ts):
+    """All tensors on the current device (launches go to its current stream)."""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != dev:
+            raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
+
+
+def _packed_rows(t: torch.Tensor, name: str, cu):
+    """Token rows as (tokens, heads, token stride): [nseq, L, heads, 128]
+    without cu_seqlens, [tokens, heads, 128] with."""
+    _need(t, name)
+    if t.dim() != (4 if cu is None else 3) or t.shape[-1] != 128:
+        raise ValueError(f"{name} must be [nseq, q_len, heads, 128], or [tokens, heads, 128] with cu_seqlens")
+    if cu is None:
+        return t.shape[0] * t.shape[1], t.shape[2], _token_rows(t, name, t.shape[2], 128)
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128)):
+        raise ValueError(f"{name} heads must be contiguous within a token")
+    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * 128
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
+               cache_seqlens: torch.Tensor, positions: Optional[torch.Tensor] = None,
+               cos_sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+               cu_seqlens: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None):
+    """Stores new tokens in the 4-bit pages (kv4_pages), keys rotated at
+    `positions` from cos_sin on the way (swl_kv4_append_bf16).  k, v [nseq, L,
+    hkv, 128], or packed [tokens, hkv, 128] with cu_seqlens int32 [nseq + 1];
+    tokens may be strided (views of the fused QKV rows).  positions int64, one
+    per token.  With q [.., hq, 128] the rotated queries are returned, in q_out
+    (contiguous, q's shape; may be q itself) or a new tensor; k and v are left
+    as they are.  Tokens behind the last sequence are not stored and their rows
+    of q_out are left as they were."""
+    ntok, hkv, ks = _packed_rows(k, "k", cu_seqlens)
+    nv, hv, vs = _packed_rows(v, "v", cu_seqlens)
+    if v.shape != k.shape:
+        raise ValueError("k and v must have one shape")
+    nseq = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", None if cu_seqlens is not None else
+                      k.shape[0], cu_seqlens)
+    if pages.shape[1] != hkv:
+        raise ValueError("cache geometry mismatch")
+    if (positions is None) != (cos_sin is None):
+        raise ValueError("positions and cos_sin go together")
+    max_pos = 0
+    if positions is not None:
+        _need(positions, "positions", torch.int64)
+        _need(cos_sin, "cos_sin")
+        if positions.numel() != ntok or not positions.is_contiguous():
+            raise ValueError("positions must be contiguous with one entry per token")
+        if cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be contiguous [max_pos, 128]")
+        max_pos = cos_sin.shape[0]
+    hq = qs = 0
+    if q is not None:
+        nq, hq, qs = _packed_rows(q, "q", cu_seqlens)
+        if q.shape[:-2] != k.shape[:-2]:
+            raise ValueError("q, k and v must have the same tokens")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
+        else:
+            _need(q_out, "q_out")
+            if q_out.shape != q.shape or not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous with q's shape")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    _same_device(k, v, positions, cos_sin, q, q_out)
+    _lib.check(_lib.load().swl_kv4_append_bf16(
+        _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(q_out), nseq, ntok, _ptr(cu_seqlens), hq, hkv, 128, _ptr(pages),
+        pages.shape[0], pages.shape[2] * 16, _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens),
+        _ptr(positions), _ptr(cos_sin), max_pos, _stream()))
+    return q_out
+
+
+def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, count: int,
+             cu_seqlens: Optional[torch.Tensor] = None):
+    """Cached tokens as bf16 (exact): (k, v) [nseq, count, hkv, 128] of tokens
+    starts[s] .. + count - 1 of every sequence, or, with cu_seqlens, packed
+    [count, hkv, 128] of cu_seqlens[s + 1] - cu_seqlens[s] tokens each
+    (swl_kv4_read_bf16).  Tokens without a page are zeros; rows behind the last
+    sequence hold anything."""
+    if count < 0:
+        raise ValueError("count must not be negative")
+    _need(starts, "starts", torch.int32)
+    nseq = _kv4_cache(pages, block_table, starts, "starts", starts.numel(), cu_seqlens)
+    hkv = pages.shape[1]
+    shape = (count, hkv, 128) if cu_seqlens is not None else (nseq, count, hkv, 128)
+    ntok = count if cu_seqlens is not None else nseq * count
+    k = torch.empty(shape, dtype=BF16, device=pages.device)
+    v = torch.empty(shape, dtype=BF16, device=pages.device)
+    _lib.check(_lib.load().swl_kv4_read_bf16(
+        _ptr(pages), pages.shape[0], pages.shape[2] * 16, _ptr(block_table), block_table.shape[1], _ptr(starts), nseq,
+        ntok, _ptr(cu_seqlens), hkv, 128, _ptr(k), _ptr(v), _stream()))
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
+                  softmax_scale: float, cu_seqlens: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
+                  out: Optional[torch.Tensor] = None):
+    """Causal grouped-head attention of new tokens, appended before
+    (kv4_append), over the 4-bit pages (swl_kv4_attention_bf16): query i of
+    sequence s sees tokens 0 .. cache_seqlens[s] + i.  q [nseq, L, hq, 128]
+    gives [nseq, L, hq * 128]; packed q [tokens, hq, 128] with cu_seqlens gives
+    [tokens, hq * 128], rows behind the last sequence left as they were in
+    `out`.  max_q_len: the most new tokens of a sequence where the host knows
+    it (a hint for speed alone)."""
+    ntok, hq, qs = _packed_rows(q, "q", cu_seqlens)
+    nseq = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", None if cu_seqlens is not None else
+                      q.shape[0], cu_seqlens)
+    hkv = pages.shape[1]
+    if hq < 1 or hkv < 1 or hq % hkv:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    if cu_seqlens is None:
+        max_q_len = q.shape[1]
+    elif max_q_len is None:
+        max_q_len = ntok
+    max_q_len = max(int(max_q_len), 1)
+    shape = (*q.shape[:-2], hq * 128)
+    if out is None:
+        out = torch.empty(shape, dtype=BF16, device=q.device)
+    else:
+        _need(out, "out")
+        if out.shape != shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous [.., hq * 128] with q's tokens")
+    _same_device(q, out)
+    lib = _lib.load()
+    bs = pages.shape[2] * 16
+    need = lib.swl_kv4_attention_workspace(nseq, ntok, max_q_len, hq, hkv, block_table.shape[1] * bs)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(lib.swl_kv4_attention_bf16(
+        _ptr(q), qs, nseq, ntok, _ptr(cu_seqlens), max_q_len, hq, hkv, 128, _ptr(pages), pages.shape[0], bs,
+        _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), float(softmax_scale), _ptr(out), _ptr(ws), need,
+        _stream()))
+    return out
+
+
 # -------------------------------------------------------------- timing ---
 def timer_arm(capacity: int):
     """Record HIP events around the next `capacity` decode-projection launches
