@@ -466,6 +466,35 @@ int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t nt
                            const int32_t* cache_seqlens, float softmax_scale, void* out, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
+/* Verification of drafted tokens (speculative decoding) from given random
+ * numbers; no counterpart in the reference.  Sequence s has drafts
+ * cu_drafts[s] .. cu_drafts[s + 1] - 1 of the ndraft draft_ids (device int32
+ * [nseq + 1]; NULL: ndraft / nseq each; at most max_drafts of them count), and
+ * one target row more: rows cu_drafts[s] + s .. cu_drafts[s + 1] + s of target
+ * (bf16 logits, row stride ld_target).  draft: the drafter's logits, a row per
+ * draft (row stride ld_draft); NULL: the drafter was certain of every draft
+ * (q = 1 there).
+ * p, q: softmax of logits / temperature[s], held in 64 bits.  Draft j is
+ * accepted while u_accept[j] * q_j(d) < p_j(d) (u in [0, 1)); the token after
+ * the accepted ones is drawn from max(p - q, 0) where a draft was refused, else
+ * from the row after the last one: the first index whose cumulative weight
+ * exceeds u_final[s] of the whole.  temperature <= 0: greedy (a draft is
+ * accepted while it is the first largest logit, which is the next token too).
+ * A draft outside the vocabulary is refused and the token drawn from p.  Rows
+ * whose probabilities are not numbers (a NaN, an infinity as the largest
+ * logit) refuse, and give their first largest logit, a NaN above all; so does
+ * a row with nothing left.  Logits of -inf are tokens that never come.
+ * out_tokens [nseq, max_drafts + 1]: the accepted drafts, the drawn token, then
+ * -1; out_accepted [nseq]: how many were accepted.  2 ndraft + nseq at most
+ * 65535.  workspace: swl_verify_drafts_workspace(...) bytes of device memory,
+ * 16-byte aligned, owned by the call until its kernels have run. */
+int64_t swl_verify_drafts_workspace(int nseq, int64_t ndraft, int64_t vocab, int with_draft);
+int swl_verify_drafts_bf16(const void* target, int64_t ld_target, const void* draft, int64_t ld_draft, int64_t vocab,
+                           const int64_t* draft_ids, const int32_t* cu_drafts, int nseq, int64_t ndraft,
+                           int max_drafts, const float* temperature, const float* u_accept, const float* u_final,
+                           int64_t* out_tokens, int32_t* out_accepted, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

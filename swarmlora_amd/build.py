@@ -26,6 +26,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 SOURCES = [
     "kernels.hip",
     "kv4.hip",
+    "verify.hip",
     "ipc_queue.cpp",
     "aggregator.cpp",
     "worker_slots.cpp",

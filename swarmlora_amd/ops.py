@@ -641,6 +641,85 @@ def sample(logits: torch.Tensor, out_tok: Sequence[torch.Tensor], do_sample: Seq
                                            _i32_array(top_k), f32(top_p), int(seed), _stream()))
 
 
+def _logit_rows(t: torch.Tensor, name: str, packed: bool):
+    """Logits as (rows, vocab, row stride): [rows, vocab] where packed, else
+    [nseq, n, vocab]; rows may be strided."""
+    _need(t, name)
+    if t.dim() != (2 if packed else 3):
+        raise ValueError(f"{name} must be [rows, vocab] with cu_drafts, else [nseq, n, vocab]")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    rows, vocab = t.shape[:-1].numel(), t.shape[-1]
+    ld = max(t.stride(-2), vocab) if t.shape[-2] > 1 else max(vocab, t.stride(0) if t.dim() == 3 else 0)
+    if rows > 1 and t.shape[-2] > 1 and t.stride(-2) < vocab:
+        raise ValueError(f"{name} rows must not overlap")
+    if not packed and t.shape[0] > 1 and t.shape[1] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
+        raise ValueError(f"{name} rows must be evenly strided")
+    return rows, vocab, ld
+
+
+def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept: torch.Tensor,
+                  u_final: torch.Tensor, temperature: torch.Tensor, draft_logits: Optional[torch.Tensor] = None,
+                  cu_drafts: Optional[torch.Tensor] = None, max_drafts: Optional[int] = None):
+    """Accepts drafted tokens against the target's probabilities and draws the
+    next token of every sequence, from given random numbers
+    (swl_verify_drafts_bf16, which states the rule).  draft_ids int64 [nseq, n]
+    with target_logits bf16 [nseq, n + 1, vocab] and draft_logits [nseq, n,
+    vocab]; or packed: draft_ids [tokens], cu_drafts int32 [nseq + 1], target
+    rows [tokens + nseq, vocab], draft rows [tokens, vocab], and max_drafts, the
+    most drafts of a sequence (later ones do not count).  draft_logits None: the
+    drafter was certain.  u_accept fp32, one per draft, u_final and temperature
+    fp32 [nseq] (temperature <= 0: greedy).  Top-k or top-p: set the logits that
+    are out to -inf in both.  Returns (tokens int64 [nseq, max_drafts + 1]:
+    accepted drafts, the drawn token, -1; accepted int32 [nseq])."""
+    packed = cu_drafts is not None
+    rows, vocab, ldt = _logit_rows(target_logits, "target_logits", packed)
+    _need(draft_ids, "draft_ids", torch.int64)
+    _need(u_accept, "u_accept", torch.float32)
+    _need(u_final, "u_final", torch.float32)
+    _need(temperature, "temperature", torch.float32)
+    nd = draft_ids.numel()
+    if packed:
+        _need(cu_drafts, "cu_drafts", torch.int32)
+        if cu_drafts.dim() != 1 or cu_drafts.numel() < 1 or not cu_drafts.is_contiguous():
+            raise ValueError("cu_drafts must be contiguous [nseq + 1]")
+        if max_drafts is None or max_drafts < 0:
+            raise ValueError("cu_drafts needs max_drafts")
+        nseq = cu_drafts.numel() - 1
+        if draft_ids.dim() != 1 or rows != nd + nseq:
+            raise ValueError("packed drafts need draft_ids [tokens] and tokens + nseq target rows")
+    else:
+        if draft_ids.dim() != 2:
+            raise ValueError("draft_ids must be [nseq, n]")
+        nseq, n = draft_ids.shape
+        if target_logits.shape[0] != nseq or target_logits.shape[1] != n + 1:
+            raise ValueError("target_logits must be [nseq, n + 1, vocab]")
+        max_drafts = n if max_drafts is None else int(max_drafts)
+        if max_drafts != n:
+            raise ValueError("max_drafts goes with cu_drafts")
+    if u_accept.numel() != nd or u_final.numel() != nseq or temperature.numel() != nseq:
+        raise ValueError("u_accept needs one number per draft, u_final and temperature one per sequence")
+    for t, nm in ((draft_ids, "draft_ids"), (u_accept, "u_accept"), (u_final, "u_final"), (temperature, "temperature")):
+        if not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous")
+    ldd = 0
+    if draft_logits is not None:
+        dr, dv, ldd = _logit_rows(draft_logits, "draft_logits", packed)
+        if dr != nd or dv != vocab or (not packed and nd and draft_logits.shape[:2] != draft_ids.shape):
+            raise ValueError("draft_logits need one row of the target's vocabulary per draft")
+    _same_device(target_logits, draft_ids, u_accept, u_final, temperature, draft_logits, cu_drafts)
+    dev = target_logits.device
+    tok = torch.empty(nseq, max_drafts + 1, dtype=torch.int64, device=dev)
+    acc = torch.empty(nseq, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    need = lib.swl_verify_drafts_workspace(nseq, nd, vocab, 1 if draft_logits is not None else 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.check(lib.swl_verify_drafts_bf16(
+        _ptr(target_logits), ldt, _ptr(draft_logits), ldd, vocab, _ptr(draft_ids), _ptr(cu_drafts), nseq, nd, max_drafts,
+        _ptr(temperature), _ptr(u_accept), _ptr(u_final), _ptr(tok), _ptr(acc), _ptr(ws), need, _stream()))
+    return tok, acc
+
+
 def zero_blocks(caches: Sequence[torch.Tensor], block_ids: torch.Tensor):
     """Zero whole pages block_ids of every cache [num_blocks, ...]."""
     _need(block_ids, "block_ids", torch.int64)

@@ -1,0 +1,251 @@
+"""GPU tests of the verification of drafted tokens (swl_verify_drafts_bf16)
+against the rule in 64 bits on the CPU: tokens and counts have to be equal.
+(A draw within 1e-13 of a border could differ; the seeds here have none.)"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests._util import BF16
+
+pytestmark = pytest.mark.gpu
+
+
+def _ops():
+    from swarmlora_amd import ops
+    return ops
+
+
+def _first_largest(x):
+    """First index of the largest logit, a NaN above all."""
+    x = x.float().clone()
+    if torch.isnan(x).any():
+        return int(torch.isnan(x).int().argmax())
+    return int((x == x.max()).int().argmax())
+
+
+def _soft(x, t):
+    x = x.double()
+    e = torch.exp((x - x.max()) / t)
+    return e / e.sum()
+
+
+def rule(tgt, ids, u, u_last, temp, drf, new, max_drafts):
+    toks, acc = [], []
+    at = row = 0
+    V = tgt.shape[1]
+    for s, n in enumerate(new):
+        t = float(temp[s])
+        out, take = [], 0
+        less = None
+        for j in range(min(n, max_drafts)):
+            x, d = tgt[row + j], int(ids[at + j])
+            if t <= 0:
+                if d != _first_largest(x):
+                    break
+            elif not 0 <= d < V:
+                break
+            else:
+                p = _soft(x, t)
+                q = _soft(drf[at + j], t) if drf is not None else torch.zeros(V, dtype=torch.float64).index_fill_(
+                    0, torch.tensor([d]), 1.0)
+                if not float(u[at + j]) * float(q[d]) < float(p[d]):
+                    less = q if drf is not None else torch.where(torch.arange(V) == d, math.inf, 0.0).double()
+                    break
+            out.append(d)
+            take += 1
+        x = tgt[row + take]
+        w = _soft(x, t) if t > 0 else torch.full((V,), math.nan)
+        if less is not None:
+            w = (w - less).clamp(min=0)
+        c = np.cumsum(w.numpy())
+        if t <= 0 or not c[-1] > 0:
+            pick = _first_largest(x)
+        else:
+            want = float(u_last[s]) * c[-1]
+            above = np.nonzero((c > want) & (w.numpy() > 0))[0]
+            pick = int(above[0]) if len(above) else int(np.nonzero(w.numpy() > 0)[0][-1])
+        toks.append(out + [pick] + [-1] * (max_drafts - take))
+        acc.append(take)
+        at += n
+        row += n + 1
+    return torch.tensor(toks), torch.tensor(acc, dtype=torch.int32)
+
+
+def _case(seed, new, vocab, drafter, temps, near=0.7, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    n, T = len(new), sum(new)
+    tgt = 2.5 * torch.randn(T + n, vocab + pad, generator=g)
+    rows = [r for s in range(n) for r in range(sum(new[:s]) + s, sum(new[:s]) + s + new[s])]
+    drf = tgt[rows] + near * torch.randn(T, vocab + pad, generator=g)
+    tgt, drf = tgt.to(BF16), drf.to(BF16)
+    temp = torch.tensor([temps[s % len(temps)] for s in range(n)], dtype=torch.float32)
+    seq = [s for s in range(n) for _ in range(new[s])]
+    t = temp[seq].clamp(min=1e-3).unsqueeze(1)
+    noise = -torch.log(-torch.log(torch.rand(T, vocab, generator=g).clamp(1e-20, 1 - 1e-7)))
+    ids = (drf[:, :vocab].float() / t + noise).argmax(1) if T else torch.zeros(0, dtype=torch.int64)
+    return {"tgt": tgt[:, :vocab], "drf": drf[:, :vocab] if drafter else None, "ids": ids, "temp": temp,
+            "u": torch.rand(T, generator=g), "u_last": torch.rand(n, generator=g), "new": new}
+
+
+def _run(c, dev, max_drafts=None):
+    def put(x):  # (a padded row stays padded)
+        if x is None:
+            return None
+        base = torch.empty(x.shape[0], x.stride(0), dtype=x.dtype, device=dev)
+        base[:, :x.shape[1]] = x.to(dev)
+        return base[:, :x.shape[1]]
+    m = max(c["new"]) if max_drafts is None else max_drafts
+    cu = torch.tensor([0] + list(c["new"])).cumsum(0).to(torch.int32).to(dev)
+    tok, acc = _ops().verify_drafts(put(c["tgt"]), c["ids"].to(dev), c["u"].to(dev), c["u_last"].to(dev),
+                                    c["temp"].to(dev), put(c["drf"]), cu_drafts=cu, max_drafts=m)
+    torch.cuda.synchronize()
+    return tok.cpu(), acc.cpu()
+
+
+def _same(c, dev, max_drafts=None):
+    m = max(c["new"]) if max_drafts is None else max_drafts
+    got = _run(c, dev, max_drafts)
+    want = rule(c["tgt"], c["ids"], c["u"], c["u_last"], c["temp"], c["drf"], c["new"], m)
+    assert torch.equal(got[1], want[1]), (got[1], want[1])
+    assert torch.equal(got[0], want[0]), (got[0], want[0])
+    return got
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("new,vocab,temps,pad", [
+    ([1], 1, [1.0], 0),
+    ([0], 7, [0.5], 0),
+    ([4], 32000, [0.8], 0),
+    ([2, 0, 5, 1, 0, 3], 1001, [1.0, 0.0, 0.3], 0),          # rows that are not 16-byte aligned
+    ([3, 1, 2], 2048, [0.7, 1.3], 40),                       # padded rows
+    ([3] * 5, 2049, [1.0], 0),
+    ([1, 5, 3, 2], 128256, [0.6, 1.0, 0.0], 0),
+    ([2] * 70, 3000, [1.0, 0.9, 0.0, 2.0], 0),               # more than 64 sequences
+    ([40, 17, 33], 500, [3.0, 8.0], 3),                      # more drafts than sixteen
+    ([3] * 180, 16500, [0.9], 0),                            # slices of 8192
+])
+def test_tokens_and_counts_equal_the_rule(dev, new, vocab, temps, pad, drafter):
+    for seed in range(3):
+        _same(_case(seed + 10 * vocab, new, vocab, drafter, temps, near=0.3 if max(new) > 10 else 0.7, pad=pad), dev)
+
+
+def test_uniform_form_and_fewer_drafts_than_given(dev):
+    ops = _ops()
+    c = _case(5, [4] * 6, 700, True, [0.9])
+    tok, acc = ops.verify_drafts(c["tgt"].reshape(6, 5, 700).to(dev), c["ids"].view(6, 4).to(dev), c["u"].to(dev),
+                                 c["u_last"].to(dev), c["temp"].to(dev), c["drf"].reshape(6, 4, 700).to(dev))
+    want = _same(c, dev)
+    assert torch.equal(tok.cpu(), want[0]) and torch.equal(acc.cpu(), want[1])
+    _same(c, dev, max_drafts=2)   # later drafts do not count
+    _same(c, dev, max_drafts=0)
+    _same(c, dev, max_drafts=9)   # a wider output
+    tok, acc = ops.verify_drafts(c["tgt"][:6].reshape(6, 1, 700).to(dev), torch.zeros(6, 0, dtype=torch.int64, device=dev),
+                                 torch.zeros(0, device=dev), c["u_last"].to(dev), c["temp"].to(dev))
+    assert tok.shape == (6, 1) and bool((acc == 0).all())
+
+
+def test_greedy_ties_take_the_first(dev):
+    new, V = [3, 2, 1], 5000
+    c = _case(3, new, V, False, [0.0])
+    for r in range(c["tgt"].shape[0]):
+        c["tgt"][r, [100 + r, 4000]] = 30.0
+    c["ids"] = torch.tensor([100, 101, 4000, 104, 105, 100])  # rows 0 1 2 3 | 4 5 6 | 7 8
+    got = _same(c, dev)
+    assert got[1].tolist() == [2, 2, 0]
+
+
+def test_certain_tokens_masked_vocabularies_and_the_ends_of_u(dev):
+    new, V = [2, 2, 2, 2], 3000
+    c = _case(8, new, V, True, [1.0])
+    for r in range(c["tgt"].shape[0]):  # a handful of tokens allowed
+        keep = torch.randperm(V, generator=torch.Generator().manual_seed(r))[:5]
+        m = torch.full((V,), -math.inf, dtype=BF16)
+        m[keep] = c["tgt"][r, keep]
+        c["tgt"][r] = m
+    for u in (0.0, 1 - 2.0 ** -24, 1.0):
+        c["u"][:], c["u_last"][:] = u, u
+        _same(c, dev)
+    # one token allowed: certain, and refused if it is not the draft
+    c["tgt"][:] = -math.inf
+    c["tgt"][:, 17] = 1.0
+    c["ids"][:] = torch.tensor([17, 17, 17, 5, 5, 17, 17, 17])
+    c["u"][:], c["u_last"][:] = 0.5, 0.5
+    c["drf"] = None
+    got = _same(c, dev)
+    assert got[1].tolist() == [2, 1, 0, 2]
+    # drafter and target agree wholly: accepted whatever u is
+    c = _case(9, [3, 3], V, True, [0.7], near=0.0)
+    c["u"][:] = 1 - 2.0 ** -24
+    got = _same(c, dev)
+    assert got[1].tolist() == [3, 3]
+
+
+def test_rows_that_are_no_numbers_and_drafts_outside_the_vocabulary(dev):
+    new, V = [2, 2, 2, 2, 2], 1500
+    c = _case(12, new, V, True, [1.0])
+    c["u"][:] = 0.0  # everything that can be is accepted
+    c["tgt"][1, 700] = -math.nan               # row 1 of sequence 0 (a NaN of either sign)
+    c["tgt"][1, 900] = math.nan
+    c["tgt"][3, [9, 1200]] = math.inf          # row 0 of sequence 1
+    c["tgt"][8] = -math.inf                    # row 2 of sequence 2
+    c["ids"][6] = -1                           # sequence 3
+    c["ids"][9] = V                            # sequence 4
+    got = _same(c, dev)
+    assert got[1].tolist() == [1, 0, 2, 0, 1]
+    assert got[0][0, 1] == 700 and got[0][1, 0] == 9 and got[0][2, 2] == 0
+    c["temp"][:] = 0.0
+    _same(c, dev)
+
+
+def test_drawn_tokens_follow_the_target(dev):
+    """Over 20000 requests of the same two rows the first token (draft or
+    drawn) has the target's distribution whatever the drafter's is: every
+    frequency within 6 standard deviations of p (20 tokens: a chance of 4e-8)."""
+    ops = _ops()
+    n, V = 20000, 20
+    g = torch.Generator().manual_seed(4)
+    t, d = torch.randn(V, generator=g), torch.randn(V, generator=g)
+    for drafter in (True, False):
+        tgt = t.to(BF16).expand(n, 2, V).contiguous().to(dev)
+        drf = d.to(BF16).expand(n, 1, V).contiguous().to(dev)
+        ids = torch.multinomial(_soft(d.to(BF16), 0.8).float(), n, replacement=True, generator=g)
+        u, ul = torch.rand(n, 1, generator=g), torch.rand(n, generator=g)
+        tok, acc = ops.verify_drafts(tgt, ids.view(n, 1).to(dev), u.to(dev), ul.to(dev), torch.full((n,), 0.8, device=dev),
+                                     drf if drafter else None)
+        p = _soft(t.to(BF16), 0.8)
+        f = torch.bincount(tok[:, 0].cpu(), minlength=V).double() / n
+        assert bool(((f - p).abs() <= 6 * torch.sqrt(p * (1 - p) / n)).all())
+        assert 0 < int(acc.sum()) < n
+
+
+def test_captured_call_on_another_stream(dev):
+    ops = _ops()
+    new, V = [3, 1, 4], 32000
+    c = _case(20, new, V, True, [0.9])
+    cu = torch.tensor([0, 3, 4, 8], dtype=torch.int32, device=dev)
+    d = {k: c[k].to(dev) for k in ("tgt", "drf", "ids", "u", "u_last", "temp")}
+
+    def call():
+        return ops.verify_drafts(d["tgt"], d["ids"], d["u"], d["u_last"], d["temp"], d["drf"], cu_drafts=cu, max_drafts=4)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        tok, acc = call()
+    for i in range(4):
+        c = _case(30 + i, new, V, True, [0.9])
+        for k in d:
+            d[k].copy_(c[k])
+        g.replay()
+        torch.cuda.synchronize()
+        want = rule(c["tgt"], c["ids"], c["u"], c["u_last"], c["temp"], c["drf"], new, 4)
+        assert torch.equal(tok.cpu(), want[0]) and torch.equal(acc.cpu(), want[1])
+        eager = call()
+        assert torch.equal(eager[0], tok)
