@@ -456,10 +456,11 @@ int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, con
  * 2^118 / tokens).
  * max_q_len: the most new tokens of a sequence (a hint for speed alone: it
  * chooses between kernels, any value >= 1 gives a right result).
- * workspace: swl_kv4_attention_workspace(nseq, ntok, max_q_len, hq, hkv,
- * max_blocks * block_size) bytes of device memory, 16-byte aligned, owned by
+ * workspace: swl_kv4_attention_workspace(nseq, ntok, cu_seqlens != NULL,
+ * max_q_len, hq, hkv, max_blocks * block_size) bytes of device memory, 16-byte aligned, owned by
  * the call until its kernels have run; its contents do not matter. */
-int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int64_t max_q_len, int hq, int hkv, int64_t max_keys);
+int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int packed, int64_t max_q_len, int hq, int hkv,
+                                    int64_t max_keys);
 int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t ntok, const int32_t* cu_seqlens,
                            int64_t max_q_len, int hq, int hkv, int d, const void* pages, int64_t num_blocks,
                            int block_size, const int32_t* block_table, int64_t max_blocks,

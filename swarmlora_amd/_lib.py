@@ -133,7 +133,7 @@ _SIGS = {
                                     c_int, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "swl_kv4_read_bf16": (c_int, [c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_vp, c_vp,
                                   c_vp]),
-    "swl_kv4_attention_workspace": (c_i64, [c_int, c_i64, c_i64, c_int, c_int, c_i64]),
+    "swl_kv4_attention_workspace": (c_i64, [c_int, c_i64, c_int, c_i64, c_int, c_int, c_i64]),
     "swl_kv4_attention_bf16": (c_int, [c_vp, c_i64, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_i64,
                                        c_int, c_vp, c_i64, c_vp, c_f32, c_vp, c_vp, c_i64, c_vp]),
     "swl_verify_drafts_workspace": (c_i64, [c_int, c_i64, c_i64, c_int]),

@@ -240,24 +240,45 @@ __device__ __forceinline__ SeqInfo seq_info(const Kv4Args& a, int i) {
   return r;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((long long)v, o, 64);
-  return v;
+// Inclusive prefix over the wave's lanes, in six vector instructions (row
+// shifts, then the row ends passed on).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += dpp_i<0x111, 0xF>(v);
+  v += dpp_i<0x112, 0xF>(v);
+  v += dpp_i<0x114, 0xF>(v);
+  v += dpp_i<0x118, 0xF>(v);
+  v += dpp_i<0x142, 0xA>(v);  // row_bcast 15
+  return v + dpp_i<0x143, 0xC>(v);  // row_bcast 31
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  auto add = [&](int x) { v += __int_as_float(x); };
+  add(dpp_i<0x111, 0xF>(__float_as_int(v)));
+  add(dpp_i<0x112, 0xF>(__float_as_int(v)));
+  add(dpp_i<0x114, 0xF>(__float_as_int(v)));
+  add(dpp_i<0x118, 0xF>(__float_as_int(v)));
+  add(dpp_i<0x142, 0xA>(__float_as_int(v)));
+  add(dpp_i<0x143, 0xC>(__float_as_int(v)));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // Steps of a part: as many as cut all blocks' steps into `target` parts (the
 // last one of a block may be shorter), so that there are at most `target` full
-// parts, `target` + blocks units, and 2 `target` records, whatever the lengths.
+// parts, `target` + blocks units, `target` blocks that are cut and 2 `target`
+// records, whatever the lengths.  r: seq_info of the lane's sequence.
 template <int RB, int KS>
-__device__ __forceinline__ int steps_per_part(const Kv4Args& a, int lane) {
-  int64_t sum = 0;
-  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    const SeqInfo r = seq_info<RB, KS>(a, i0 + lane);
-    sum += r.rb * r.steps;
+__device__ __forceinline__ int steps_per_part(const Kv4Args& a, int lane, const SeqInfo& r) {
+  float sum = (float)r.rb * (float)r.steps;
+  for (int i = 64 + lane; i - lane < a.nseq; i += 64) {
+    const SeqInfo x = seq_info<RB, KS>(a, i);
+    sum += (float)x.rb * (float)x.steps;
   }
-  sum = wave_sum(sum) * a.hkv;
-  return (int)max<int64_t>(a.min_spp, (sum + a.target - 1) / a.target);
+  // (rounded up past what the sum's roundings may have lost)
+  const float spp = wave_sum(sum) * (float)a.hkv * 1.0001f / (float)a.target + 1.f;
+  return max(a.min_spp, (int)fminf(spp, 2147483520.f));
 }
 
 struct Unit {
@@ -265,47 +286,48 @@ struct Unit {
   int64_t len, rec;  // rec: the block's first record (where parts > 1)
 };
 
-// COUNT_PARTS: u counts (block, part) pairs, else blocks.
-template <int RB, int KS, bool COUNT_PARTS>
-__device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int spp, int lane, Unit& o) {
-  o.h = (int)(u % a.hkv);
-  const int64_t want = u / a.hkv;
+__device__ __forceinline__ int64_t lane64(int64_t v, int l) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v & 0xffffffff), l) |
+         ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32);
+}
+
+// The unit of a workgroup: u counts (block, part) pairs, or (CUT) the blocks
+// that are cut.
+template <int RB, int KS, bool CUT>
+__device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int lane, int& spp, Unit& o) {
+  SeqInfo r = seq_info<RB, KS>(a, lane);
+  spp = steps_per_part<RB, KS>(a, lane, r);
+  const uint32_t uw = (uint32_t)u / (uint32_t)a.hkv;
+  o.h = (int)((uint32_t)u - uw * (uint32_t)a.hkv);
+  const int64_t want = uw;
   int64_t before = 0, rec = 0;
-  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    const SeqInfo r = seq_info<RB, KS>(a, i0 + lane);
-    const int parts = (int)((r.steps + spp - 1) / spp);
-    const int units = r.rb * parts, mine = COUNT_PARTS ? units : r.rb;
-    const int recs = parts > 1 ? units : 0;
-    int inc = mine, rinc = recs;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(inc, d, 64), z = __shfl_up(rinc, d, 64);
-      if (lane >= d) {
-        inc += y;
-        rinc += z;
-      }
-    }
+  for (int i0 = 0;;) {
+    const int parts = r.steps <= spp ? 1 : (int)((r.steps + spp - 1) / spp);
+    const int units = r.rb * parts, recs = parts > 1 ? units : 0, mine = CUT ? (parts > 1 ? r.rb : 0) : units;
+    const int inc = wave_prefix(mine), rinc = wave_prefix(recs);
     const uint64_t hit = __ballot(before + inc > want);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       o.s = i0 + l;
-      o.parts = __shfl(parts, l, 64);
-      o.t0 = __shfl(r.t0, l, 64);
-      o.n = __shfl(r.n, l, 64);
-      o.len = __shfl((long long)r.len, l, 64);
-      const int rb = __shfl(r.rb, l, 64);
-      const int local = (int)(want - before) - (__shfl(inc, l, 64) - __shfl(mine, l, 64));
-      const int per = COUNT_PARTS ? o.parts : 1;
-      o.b = rb - 1 - local / per;  // the blocks with the most keys first
-      o.p = local % per;
+      o.parts = __builtin_amdgcn_readlane(parts, l);
+      o.t0 = __builtin_amdgcn_readlane(r.t0, l);
+      o.n = __builtin_amdgcn_readlane(r.n, l);
+      o.len = lane64(r.len, l);
+      const int rb = __builtin_amdgcn_readlane(r.rb, l);
+      const int local = (int)(want - before) - __builtin_amdgcn_readlane(inc - mine, l);
+      const int blk = CUT ? local : local / o.parts;
+      o.b = rb - 1 - blk;  // the blocks with the most keys first
+      o.p = CUT ? 0 : local - blk * o.parts;
       if (local < 0 || o.b < 0 || o.p < 0) return false;  // (counts past 32 bits: offsets that are none)
-      o.rec = ((rec + __shfl(rinc - recs, l, 64)) + (int64_t)o.b * o.parts) * a.hkv + o.h;
+      o.rec = (rec + __builtin_amdgcn_readlane(rinc - recs, l) + (int64_t)o.b * o.parts) * a.hkv + o.h;
       return true;
     }
-    before += __shfl(inc, 63, 64);
-    rec += __shfl(rinc, 63, 64);
+    before += __builtin_amdgcn_readlane(inc, 63);
+    rec += __builtin_amdgcn_readlane(rinc, 63);
+    i0 += 64;
+    if (i0 >= a.nseq) return false;
+    r = seq_info<RB, KS>(a, i0 + lane);
   }
-  return false;
 }
 
 // A record: 16 rows as [dim % 8][row-dim slot 256] sums, then the rows' maxima
@@ -454,9 +476,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int spp = steps_per_part<RB, KS>(a, lane);
+  int spp;
   Unit u;
-  if (!find_unit<RB, KS, true>(a, blockIdx.x, spp, lane, u)) return;  // the same for the whole workgroup
+  if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
   const int rows = u.n * a.G, r0 = u.b * RB;
   const int64_t kmax = a.max_blocks * a.tpp * kTile;
   const int64_t ctx_lo = u.len + r0 / a.G + 1;                                 // of the block's first row
@@ -490,10 +512,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
         table = (((int64_t)blk * a.hkv + u.h) * a.tpp + (tile - bi * a.tpp)) * kRec;
     }
   };
-  auto from_lane = [&](int l) {
-    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(table & 0xffffffff), l) |
-           ((int64_t)__builtin_amdgcn_readlane((int)(table >> 32), l) << 32);
-  };
+  auto from_lane = [&](int l) { return lane64(table, l); };
   struct Step {
     u32x4 k[2], v[2];
     uint32_t ks[2], vs[2];
@@ -654,16 +673,263 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
   }
 }
 
+// Many rows (prompts and their chunks): a workgroup of four waves per unit of
+// 128 rows, 32 a wave, all four over the same keys, 64 a step.  Keys go from
+// the pages into every wave's registers as they are stored (the MFMA's 4-bit
+// operand: no conversion, a quarter of bf16's bytes).  Values are made bf16
+// once for the four waves: wave w turns tile w of the step into MFMA operand
+// order and leaves it in LDS for the next step, one barrier a step.  The
+// probabilities enter as one bf16 (2^-9 of each, below the result's own
+// rounding where many keys share the weight; two would add half to the matrix
+// work of PV), and their sum is an MFMA row of ones over the same rounded
+// values, so that the weights sum to 1 exactly.
+constexpr int kPromptRows = 128, kPromptKeys = 64;
+
+__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
+  const uint32_t x = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t y = __float_as_uint(v);
+  auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
+  constexpr int RB = kPromptRows, KS = kPromptKeys;
+  // values of a step: [32-key half][dim % 8][lane] 16 bytes
+  __shared__ __attribute__((aligned(16))) char vb[2][2 * 8 * 1024];
+  __shared__ uint32_t nanf[2][4][64];  // a tile's NaN groups, where some row does not see its keys
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  int spp;
+  Unit u;
+  if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
+  const int rows = u.n * a.G, r0 = u.b * RB, wr0 = r0 + 32 * w;
+  const int64_t kmax = a.max_blocks * a.tpp * kTile;
+  const int64_t ctx_lo = u.len + r0 / a.G + 1;
+  const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
+  const int64_t wend =  // keys that the wave's last row sees
+      wr0 < rows ? min<int64_t>(u.len + (min(wr0 + 32, rows) - 1) / a.G + 1, kmax) : 0;
+  const int64_t wlo = u.len + wr0 / a.G + 1;  // and its first one
+  const int64_t st0 = (int64_t)u.p * spp;
+  const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
+  const int nst = (int)max<int64_t>(0, min<int64_t>(spp, steps - st0));
+  if (nst == 0 && u.p > 0) return;
+
+  QFrag q[2];
+  int64_t ctx[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = min(wr0 + e * 16 + col, rows - 1), tok = r / a.G;
+    q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
+    ctx[e] = u.len + tok + 1;
+  }
+
+  // lane 4 i + t: offset of the record of tile t of step j0 + i (-1: past the
+  // keys, or no page), a table of 16 steps
+  const int32_t* bt = a.bt + (int64_t)u.s * a.max_blocks;
+  int64_t table = -1;
+  auto look = [&](int j) {
+    const int64_t tile = (st0 + j) * 4 + lane;
+    table = -1;
+    if (tile * kTile < kend) {
+      const int64_t bi = tile / a.tpp;
+      const int32_t blk = bt[bi];
+      if (blk >= 0 && blk < a.num_blocks)
+        table = (((int64_t)blk * a.hkv + u.h) * a.tpp + (tile - bi * a.tpp)) * kRec;
+    }
+  };
+  auto from_lane = [&](int l) { return lane64(table, l); };
+  // the next step's keys and this wave's tile of its values, requested a step
+  // ahead
+  u32x4 kn[4], vn;
+  uint32_t ksn[4], vsn, none_n = 0;
+  auto load = [&](int j) {
+    if ((j & 15) == 0) look(j);
+    none_n = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t at = from_lane(4 * (j & 15) + t);
+      none_n |= at < 0 ? 1u << t : 0u;
+      const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
+      kn[t] = ldg16(rec + 64 * col + 16 * g);
+      ksn[t] = ldg_u8(rec + kRecKs + lane);
+    }
+    const int64_t at = from_lane(4 * (j & 15) + w);
+    const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
+    vn = ldg16(rec + kRecV + 16 * lane);
+    vsn = ldg_u32(rec + kRecVs + 16 * g + (col & 12));
+  };
+  // values of step j (in vn) to LDS
+  auto stage = [&](int j) {
+    const int64_t k0 = (st0 + j) * KS;
+    const bool edge = k0 + KS > ctx_lo;
+    if (edge || none_n) {
+      const int live = (int)min<int64_t>(KS, kend - k0);
+      const bool gone = none_n >> w & 1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (gone || 16 * w + 4 * g + k >= live) {
+          vn[k] = 0;
+          vsn = (vsn & ~(0xffu << (8 * k))) | 127u << (8 * k);
+        }
+      uint32_t fl;
+      take_nan(vn, vsn, fl);
+      nanf[j & 1][w][lane] = fl;
+    }
+    uint32_t f[8][2];
+    v_pairs(vn, vsn, f);
+    char* dst = vb[j & 1] + (w >> 1) * 8192 + lane * 16 + (w & 1) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) *reinterpret_cast<u32x2*>(dst + e * 1024) = u32x2{f[e][0], f[e][1]};
+  };
+
+  const float c2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
+  const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  float m[2] = {-INFINITY, -INFINITY};
+  f32x4 acc[2][8], l[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    l[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  u32x4 kc[4];
+  uint32_t ksc[4], none = 0;
+  auto take = [&]() {
+    none = none_n;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      kc[t] = kn[t];
+      ksc[t] = ksn[t];
+    }
+  };
+  if (nst > 0) {
+    load(0);
+    stage(0);
+    take();
+    lds_barrier();
+  }
+  for (int j = 0; j < nst; ++j) {
+    const int64_t k0 = (st0 + j) * KS;
+    if (j + 1 < nst) load(j + 1);
+    const char* vp = vb[j & 1] + lane * 16;
+    if (k0 < wend) {
+      const bool edge = k0 + KS > wlo || none;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        f32x4 sv[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) sv[e][t] = scores(kc[2 * hf + t], (int)ksc[2 * hf + t], q[e]);
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int see = (int)min<int64_t>(KS, ctx[e] - k0) - 32 * hf;  // keys of the half that the row sees
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if ((none >> (2 * hf + t) & 1) || 16 * t + 4 * g + k >= see) sv[e][t][k] = -INFINITY;
+          }
+        }
+        float mx[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
+                        fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3])));
+          mx[e] = max_groups(mx[e]) * c2;
+        }
+        if (__ballot(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) != 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mn = fmaxf(m[e], mx[e]);
+            const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
+            m[e] = mn;
+            l[e] *= corr;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
+          }
+        }
+        u32x4 p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mr = m[e] == -INFINITY ? 0.f : m[e];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const f32x4& y = sv[e][k >> 1];
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1)], c2, -mr));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr));
+            p[e][k] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0), f2bf(p1)});
+          }
+          l[e] = mfma16(ones, p[e], l[e]);
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const u32x4 f = *reinterpret_cast<const u32x4*>(vp + hf * 8192 + d * 1024);
+          acc[0][d] = mfma16(f, p[0], acc[0][d]);
+          acc[1][d] = mfma16(f, p[1], acc[1][d]);
+        }
+      }
+      if (k0 + KS > ctx_lo || none) {  // (as `stage` decided: the flags are there)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint32_t fl[2] = {nanf[j & 1][2 * hf][lane], nanf[j & 1][2 * hf + 1][lane]};
+          if (__ballot((fl[0] | fl[1]) != 0) == 0) continue;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (sees_nan(fl, (int)min<int64_t>(KS, ctx[e] - k0) - 32 * hf, g))
+#pragma unroll
+              for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
+        }
+      }
+    }
+    if (j + 1 < nst) {
+      stage(j + 1);
+      take();
+    }
+    lds_barrier();  // the next step's values are there, and this one's read by all
+  }
+
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = wr0 + e * 16 + col;
+    if (r >= rows) continue;
+    if (u.parts == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float o[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] = acc[e][d][i];
+        write_row(a, u, r, (g * 16 + col) * 4 + i, l[e][0], o);
+      }
+    } else {
+      const int64_t at = u.rec + (int64_t)u.p * a.hkv;
+      if (at >= a.max_rec) continue;  // (only where offsets overlap)
+      float* rec = a.part + (at * (RB / 16) + 2 * w + e) * kRecF;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(rec + d * 256 + lane * 4) = acc[e][d];
+      if (g == 0) {
+        rec[2048 + col] = m[e];
+        rec[2064 + col] = l[e][0];
+      }
+    }
+  }
+}
+
 // Merges the parts of 16 rows of a block that was cut: a workgroup per (block,
 // kv head, set of 16 rows), thread (g, row, i) as above, parts in order.
 template <int RB, int KS>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
   constexpr int SETS = RB / 16;
   const int lane = threadIdx.x & 63;
-  const int spp = steps_per_part<RB, KS>(a, lane);
   const int e = blockIdx.x % SETS;
+  int spp;
   Unit u;
-  if (!find_unit<RB, KS, false>(a, blockIdx.x / SETS, spp, lane, u) || u.parts == 1) return;
+  if (!find_unit<RB, KS, true>(a, blockIdx.x / SETS, lane, spp, u)) return;
   const int rows = u.n * a.G, row = threadIdx.x >> 2 & 15, r = u.b * RB + e * 16 + row;
   // the block's own parts: its last row may see fewer keys than the sequence's
   const int64_t kend = min<int64_t>(u.len + (min((u.b + 1) * RB, rows) - 1) / a.G + 1, a.max_blocks * a.tpp * kTile);
@@ -698,25 +964,77 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
 
 // ------------------------------------------------------------- launchers ---
 // Geometry of one attention call, from shapes alone: bounds that hold for
-// every set of lengths (steps_per_part).
-struct Kv4Plan {
-  int sets, rb, target, min_spp;
-  int64_t blocks, units, recs;
+// every set of lengths (steps_per_part).  Sequences of at most kSplitRows rows
+// go to the kernel for few rows, the others to the one for many; a call whose
+// hint says that there are none of the others leaves them all to the first.
+struct Kv4Launch {
+  bool on;
+  int rb, target, min_spp, row_lo, row_hi;
+  int64_t blocks, units, recs, bytes;
 };
-constexpr int kMinSteps = 8;  // steps of 32 keys of a part, at least
+struct Kv4Plan {
+  Kv4Launch few, many;
+};
+constexpr int kSplitRows = 64;
 
-Kv4Plan kv4_plan(int64_t nseq, int64_t T, int64_t max_q_len, int hq, int hkv, int64_t max_keys) {
+Kv4Launch kv4_launch(int64_t nseq, int64_t T, int G, int hkv, int64_t max_keys, int64_t max_rows, int rb, int ks,
+                     int target, int min_spp) {
+  Kv4Launch p{};
+  p.on = true;
+  p.rb = rb;
+  p.target = target;
+  p.min_spp = min_spp;
+  p.row_hi = 0x7fffffff;
+  p.blocks = std::min({T * ((G + rb - 1) / rb), T * G / rb + nseq, nseq * ((max_rows + rb - 1) / rb)}) * hkv;
+  const int64_t most = std::max<int64_t>(1, ((max_keys + ks - 1) / ks + min_spp - 1) / min_spp);
+  p.units = std::min<int64_t>(p.blocks * most, p.blocks + target);
+  p.recs = most > 1 ? std::min<int64_t>(p.blocks * most, 2 * target) : 0;
+  p.bytes = p.recs * (rb / 16) * kRecF * (int64_t)sizeof(float);
+  return p;
+}
+
+Kv4Plan kv4_plan(int64_t nseq, int64_t T, bool packed, int64_t max_q_len, int hq, int hkv, int64_t max_keys) {
   Kv4Plan p{};
   const int G = hq / hkv;
-  p.sets = max_q_len * G <= 16 ? 1 : 2;
-  p.rb = 16 * p.sets;
-  p.target = 1024;
-  p.min_spp = kMinSteps;
-  p.blocks = std::min<int64_t>(T * G, T * G / p.rb + nseq) * hkv;
-  const int64_t most = std::max<int64_t>(1, ((max_keys + 31) / 32 + p.min_spp - 1) / p.min_spp);
-  p.units = std::min<int64_t>(p.blocks * most, p.blocks + p.target);
-  p.recs = most > 1 ? std::min<int64_t>(p.blocks * most, 2 * p.target) : 0;
+  const int64_t most = std::min(max_q_len, T) * G;
+  if (most <= kSplitRows || packed)  // (a packed call's hint may be too small: its rows are bounded by T alone)
+    p.few = kv4_launch(nseq, T, G, hkv, max_keys, most > kSplitRows ? kSplitRows : packed ? T * G : most,
+                       most <= 16 ? 16 : 32, 32, 1024, 8);
+  if (most > kSplitRows) {
+    p.many = kv4_launch(nseq, T, G, hkv, max_keys, T * G, kPromptRows, kPromptKeys, 512, 8);
+    p.few.row_hi = p.many.row_lo = packed ? kSplitRows : 0;
+  }
   return p;
+}
+
+int kv4_launch_combine(const Kv4Args& a, const Kv4Launch& p, hipStream_t st) {
+  if (p.recs == 0) return SWL_OK;
+  const dim3 grid((unsigned)(std::min<int64_t>(p.blocks, p.target) * (p.rb / 16)));
+  switch (p.rb) {
+    case 16: hipLaunchKernelGGL((kv4_combine_kernel<16, 32>), grid, dim3(256), 0, st, a); break;
+    case 32: hipLaunchKernelGGL((kv4_combine_kernel<32, 32>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((kv4_combine_kernel<kPromptRows, kPromptKeys>), grid, dim3(256), 0, st, a); break;
+  }
+  SWL_LAUNCH_CHECK("kv4_combine_kernel launch");
+  return SWL_OK;
+}
+
+int kv4_launch_attention(Kv4Args a, const Kv4Launch& p, void* ws, hipStream_t st) {
+  if (!p.on) return SWL_OK;
+  a.part = reinterpret_cast<float*>(ws);
+  a.max_rec = p.recs;
+  a.target = p.target;
+  a.min_spp = p.min_spp;
+  a.row_lo = p.row_lo;
+  a.row_hi = p.row_hi;
+  const dim3 grid((unsigned)p.units);
+  switch (p.rb) {
+    case 16: hipLaunchKernelGGL(kv4_split_kernel<1>, grid, dim3(64 * kSplitWaves), 0, st, a); break;
+    case 32: hipLaunchKernelGGL(kv4_split_kernel<2>, grid, dim3(64 * kSplitWaves), 0, st, a); break;
+    default: hipLaunchKernelGGL(kv4_prompt_kernel, grid, dim3(256), 0, st, a); break;
+  }
+  SWL_LAUNCH_CHECK("kv4 attention launch");
+  return kv4_launch_combine(a, p, st);
 }
 
 int kv4_check_pages(const char* what, const void* pages, int64_t num_blocks, int block_size,
@@ -821,11 +1139,11 @@ extern "C" int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int bloc
   return SWL_OK;
 }
 
-extern "C" int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int64_t max_q_len, int hq, int hkv,
+extern "C" int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int packed, int64_t max_q_len, int hq, int hkv,
                                                int64_t max_keys) {
-  if (nseq <= 0 || ntok <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0) return 0;
-  const Kv4Plan p = kv4_plan(nseq, ntok, std::min(max_q_len, ntok), hq, hkv, max_keys);
-  return p.recs * p.sets * kRecF * (int64_t)sizeof(float);
+  if (nseq <= 0 || ntok <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_keys <= 0 || max_q_len <= 0) return 0;
+  const Kv4Plan p = kv4_plan(nseq, ntok, packed != 0, max_q_len, hq, hkv, max_keys);
+  return p.few.bytes + p.many.bytes;
 }
 
 extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t ntok,
@@ -856,29 +1174,14 @@ extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq,
   a.G = hq / hkv;
   a.scale = softmax_scale;
   a.out = reinterpret_cast<bf16*>(out);
-  const Kv4Plan p = kv4_plan(nseq, ntok, std::min(max_q_len, ntok), hq, hkv, max_blocks * block_size);
-  SWL_CHECK(p.units < ((int64_t)1 << 31), SWL_ERR_INVALID, "swl_kv4_attention_bf16: too many rows");
-  SWL_CHECK(p.recs == 0 || (workspace && aligned16(workspace) &&
-                            workspace_bytes >= p.recs * p.sets * kRecF * (int64_t)sizeof(float)),
-            SWL_ERR_INVALID, "swl_kv4_attention_bf16: workspace smaller than swl_kv4_attention_workspace");
-  a.part = reinterpret_cast<float*>(workspace);
-  a.max_rec = p.recs;
-  a.target = p.target;
-  a.min_spp = p.min_spp;
-  a.row_lo = 0;
-  a.row_hi = 0x7fffffff;
-  hipStream_t st = (hipStream_t)stream;
-  if (p.sets == 1)
-    hipLaunchKernelGGL(kv4_split_kernel<1>, dim3((unsigned)p.units), dim3(64 * kSplitWaves), 0, st, a);
-  else
-    hipLaunchKernelGGL(kv4_split_kernel<2>, dim3((unsigned)p.units), dim3(64 * kSplitWaves), 0, st, a);
-  SWL_LAUNCH_CHECK("kv4_split_kernel launch");
-  if (p.recs == 0) return SWL_OK;
-  const dim3 grid((unsigned)(p.blocks * p.sets));
-  if (p.sets == 1)
-    hipLaunchKernelGGL((kv4_combine_kernel<16, 32>), grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((kv4_combine_kernel<32, 32>), grid, dim3(256), 0, st, a);
-  SWL_LAUNCH_CHECK("kv4_combine_kernel launch");
-  return SWL_OK;
+  if (!cu_seqlens) max_q_len = ntok / nseq;
+  const Kv4Plan p = kv4_plan(nseq, ntok, cu_seqlens != nullptr, max_q_len, hq, hkv, max_blocks * block_size);
+  SWL_CHECK(p.few.units < ((int64_t)1 << 31) && p.many.units < ((int64_t)1 << 31), SWL_ERR_INVALID,
+            "swl_kv4_attention_bf16: too many rows");
+  const int64_t need = p.few.bytes + p.many.bytes;
+  SWL_CHECK(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), SWL_ERR_INVALID,
+            "swl_kv4_attention_bf16: workspace smaller than swl_kv4_attention_workspace");
+  rc = kv4_launch_attention(a, p.few, workspace, (hipStream_t)stream);
+  if (rc) return rc;
+  return kv4_launch_attention(a, p.many, reinterpret_cast<char*>(workspace) + p.few.bytes, (hipStream_t)stream);
 }

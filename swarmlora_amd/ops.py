@@ -1031,7 +1031,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     _same_device(q, out)
     lib = _lib.load()
     bs = pages.shape[2] * 16
-    need = lib.swl_kv4_attention_workspace(nseq, ntok, max_q_len, hq, hkv, block_table.shape[1] * bs)
+    need = lib.swl_kv4_attention_workspace(nseq, ntok, 0 if cu_seqlens is None else 1, max_q_len, hq, hkv,
+                                           block_table.shape[1] * bs)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.check(lib.swl_kv4_attention_bf16(
         _ptr(q), qs, nseq, ntok, _ptr(cu_seqlens), max_q_len, hq, hkv, 128, _ptr(pages), pages.shape[0], bs,

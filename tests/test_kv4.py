@@ -19,11 +19,11 @@ def test_record_size_and_workspace():
     from swarmlora_amd import ops
     lib = _lib().load()
     assert lib.swl_kv4_record_bytes() == ops.KV4_RECORD == _kv4.REC
-    assert lib.swl_kv4_attention_workspace(0, 0, 1, 8, 2, 64) == 0
+    assert lib.swl_kv4_attention_workspace(0, 0, 0, 1, 8, 2, 64) == 0
     # a table of at most one part needs none; a long one does, bounded whatever its length
-    assert lib.swl_kv4_attention_workspace(4, 4, 1, 32, 8, 16) == 0
-    big = lib.swl_kv4_attention_workspace(28, 28, 1, 32, 8, 1 << 20)
-    assert 0 < big == lib.swl_kv4_attention_workspace(28, 28, 1, 32, 8, 1 << 24) < 1 << 28
+    assert lib.swl_kv4_attention_workspace(4, 4, 0, 1, 32, 8, 16) == 0
+    big = lib.swl_kv4_attention_workspace(28, 28, 1, 1, 32, 8, 1 << 20)
+    assert 0 < big == lib.swl_kv4_attention_workspace(28, 28, 1, 1, 32, 8, 1 << 24) < 1 << 28
 
 
 P = 4096  # a pointer that is never followed: the checks come first

@@ -228,6 +228,8 @@ ATTEND = [  # ctx, new, hq, hkv, page
     ([40, 300], [1, 1], 7, 1, 48),                            # seven heads a kv head
     ([100, 80], [1, 1], 3, 3, 32),                            # a head each
     ([64, 900], [1, 1], 40, 2, 16),                           # twenty heads a kv head
+    ([30, 500], [1, 1], 40, 1, 16),                           # forty, and seventy: a token's rows in several blocks
+    ([30, 500], [1, 2], 70, 1, 16),
     ([12, 700, 0, 90], [3, 5, 2, 0], 32, 8, 16),              # drafted tokens, an empty sequence
     ([1500, 0, 33], [8, 1, 4], 16, 4, 32),
     ([0, 0, 0], [1, 70, 129], 8, 2, 16),                      # prompts
