@@ -19,6 +19,7 @@
 #include <stdint.h>
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dev_util.h"
 #include "swl.h"
@@ -381,28 +382,46 @@ __device__ __forceinline__ QFrag q_frag(const bf16* row, int g) {
 }
 
 // scores of a 16-key tile (key 4 (lane / 16) + i) with 16 rows (lane % 16)
-__device__ __forceinline__ f32x4 scores(u32x4 k, int ks, const QFrag& q) {
+__device__ __forceinline__ f32x4 qk_hi(u32x4 k, int ks, const QFrag& q) {
   const i32x8 A = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  f32x4 c = {0.f, 0.f, 0.f, 0.f};
-  c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, q.hi, c, 4, 0, 0, ks, 0, q.sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, q.hi, f32x4{0.f, 0.f, 0.f, 0.f}, 4, 0, 0, ks, 0, q.sb);
+}
+__device__ __forceinline__ f32x4 qk_lo(u32x4 k, int ks, const QFrag& q, f32x4 c) {
+  const i32x8 A = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, q.lo, c, 4, 0, 0, ks, 0, q.sb - 4);
 }
+__device__ __forceinline__ f32x4 scores(u32x4 k, int ks, const QFrag& q) { return qk_lo(k, ks, q, qk_hi(k, ks, q)); }
 
 // A lane's dwords of a tile's values (8 dims of four tokens) as pairs of
-// tokens: f[e][0], f[e][1] = tokens (0, 1), (2, 3) of dim e.
+// tokens: f[e][0], f[e][1] = tokens (0, 1), (2, 3) of dim 2 J + e.
+template <int J>
+__device__ __forceinline__ void v_pair(u32x4 v, uint32_t vs, uint32_t (&f)[2][2]) {
+  const uint32_t w0 = pair_bf16<J>(v[0], __uint_as_float((vs & 0xffu) << 23));
+  const uint32_t w1 = pair_bf16<J>(v[1], __uint_as_float((vs >> 8 & 0xffu) << 23));
+  const uint32_t w2 = pair_bf16<J>(v[2], __uint_as_float((vs >> 16 & 0xffu) << 23));
+  const uint32_t w3 = pair_bf16<J>(v[3], __uint_as_float((vs >> 24) << 23));
+  f[0][0] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+  f[0][1] = __builtin_amdgcn_perm(w3, w2, 0x05040100u);
+  f[1][0] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+  f[1][1] = __builtin_amdgcn_perm(w3, w2, 0x07060302u);
+}
+// All eight dims: f[e] of dim e.
 __device__ __forceinline__ void v_pairs(u32x4 v, uint32_t vs, uint32_t (&f)[8][2]) {
-  const float s0 = __uint_as_float((vs & 0xffu) << 23), s1 = __uint_as_float((vs >> 8 & 0xffu) << 23);
-  const float s2 = __uint_as_float((vs >> 16 & 0xffu) << 23), s3 = __uint_as_float((vs >> 24) << 23);
-  auto put = [&](int e, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-    f[e][0] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-    f[e][1] = __builtin_amdgcn_perm(w3, w2, 0x05040100u);
-    f[e + 1][0] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
-    f[e + 1][1] = __builtin_amdgcn_perm(w3, w2, 0x07060302u);
+  auto put = [&](int e, const uint32_t (&x)[2][2]) {
+    f[e][0] = x[0][0];
+    f[e][1] = x[0][1];
+    f[e + 1][0] = x[1][0];
+    f[e + 1][1] = x[1][1];
   };
-  put(0, pair_bf16<0>(v[0], s0), pair_bf16<0>(v[1], s1), pair_bf16<0>(v[2], s2), pair_bf16<0>(v[3], s3));
-  put(2, pair_bf16<1>(v[0], s0), pair_bf16<1>(v[1], s1), pair_bf16<1>(v[2], s2), pair_bf16<1>(v[3], s3));
-  put(4, pair_bf16<2>(v[0], s0), pair_bf16<2>(v[1], s1), pair_bf16<2>(v[2], s2), pair_bf16<2>(v[3], s3));
-  put(6, pair_bf16<3>(v[0], s0), pair_bf16<3>(v[1], s1), pair_bf16<3>(v[2], s2), pair_bf16<3>(v[3], s3));
+  uint32_t x[2][2];
+  v_pair<0>(v, vs, x);
+  put(0, x);
+  v_pair<1>(v, vs, x);
+  put(2, x);
+  v_pair<2>(v, vs, x);
+  put(4, x);
+  v_pair<3>(v, vs, x);
+  put(6, x);
 }
 
 __device__ __forceinline__ uint32_t ldg_u8(const uint8_t* p) {
@@ -683,6 +702,13 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
 // rounding where many keys share the weight; two would add half to the matrix
 // work of PV), and their sum is an MFMA row of ones over the same rounded
 // values, so that the weights sum to 1 exactly.
+//
+// Exponents are taken from the row's largest score of its first 32 keys, and
+// no maximum is kept after that: a reference too low makes all terms larger by
+// one factor, which the quotient does not see, until a term passes the largest
+// number.  That, an infinity or NaN, or a row without a key in its first 32
+// leaves sums outside [2^-60, 2^100); the unit is then done again with a
+// running maximum.
 constexpr int kPromptRows = 128, kPromptKeys = 64;
 
 __device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
@@ -699,6 +725,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   // values of a step: [32-key half][dim % 8][lane] 16 bytes
   __shared__ __attribute__((aligned(16))) char vb[2][2 * 8 * 1024];
   __shared__ uint32_t nanf[2][4][64];  // a tile's NaN groups, where some row does not see its keys
+  __shared__ uint32_t again[4];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -707,70 +734,68 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
   const int rows = u.n * a.G, r0 = u.b * RB, wr0 = r0 + 32 * w;
   const int64_t kmax = a.max_blocks * a.tpp * kTile;
-  const int64_t ctx_lo = u.len + r0 / a.G + 1;
+  const int64_t ctx_lo = u.len + r0 / a.G + 1;  // of the block's first row
   const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
-  const int64_t wend =  // keys that the wave's last row sees
-      wr0 < rows ? min<int64_t>(u.len + (min(wr0 + 32, rows) - 1) / a.G + 1, kmax) : 0;
-  const int64_t wlo = u.len + wr0 / a.G + 1;  // and its first one
   const int64_t st0 = (int64_t)u.p * spp;
   const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
   const int nst = (int)max<int64_t>(0, min<int64_t>(spp, steps - st0));
   if (nst == 0 && u.p > 0) return;
 
   QFrag q[2];
-  int64_t ctx[2];
+  int ctx[2];  // keys that the lane's rows see, from the part's first step
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = min(wr0 + e * 16 + col, rows - 1), tok = r / a.G;
     q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
-    ctx[e] = u.len + tok + 1;
+    ctx[e] = (int)min<int64_t>(max<int64_t>(u.len + tok + 1 - st0 * KS, 0), (int64_t)nst * KS);
   }
+  const int all_see = (int)min<int64_t>(max<int64_t>(ctx_lo - st0 * KS, 0), (int64_t)nst * KS);  // by every row
+  const int live = (int)min<int64_t>(max<int64_t>(kend - st0 * KS, 0), (int64_t)nst * KS);       // by any
 
-  // lane 4 i + t: offset of the record of tile t of step j0 + i (-1: past the
-  // keys, or no page), a table of 16 steps
+  // lane 4 i + t: address of the record of tile t of step j0 + i (the first
+  // record's where it is past the keys or has no page: `gone` tells), a table of
+  // 16 steps; the pages of the next 16 are requested when a table is made
   const int32_t* bt = a.bt + (int64_t)u.s * a.max_blocks;
-  int64_t table = -1;
+  int64_t table = 0;
+  uint64_t gone = 0;
+  int32_t blk_next = -1;
+  auto request = [&](int j) {
+    const uint32_t tile = (uint32_t)(st0 + j) * 4 + lane;  // (fewer than 2^26)
+    blk_next = (int64_t)tile * kTile < kend ? bt[tile / (uint32_t)a.tpp] : -1;
+  };
   auto look = [&](int j) {
-    const int64_t tile = (st0 + j) * 4 + lane;
-    table = -1;
-    if (tile * kTile < kend) {
-      const int64_t bi = tile / a.tpp;
-      const int32_t blk = bt[bi];
-      if (blk >= 0 && blk < a.num_blocks)
-        table = (((int64_t)blk * a.hkv + u.h) * a.tpp + (tile - bi * a.tpp)) * kRec;
-    }
+    const uint32_t tile = (uint32_t)(st0 + j) * 4 + lane;
+    const bool there = blk_next >= 0 && blk_next < a.num_blocks;
+    gone = __ballot(!there);
+    table = (int64_t)a.pages +
+            (there ? (((int64_t)blk_next * a.hkv + u.h) * a.tpp + tile % (uint32_t)a.tpp) * kRec : 0);
+    request(j + 16);
   };
-  auto from_lane = [&](int l) { return lane64(table, l); };
-  // the next step's keys and this wave's tile of its values, requested a step
-  // ahead
-  u32x4 kn[4], vn;
-  uint32_t ksn[4], vsn, none_n = 0;
-  auto load = [&](int j) {
-    if ((j & 15) == 0) look(j);
-    none_n = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t at = from_lane(4 * (j & 15) + t);
-      none_n |= at < 0 ? 1u << t : 0u;
-      const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
-      kn[t] = ldg16(rec + 64 * col + 16 * g);
-      ksn[t] = ldg_u8(rec + kRecKs + lane);
-    }
-    const int64_t at = from_lane(4 * (j & 15) + w);
-    const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
-    vn = ldg16(rec + kRecV + 16 * lane);
-    vsn = ldg_u32(rec + kRecVs + 16 * g + (col & 12));
+  auto tile_at = [&](int j, int t) { return reinterpret_cast<const uint8_t*>(lane64(table, 4 * (j & 15) + t)); };
+  auto missing = [&](int j) { return (uint32_t)(gone >> (4 * (j & 15))) & 15u; };  // bit t: tile t is not there
+  uint32_t koff = 64 * col + 16 * g, soff = lane, voff = 16 * lane, xoff = 16 * g + (col & 12);
+  u32x4 kc[4], vn;
+  uint32_t ks[4], vsn;
+  // (scalar base, 32-bit lane offset: the offsets are kept from being widened
+  // once, outside the loop, which costs a 64-bit addition per load)
+  auto load_k = [&](int j, int t) {
+    const uint8_t* rec = tile_at(j, t);
+    asm("" : "+v"(koff), "+v"(soff));
+    kc[t] = ldg16(rec + koff);
+    ks[t] = ldg_u8(rec + soff + kRecKs);
   };
-  // values of step j (in vn) to LDS
-  auto stage = [&](int j) {
-    const int64_t k0 = (st0 + j) * KS;
-    const bool edge = k0 + KS > ctx_lo;
-    if (edge || none_n) {
-      const int live = (int)min<int64_t>(KS, kend - k0);
-      const bool gone = none_n >> w & 1;
+  auto load_v = [&](int j) {
+    const uint8_t* rec = tile_at(j, w);
+    asm("" : "+v"(voff), "+v"(xoff));
+    vn = ldg16(rec + voff + kRecV);
+    vsn = ldg_u32(rec + xoff + kRecVs);
+  };
+  // values of step j (in vn) to LDS; none: its missing tiles
+  auto clean = [&](int j, uint32_t none) {
+    if ((j + 1) * KS > all_see || none) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (gone || 16 * w + 4 * g + k >= live) {
+        if ((none >> w & 1) || j * KS + 16 * w + 4 * g + k >= live) {  // what is stored there is anything
           vn[k] = 0;
           vsn = (vsn & ~(0xffu << (8 * k))) | 127u << (8 * k);
         }
@@ -778,6 +803,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
       take_nan(vn, vsn, fl);
       nanf[j & 1][w][lane] = fl;
     }
+  };
+  auto stage = [&](int j) {
     uint32_t f[8][2];
     v_pairs(vn, vsn, f);
     char* dst = vb[j & 1] + (w >> 1) * 8192 + lane * 16 + (w & 1) * 8;
@@ -787,134 +814,214 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
 
   const float c2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
   const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-  float m[2] = {-INFINITY, -INFINITY};
+  float m[2];
   f32x4 acc[2][8], l[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  bool nan_v[2];  // the row sees a NaN group of the lane's dims
 
-  u32x4 kc[4];
-  uint32_t ksc[4], none = 0;
-  auto take = [&]() {
-    none = none_n;
+  auto pass = [&](auto running) {
+    constexpr bool RUNNING = decltype(running)::value;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      kc[t] = kn[t];
-      ksc[t] = ksn[t];
+    for (int e = 0; e < 2; ++e) {
+      m[e] = -INFINITY;
+      nan_v[e] = false;
+      l[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  };
-  if (nst > 0) {
-    load(0);
+    if (nst == 0) return;
+    // scores of tiles t0, t0 + 1 of step j (none: its missing tiles)
+    f32x4 sv[2][2];
+    auto qk = [&](f32x4 (&s)[2][2], int t0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[e][t] = scores(kc[t0 + t], (int)ks[t0 + t], q[e]);
+    };
+    auto mask = [&](f32x4 (&s)[2][2], int j, int t0, uint32_t none) {
+      if ((j + 1) * KS <= all_see && none == 0) return;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int see = ctx[e] - j * KS - 16 * t0 - 4 * g;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((none >> (t0 + t) & 1) || 16 * t + k >= see) s[e][t][k] = -INFINITY;
+      }
+    };
+    auto top = [&](int e) {
+      return max_groups(fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
+                              fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3])))) * c2;
+    };
+    request(0);
+    look(0);
+    uint32_t none = missing(0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load_k(0, t);
+    load_v(0);
+    clean(0, none);
     stage(0);
-    take();
+    qk(sv, 0);
+    mask(sv, 0, 0, none);
+    load_k(1, 0);
+    load_k(1, 1);
+    if constexpr (!RUNNING) {
+      m[0] = top(0);
+      m[1] = top(1);
+    }
+    float mr[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
     lds_barrier();
-  }
-  for (int j = 0; j < nst; ++j) {
-    const int64_t k0 = (st0 + j) * KS;
-    if (j + 1 < nst) load(j + 1);
-    const char* vp = vb[j & 1] + lane * 16;
-    if (k0 < wend) {
-      const bool edge = k0 + KS > wlo || none;
+    for (int j = 0; j < nst; ++j) {
+      const uint32_t none_next = missing(j + 1);
+      const char* vp = vb[j & 1] + lane * 16;
+      load_v(j + 1);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        f32x4 sv[2][2];
+        if constexpr (RUNNING) {
+          const float mx[2] = {top(0), top(1)};
+          if (__ballot(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) != 0) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float mn = fmaxf(m[e], mx[e]);
+              const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
+              m[e] = mn;
+              l[e] *= corr;
+#pragma unroll
+              for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
+              mr[e] = mn == -INFINITY ? 0.f : mn;
+            }
+          }
+        }
+        if (hf == 1) {
+          clean(j + 1, none_next);
+          if (((j + 2) & 15) == 0) look(j + 2);
+        }
+        // One block without branches: the half's values from LDS, the next
+        // half's scores beside this one's exponentials, then PV beside the next
+        // step's values.  The order is held by scheduling barriers: left to
+        // itself the compiler puts all exponentials before the matrix
+        // instructions, and one wave's matrix and vector units take turns.
+        u32x4 vf[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) vf[d] = *reinterpret_cast<const u32x4*>(vp + hf * 8192 + d * 1024);
+        f32x4 sn[2][2];
+        u32x4 p[2];
+        __builtin_amdgcn_sched_barrier(0);
+        float x0 = 0.f, x1 = 0.f;  // exponentials of the pair before, rounded while the next are on their way
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = i >> 1 & 1, t = i & 1, kt = 2 - 2 * hf + t;
+          sn[e][t] = i < 4 ? qk_hi(kc[kt], (int)ks[kt], q[e]) : qk_lo(kc[kt], (int)ks[kt], q[e], sn[e][t]);
+          __builtin_amdgcn_sched_barrier(0);
+          const int pe = i >> 2, k = i & 3;
+          const f32x4& y = sv[pe][k >> 1];
+          const float y0 = __builtin_fmaf(y[2 * (k & 1)], c2, -mr[pe]);
+          const float y1 = __builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr[pe]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i > 0) p[(i - 1) >> 2][(i - 1) & 3] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(x0), f2bf(x1)});
+          x0 = __builtin_amdgcn_exp2f(y0);
+          x1 = __builtin_amdgcn_exp2f(y1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        p[1][3] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(x0), f2bf(x1)});
+        const int jn = hf == 0 ? j + 1 : j + 2;
+        load_k(jn, 2 - 2 * hf);
+        load_k(jn, 3 - 2 * hf);
+        char* dst = vb[(j + 1) & 1] + (w >> 1) * 8192 + lane * 16 + (w & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          acc[0][d] = mfma16(vf[d], p[0], acc[0][d]);
+          acc[1][d] = mfma16(vf[d], p[1], acc[1][d]);
+          if (hf == 1 && (d & 1) == 0) {
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t f[2][2];
+            switch (d) {
+              case 0: v_pair<0>(vn, vsn, f); break;
+              case 2: v_pair<1>(vn, vsn, f); break;
+              case 4: v_pair<2>(vn, vsn, f); break;
+              default: v_pair<3>(vn, vsn, f); break;
+            }
+            *reinterpret_cast<u32x2*>(dst + d * 1024) = u32x2{f[0][0], f[0][1]};
+            *reinterpret_cast<u32x2*>(dst + (d + 1) * 1024) = u32x2{f[1][0], f[1][1]};
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[e] = mfma16(ones, p[e], l[e]);
+        if (hf == 0)
+          mask(sn, j, 2, none);
+        else
+          mask(sn, j + 1, 0, none_next);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) sv[e][t] = scores(kc[2 * hf + t], (int)ksc[2 * hf + t], q[e]);
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int see = (int)min<int64_t>(KS, ctx[e] - k0) - 32 * hf;  // keys of the half that the row sees
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if ((none >> (2 * hf + t) & 1) || 16 * t + 4 * g + k >= see) sv[e][t][k] = -INFINITY;
-          }
-        }
-        float mx[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
-                        fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3])));
-          mx[e] = max_groups(mx[e]) * c2;
-        }
-        if (__ballot(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f) != 0) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[e], mx[e]);
-            const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
-            m[e] = mn;
-            l[e] *= corr;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
-          }
-        }
-        u32x4 p[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mr = m[e] == -INFINITY ? 0.f : m[e];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const f32x4& y = sv[e][k >> 1];
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1)], c2, -mr));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr));
-            p[e][k] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0), f2bf(p1)});
-          }
-          l[e] = mfma16(ones, p[e], l[e]);
-        }
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const u32x4 f = *reinterpret_cast<const u32x4*>(vp + hf * 8192 + d * 1024);
-          acc[0][d] = mfma16(f, p[0], acc[0][d]);
-          acc[1][d] = mfma16(f, p[1], acc[1][d]);
-        }
+          for (int t = 0; t < 2; ++t) sv[e][t] = sn[e][t];
       }
-      if (k0 + KS > ctx_lo || none) {  // (as `stage` decided: the flags are there)
+      if ((j + 1) * KS > all_see || none) {  // (as `clean` decided: the flags are there)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const uint32_t fl[2] = {nanf[j & 1][2 * hf][lane], nanf[j & 1][2 * hf + 1][lane]};
           if (__ballot((fl[0] | fl[1]) != 0) == 0) continue;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (sees_nan(fl, (int)min<int64_t>(KS, ctx[e] - k0) - 32 * hf, g))
-#pragma unroll
-              for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
+          for (int e = 0; e < 2; ++e) nan_v[e] |= sees_nan(fl, ctx[e] - j * KS - 32 * hf, g);
         }
       }
+      none = none_next;
+      lds_barrier();  // the next step's values are there, and this one's read by all
     }
-    if (j + 1 < nst) {
-      stage(j + 1);
-      take();
-    }
-    lds_barrier();  // the next step's values are there, and this one's read by all
+  };
+  pass(std::false_type{});
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    bad |= !(l[e][0] >= 0x1p-60f && l[e][0] < 0x1p100f);
+    float t = 0.f;  // (a NaN or an infinity stays one)
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t = fmaxf(t, fabsf(acc[e][d][i])) + 0.f * acc[e][d][i];
+    bad |= !(t < INFINITY);
+  }
+  const bool any = __ballot(bad) != 0;
+  if (lane == 0) again[w] = any ? 1 : 0;
+  __syncthreads();
+  if (again[0] | again[1] | again[2] | again[3]) {  // the same for the whole workgroup
+    __syncthreads();
+    pass(std::true_type{});
   }
 
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = wr0 + e * 16 + col;
     if (r >= rows) continue;
+    // sums to [1, 2): their reference may be far from the largest score
+    float L = l[e][0], f = 1.f;
+    if (nan_v[e])
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
+    if (L > 0.f && L < INFINITY) {
+      const int x = (int)(__float_as_uint(L) >> 23) - 127;  // (L >= 2^-60, or >= 1 with a running maximum)
+      f = __uint_as_float((uint32_t)(127 - x) << 23);
+      L *= f;
+      m[e] += (float)x;
+    }
     if (u.parts == 1) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float o[8];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d] = acc[e][d][i];
-        write_row(a, u, r, (g * 16 + col) * 4 + i, l[e][0], o);
+        for (int d = 0; d < 8; ++d) o[d] = acc[e][d][i] * f;
+        write_row(a, u, r, (g * 16 + col) * 4 + i, L, o);
       }
     } else {
       const int64_t at = u.rec + (int64_t)u.p * a.hkv;
       if (at >= a.max_rec) continue;  // (only where offsets overlap)
       float* rec = a.part + (at * (RB / 16) + 2 * w + e) * kRecF;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(rec + d * 256 + lane * 4) = acc[e][d];
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(rec + d * 256 + lane * 4) = acc[e][d] * f;
       if (g == 0) {
         rec[2048 + col] = m[e];
-        rec[2064 + col] = l[e][0];
+        rec[2064 + col] = L;
       }
     }
   }
@@ -1046,7 +1153,7 @@ int kv4_check_pages(const char* what, const void* pages, int64_t num_blocks, int
   if (block_size < 16 || block_size % 16 != 0 || block_size > (1 << 20))
     return bad("block_size must be a multiple of 16");
   if (num_blocks < 1 || num_blocks >= ((int64_t)1 << 31) || max_blocks < 1 ||
-      max_blocks > ((int64_t)1 << 31) / block_size)
+      max_blocks > ((int64_t)1 << 30) / block_size)
     return bad("bad page geometry");
   if (nseq == 0 || T == 0) return SWL_OK;
   if (!pages || !block_table || !cache_seqlens) return bad("null argument");
