@@ -50,9 +50,9 @@ struct Kv4Args {
   int32_t nseq, L, hq, hkv, G;
   int32_t tpp;              // tiles of a page
   float scale;
-  // attention: records of parts, and how many parts are wanted
+  // attention: records of parts; workgroups that run at once
   float* part;
-  int32_t target, min_spp, row_lo, row_hi;
+  int32_t slots, min_spp, row_lo, row_hi;
   int64_t max_rec;
 };
 
@@ -216,8 +216,8 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
 // units (sequence, kv head, block of RB rows, part of the keys); every wave
 // finds its unit by itself from the lengths (a scan over the sequences, 64 at
 // a time), so that the host knows none of them and a captured call follows
-// them.  A part is `spp` steps of KS keys, as many as make about `target`
-// units of the whole call, so that units are equally long whatever the
+// them.  A part is `spp` steps of KS keys, as many as make the whole call's
+// units fit the GPU at once, so that units are equally long whatever the
 // lengths are.  A block of one part writes its rows; others leave a record per
 // part, merged by kv4_combine_kernel.
 struct SeqInfo {
@@ -266,20 +266,39 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Steps of a part: as many as cut all blocks' steps into `target` parts (the
-// last one of a block may be shorter), so that there are at most `target` full
-// parts, `target` + blocks units, `target` blocks that are cut and 2 `target`
-// records, whatever the lengths.  r: seq_info of the lane's sequence.
+// Steps of a part: the fewest (at least min_spp) that cut the call into no more
+// units than `slots`, the workgroups that run at once: a second round of a few
+// units costs as much as a whole one (28 sequences with drafted tokens, 736
+// units for 512 places 42.6 us, 496 units 34.8).  With as many blocks as
+// places, or more sequences than a wave's lanes, the steps are shared out
+// evenly instead.  Either way a part is at least steps / slots, so that there
+// are at most `slots` full parts, `slots` + blocks units, `slots` blocks that
+// are cut and 2 `slots` records, whatever the lengths.  r: seq_info of the
+// lane's sequence.
 template <int RB, int KS>
 __device__ __forceinline__ int steps_per_part(const Kv4Args& a, int lane, const SeqInfo& r) {
-  float sum = (float)r.rb * (float)r.steps;
+  const float mine = (float)r.rb * (float)a.hkv, st = (float)r.steps;
+  float sum = mine * st;
   for (int i = 64 + lane; i - lane < a.nseq; i += 64) {
     const SeqInfo x = seq_info<RB, KS>(a, i);
-    sum += (float)x.rb * (float)x.steps;
+    sum += (float)x.rb * (float)a.hkv * (float)x.steps;
   }
   // (rounded up past what the sum's roundings may have lost)
-  const float spp = wave_sum(sum) * (float)a.hkv * 1.0001f / (float)a.target + 1.f;
-  return max(a.min_spp, (int)fminf(spp, 2147483520.f));
+  const float slots = (float)a.slots, all = wave_sum(sum) * 1.0001f;
+  int lo = max(a.min_spp, (int)fminf(all / slots + 1.f, 1073741824.f));
+  if (a.nseq > 64) return lo;
+  auto units = [&](int spp) { return wave_sum(mine * ceilf(st / (float)spp)); };
+  const float blocks = wave_sum(mine);
+  if (blocks >= slots || units(lo) <= slots) return lo;
+  int hi = max(lo, (int)fminf(all / (slots - blocks) + 1.f, 1073741824.f));  // enough: a block has under one part more
+  while (hi - lo > max(1, lo >> 4)) {
+    const int mid = (lo + hi) >> 1;
+    if (units(mid) <= slots)
+      hi = mid;
+    else
+      lo = mid;
+  }
+  return hi;
 }
 
 struct Unit {
@@ -431,6 +450,15 @@ __device__ __forceinline__ uint32_t ldg_u32(const uint8_t* p) {
   return *(const __attribute__((address_space(1))) uint32_t*)(p);
 }
 
+__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
+  const uint32_t x = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t y = __float_as_uint(v);
+  auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // Takes the NaN groups out of a tile's values where some row does not see
 // their token (0 times a NaN is one); flags gets 0xff in the bytes of theirs.
 __device__ __forceinline__ void take_nan(u32x4& v, uint32_t& vs, uint32_t& flags) {
@@ -480,16 +508,16 @@ __device__ __forceinline__ void write_row(const Kv4Args& a, const Unit& u, int r
 
 // Few rows, many keys (single and drafted tokens): a workgroup of four waves
 // per unit of 16 SETS rows; wave w takes the part's steps of 32 keys (two
-// tiles) w, w + 4, ... on its own, loading each step's operands straight from
-// the pages into registers one step ahead; the waves' results meet in LDS.
-// S^T = K Q^T (scaled MFMA, keys as stored) leaves in a lane the keys 4 g .. +
-// 3 of both tiles of its row, which is the B operand of O^T = V^T P^T as it
-// is.  The probabilities enter as two bf16 (2^-17 of them unaccounted): the
-// matrix units idle here, the cache's bytes are the bound.
+// tiles) w, w + 4, ... on its own, the operands straight from the pages into
+// registers, each requested anew as soon as it has been used; the waves'
+// results meet in LDS.  S^T = K Q^T (scaled MFMA, keys as stored) leaves in a
+// lane the keys 4 g .. + 3 of both tiles of its row, which is the B operand of
+// O^T = V^T P^T as it is.  The probabilities enter as one bf16 and are summed as
+// they are, as in the kernel for many rows.
 constexpr int kSplitWaves = 4;
 
 template <int SETS>
-__global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split_kernel(Kv4Args a) {
+__global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split_kernel(Kv4Args a) {
   constexpr int RB = 16 * SETS, KS = 32, W = kSplitWaves;
   __shared__ __attribute__((aligned(16))) float mg[W][kRecF];
   const int lane = threadIdx.x & 63;
@@ -500,7 +528,6 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
   if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
   const int rows = u.n * a.G, r0 = u.b * RB;
   const int64_t kmax = a.max_blocks * a.tpp * kTile;
-  const int64_t ctx_lo = u.len + r0 / a.G + 1;                                 // of the block's first row
   const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
   const int64_t st0 = (int64_t)u.p * spp;                                      // the part's first step
   const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
@@ -508,163 +535,190 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
   if (nst == 0 && u.p > 0) return;  // (the longest row's part; this block's end before it)
   const int nw = nst > w ? (nst - w + W - 1) / W : 0;  // this wave's steps: st0 + w + j W
 
+  // lane 2 i + t: address of the record of tile t of this wave's step j0 + i
+  // (the first record's where it is past the keys or has no page: `gone`
+  // tells), a table of 32 steps; the pages of the next 32 are requested when a
+  // table is made
+  const int32_t* bt = a.bt + (int64_t)u.s * a.max_blocks;
+  int64_t table = 0;
+  uint64_t gone = 0;
+  int32_t blk_next = -1;
+  auto tile_of_lane = [&](int j) { return ((uint32_t)st0 + w + (j + (lane >> 1)) * W) * 2 + (lane & 1); };
+  auto request = [&](int j) {
+    const uint32_t tile = tile_of_lane(j);
+    blk_next = (int64_t)tile * kTile < kend ? bt[tile / (uint32_t)a.tpp] : -1;
+  };
+  auto look = [&](int j) {
+    const bool there = blk_next >= 0 && blk_next < a.num_blocks;
+    gone = __ballot(!there);
+    table = (int64_t)a.pages + (there ? (((int64_t)blk_next * a.hkv + u.h) * a.tpp +
+                                         tile_of_lane(j) % (uint32_t)a.tpp) * kRec : 0);
+    request(j + 32);
+  };
+  request(0);
+
   QFrag q[SETS];
-  int64_t ctx[SETS];
+  int ctx[SETS];  // keys that the lane's rows see, from the part's first step
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
     const int r = min(r0 + e * 16 + col, rows - 1), tok = r / a.G;
     q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
-    ctx[e] = u.len + tok + 1;
+    ctx[e] = (int)min<int64_t>(max<int64_t>(u.len + tok + 1 - st0 * KS, 0), (int64_t)nst * KS);
   }
+  const int all_see = (int)min<int64_t>(max<int64_t>(u.len + r0 / a.G + 1 - st0 * KS, 0), (int64_t)nst * KS);
+  const int live = (int)min<int64_t>(max<int64_t>(kend - st0 * KS, 0), (int64_t)nst * KS);
 
-  // lane 2 i + t: offset of the record of tile t of this wave's step j0 + i
-  // (-1: past the keys, or no page), a table of 32 steps
-  const int32_t* bt = a.bt + (int64_t)u.s * a.max_blocks;
-  int64_t table = -1;
-  auto look = [&](int j) {
-    const int64_t tile = (st0 + w + (int64_t)(j + (lane >> 1)) * W) * 2 + (lane & 1);
-    table = -1;
-    if (tile * kTile < kend) {
-      const int64_t bi = tile / a.tpp;
-      const int32_t blk = bt[bi];
-      if (blk >= 0 && blk < a.num_blocks)
-        table = (((int64_t)blk * a.hkv + u.h) * a.tpp + (tile - bi * a.tpp)) * kRec;
-    }
-  };
-  auto from_lane = [&](int l) { return lane64(table, l); };
-  struct Step {
-    u32x4 k[2], v[2];
-    uint32_t ks[2], vs[2];
-    uint32_t none;  // bit t: tile t is not there
-  };
-  auto load = [&](int j) {
-    Step x;
-    if ((j & 31) == 0) look(j);
-    x.none = 0;
+  auto tile_at = [&](int j, int t) { return reinterpret_cast<const uint8_t*>(lane64(table, 2 * (j & 31) + t)); };
+  uint32_t koff = 64 * col + 16 * g, soff = lane, voff = 16 * lane, xoff = 16 * g + (col & 12);
+  u32x4 kc[2], vc[2];
+  uint32_t ks[2], vs[2];
+  auto load_k = [&](int j) {
+    asm("" : "+v"(koff), "+v"(soff));  // (a scalar base and a 32-bit offset: not widened outside the loop)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int64_t at = from_lane(2 * (j & 31) + t);
-      x.none |= at < 0 ? 1u << t : 0u;
-      const uint8_t* rec = a.pages + (at < 0 ? 0 : at);
-      x.k[t] = ldg16_nt(rec + 64 * col + 16 * g);
-      x.v[t] = ldg16_nt(rec + kRecV + 16 * lane);
-      x.ks[t] = ldg_u8(rec + kRecKs + lane);
-      x.vs[t] = ldg_u32(rec + kRecVs + 16 * g + (col & 12));
+      const uint8_t* rec = tile_at(j, t);
+      kc[t] = ldg16_nt(rec + koff);
+      ks[t] = ldg_u8(rec + soff + kRecKs);
     }
-    return x;
+  };
+  auto load_v = [&](int j) {
+    asm("" : "+v"(voff), "+v"(xoff));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* rec = tile_at(j, t);
+      vc[t] = ldg16_nt(rec + voff + kRecV);
+      vs[t] = ldg_u32(rec + xoff + kRecVs);
+    }
   };
 
   const float c2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
-  float m[SETS], l[SETS];
-  f32x4 acc[SETS][8];
+  const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  float m[SETS];
+  bool nan_v[SETS];  // the row sees a NaN group of the lane's dims
+  f32x4 acc[SETS][8], l[SETS];
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
     m[e] = -INFINITY;
-    l[e] = 0.f;
+    nan_v[e] = false;
+    l[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  Step x;
-  if (nw > 0) x = load(0);
-  for (int j = 0; j < nw; ++j) {
-    Step nx;
-    if (j + 1 < nw) nx = load(j + 1);
-    const int64_t k0 = (st0 + w + (int64_t)j * W) * KS;
-    f32x4 sv[SETS][2];
+  look(0);
+  load_k(0);
+  load_v(0);
+  auto walk = [&](auto sets) {  // the wave's steps, for the sets that have rows
+    constexpr int NS = decltype(sets)::value;
+    for (int j = 0; j < nw; ++j) {
+      const int k0 = (w + j * W) * KS;  // from the part's first step
+      const uint32_t none = (uint32_t)(gone >> (2 * (j & 31))) & 3u;  // bit t: tile t is not there
+      // a row of the block ends inside the step, or a tile is missing
+      const bool edge = k0 + KS > all_see || none;
+      f32x4 sv[NS][2];
 #pragma unroll
-    for (int e = 0; e < SETS; ++e)
+      for (int e = 0; e < NS; ++e)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) sv[e][t] = scores(x.k[t], (int)x.ks[t], q[e]);
-    // a row of the block ends inside the step, or a tile is missing
-    uint32_t nan_v[2] = {0, 0};  // scales of NaN groups, taken out of the values
-    if (k0 + KS > ctx_lo || x.none) {
-      const int live = (int)min<int64_t>(KS, kend - k0);
+        for (int t = 0; t < 2; ++t) sv[e][t] = scores(kc[t], (int)ks[t], q[e]);
+      if (edge) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bool gone = x.none >> t & 1;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (gone || 16 * t + 4 * g + k >= live) {  // what is stored there is anything: 0 times a NaN is one
-            x.v[t][k] = 0;
-            x.vs[t] = (x.vs[t] & ~(0xffu << (8 * k))) | 127u << (8 * k);
-          }
-        take_nan(x.v[t], x.vs[t], nan_v[t]);
-#pragma unroll
-        for (int e = 0; e < SETS; ++e) {
-          const int see = (int)min<int64_t>(KS, ctx[e] - k0);  // keys of the step that the row sees
+        for (int t = 0; t < 2; ++t) {
+          const bool no = none >> t & 1;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (gone || 16 * t + 4 * g + k >= see) sv[e][t][k] = -INFINITY;
+            if (no || k0 + 16 * t + 4 * g + k >= live) {  // what is stored there is anything: 0 times a NaN is one
+              vc[t][k] = 0;
+              vs[t] = (vs[t] & ~(0xffu << (8 * k))) | 127u << (8 * k);
+            }
+#pragma unroll
+          for (int e = 0; e < NS; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (no || k0 + 16 * t + 4 * g + k >= ctx[e]) sv[e][t][k] = -INFINITY;
+        }
+        uint32_t fl[2];  // NaN groups
+        take_nan(vc[0], vs[0], fl[0]);
+        take_nan(vc[1], vs[1], fl[1]);
+        if (__ballot((fl[0] | fl[1]) != 0) != 0) {
+#pragma unroll
+          for (int e = 0; e < NS; ++e) nan_v[e] |= sees_nan(fl, ctx[e] - k0, g);
         }
       }
-    }
-    uint32_t vf[2][8][2];
-    v_pairs(x.v[0], x.vs[0], vf[0]);
-    v_pairs(x.v[1], x.vs[1], vf[1]);
+      if (((j + 1) & 31) == 0) look(j + 1);
+      load_k(j + 1);  // (past the last step: the first record, or one of the next part's)
+      u32x4 p[NS];
 #pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      float mx = fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
-                       fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3])));
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
-      // the reference the exponents are taken from moves only when the maximum
-      // has grown by 2^8 since: any reference gives the same quotient
-      if (__ballot(mx > m[e] + 8.f) != 0) {
-        const float mn = fmaxf(m[e], mx);
-        const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
-        m[e] = mn;
-        l[e] *= corr;
+      for (int e = 0; e < NS; ++e) {
+        const float mx = c2 * max_groups(fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
+                                               fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3]))));
+        // the reference the exponents are taken from moves only when the maximum
+        // has grown by 2^8 since: any reference gives the same quotient
+        if (__ballot(mx > m[e] + 8.f) != 0) {
+          const float mn = fmaxf(m[e], mx);
+          const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
+          m[e] = mn;
+          l[e] *= corr;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
+          for (int d = 0; d < 8; ++d) acc[e][d] *= corr;
+        }
+        const float mr = m[e] == -INFINITY ? 0.f : m[e];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // tokens in pairs: one conversion for both
+          const f32x4& y = sv[e][k >> 1];
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1)], c2, -mr));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr));
+          p[e][k] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0), f2bf(p1)});
+        }
+        l[e] = mfma16(ones, p[e], l[e]);
       }
-      const float mr = m[e] == -INFINITY ? 0.f : m[e];
-      u32x4 ph, pl;
+      auto pv = [&](int d, const uint32_t (&f0)[2][2], const uint32_t (&f1)[2][2]) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {  // tokens in pairs: one conversion for both
-        const f32x4& y = sv[e][k >> 1];
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1)], c2, -mr));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (k & 1) + 1], c2, -mr));
-        l[e] += p0;
-        l[e] += p1;
-        const uint32_t hi = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0), f2bf(p1)});
-        ph[k] = hi;
-        pl[k] = __builtin_bit_cast(uint32_t, (bf16x2){f2bf(p0 - __uint_as_float(hi << 16)),
-                                                      f2bf(p1 - __uint_as_float(hi & 0xffff0000u))});
-      }
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const u32x4 f = u32x4{vf[0][d][0], vf[0][d][1], vf[1][d][0], vf[1][d][1]};
-        acc[e][d] = mfma16(f, ph, acc[e][d]);
-        acc[e][d] = mfma16(f, pl, acc[e][d]);
-      }
+          for (int e = 0; e < NS; ++e)
+            acc[e][d + x] = mfma16(u32x4{f0[x][0], f0[x][1], f1[x][0], f1[x][1]}, p[e], acc[e][d + x]);
+      };
+      uint32_t f0[2][2], f1[2][2];
+      v_pair<0>(vc[0], vs[0], f0);
+      v_pair<0>(vc[1], vs[1], f1);
+      pv(0, f0, f1);
+      v_pair<1>(vc[0], vs[0], f0);
+      v_pair<1>(vc[1], vs[1], f1);
+      pv(2, f0, f1);
+      v_pair<2>(vc[0], vs[0], f0);
+      v_pair<2>(vc[1], vs[1], f1);
+      pv(4, f0, f1);
+      v_pair<3>(vc[0], vs[0], f0);
+      v_pair<3>(vc[1], vs[1], f1);
+      load_v(j + 1);
+      pv(6, f0, f1);
     }
-    if (__ballot((nan_v[0] | nan_v[1]) != 0) != 0) {
-#pragma unroll
-      for (int e = 0; e < SETS; ++e)
-        if (sees_nan(nan_v, (int)min<int64_t>(KS, ctx[e] - k0), g))
-#pragma unroll
-          for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
-    }
-    x = nx;
-  }
+  };
+  if (SETS > 1 && rows - r0 <= 16)
+    walk(std::integral_constant<int, 1>{});
+  else
+    walk(std::integral_constant<int, SETS>{});
 
-  // the row sums over the four lane groups, then the waves' results in LDS;
-  // thread = (g, row, i): dims 32 g + 8 i .. + 7
+  // the waves' results in LDS, rows that there are; thread = (g, row, i): dims
+  // 32 g + 8 i .. + 7
   const int row = threadIdx.x >> 2 & 15;
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
-    l[e] += __shfl_xor(l[e], 16, 64);
-    l[e] += __shfl_xor(l[e], 32, 64);
-    if (e > 0) __syncthreads();
+    const int nr = rows - r0 - 16 * e;
+    if (e > 0) {
+      if (nr <= 0) return;  // the same for the whole workgroup
+      __syncthreads();
+    }
+    if (col < nr) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(&mg[w][d * 256 + lane * 4]) = acc[e][d];
-    if (g == 0) {
-      mg[w][2048 + col] = m[e];
-      mg[w][2064 + col] = l[e];
+      for (int d = 0; d < 8; ++d)
+        *reinterpret_cast<f32x4*>(&mg[w][d * 256 + lane * 4]) = nan_v[e] ? f32x4{NAN, NAN, NAN, NAN} : acc[e][d];
+      if (g == 0) {
+        mg[w][2048 + col] = m[e];
+        mg[w][2064 + col] = l[e][0];
+      }
     }
     __syncthreads();
-    const int r = r0 + e * 16 + row;
+    if (row >= nr) continue;
     float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < W; ++v) M = fmaxf(M, mg[v][2048 + row]);
@@ -675,9 +729,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[d] += mg[v][d * 256 + threadIdx.x] * f;
     }
-    if (r >= rows) continue;
     if (u.parts == 1) {
-      write_row(a, u, r, threadIdx.x, L, o);
+      write_row(a, u, r0 + e * 16 + row, threadIdx.x, L, o);
     } else {
       const int64_t at = u.rec + (int64_t)u.p * a.hkv;
       if (at >= a.max_rec) continue;  // (only where offsets overlap)
@@ -710,15 +763,6 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 3 : 2) void kv4_split
 // leaves sums outside [2^-60, 2^100); the unit is then done again with a
 // running maximum.
 constexpr int kPromptRows = 128, kPromptKeys = 64;
-
-__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
-  const uint32_t x = __float_as_uint(v);
-  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const uint32_t y = __float_as_uint(v);
-  auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
 
 __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   constexpr int RB = kPromptRows, KS = kPromptKeys;
@@ -1076,26 +1120,30 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
 // hint says that there are none of the others leaves them all to the first.
 struct Kv4Launch {
   bool on;
-  int rb, target, min_spp, row_lo, row_hi;
+  int rb, slots, min_spp, row_lo, row_hi;
   int64_t blocks, units, recs, bytes;
 };
 struct Kv4Plan {
   Kv4Launch few, many;
 };
 constexpr int kSplitRows = 64;
+constexpr int kCus = 256;  // of an MI355X
+// Workgroups of a CU (registers), and steps of a part at least (16 of 32 keys:
+// four a wave; 28 single tokens over 128 to 2048 keys with 8: 21.8 us, 16: 17)
+constexpr int kSplit1PerCu = 4, kSplit2PerCu = 2, kPromptPerCu = 2, kSplitSteps = 16, kPromptSteps = 8;
 
 Kv4Launch kv4_launch(int64_t nseq, int64_t T, int G, int hkv, int64_t max_keys, int64_t max_rows, int rb, int ks,
-                     int target, int min_spp) {
+                     int per_cu, int min_spp) {
   Kv4Launch p{};
   p.on = true;
   p.rb = rb;
-  p.target = target;
+  p.slots = per_cu * kCus;
   p.min_spp = min_spp;
   p.row_hi = 0x7fffffff;
   p.blocks = std::min({T * ((G + rb - 1) / rb), T * G / rb + nseq, nseq * ((max_rows + rb - 1) / rb)}) * hkv;
   const int64_t most = std::max<int64_t>(1, ((max_keys + ks - 1) / ks + min_spp - 1) / min_spp);
-  p.units = std::min<int64_t>(p.blocks * most, p.blocks + target);
-  p.recs = most > 1 ? std::min<int64_t>(p.blocks * most, 2 * target) : 0;
+  p.units = std::min<int64_t>(p.blocks * most, p.blocks + p.slots);
+  p.recs = most > 1 ? std::min<int64_t>(p.blocks * most, 2 * p.slots) : 0;
   p.bytes = p.recs * (rb / 16) * kRecF * (int64_t)sizeof(float);
   return p;
 }
@@ -1106,9 +1154,9 @@ Kv4Plan kv4_plan(int64_t nseq, int64_t T, bool packed, int64_t max_q_len, int hq
   const int64_t most = std::min(max_q_len, T) * G;
   if (most <= kSplitRows || packed)  // (a packed call's hint may be too small: its rows are bounded by T alone)
     p.few = kv4_launch(nseq, T, G, hkv, max_keys, most > kSplitRows ? kSplitRows : packed ? T * G : most,
-                       most <= 16 ? 16 : 32, 32, 1024, 8);
+                       most <= 16 ? 16 : 32, 32, most <= 16 ? kSplit1PerCu : kSplit2PerCu, kSplitSteps);
   if (most > kSplitRows) {
-    p.many = kv4_launch(nseq, T, G, hkv, max_keys, T * G, kPromptRows, kPromptKeys, 512, 8);
+    p.many = kv4_launch(nseq, T, G, hkv, max_keys, T * G, kPromptRows, kPromptKeys, kPromptPerCu, kPromptSteps);
     p.few.row_hi = p.many.row_lo = packed ? kSplitRows : 0;
   }
   return p;
@@ -1116,7 +1164,7 @@ Kv4Plan kv4_plan(int64_t nseq, int64_t T, bool packed, int64_t max_q_len, int hq
 
 int kv4_launch_combine(const Kv4Args& a, const Kv4Launch& p, hipStream_t st) {
   if (p.recs == 0) return SWL_OK;
-  const dim3 grid((unsigned)(std::min<int64_t>(p.blocks, p.target) * (p.rb / 16)));
+  const dim3 grid((unsigned)(std::min<int64_t>(p.blocks, p.slots) * (p.rb / 16)));
   switch (p.rb) {
     case 16: hipLaunchKernelGGL((kv4_combine_kernel<16, 32>), grid, dim3(256), 0, st, a); break;
     case 32: hipLaunchKernelGGL((kv4_combine_kernel<32, 32>), grid, dim3(256), 0, st, a); break;
@@ -1130,7 +1178,7 @@ int kv4_launch_attention(Kv4Args a, const Kv4Launch& p, void* ws, hipStream_t st
   if (!p.on) return SWL_OK;
   a.part = reinterpret_cast<float*>(ws);
   a.max_rec = p.recs;
-  a.target = p.target;
+  a.slots = p.slots;
   a.min_spp = p.min_spp;
   a.row_lo = p.row_lo;
   a.row_hi = p.row_hi;
