@@ -32,6 +32,23 @@ constexpr int kTile = 16;        // tokens of a record
 constexpr int kRec = 17 * kD;    // bytes of a record
 constexpr int kRecV = 1024, kRecKs = 2048, kRecVs = 2112;
 
+// Division by a number that the host knows, for dividends under 2^31.
+struct FastDiv {
+  uint32_t d, mul, shift;  // mul 0: d is 1
+};
+FastDiv fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  if (d > 1) {
+    const int s = 32 - __builtin_clz(d - 1);  // 2^s >= d
+    f.mul = (uint32_t)((((uint64_t)1 << (31 + s)) / d) + 1);
+    f.shift = (uint32_t)(s - 1);
+  }
+  return f;
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv& f) {
+  return f.mul ? __umulhi(n, f.mul) >> f.shift : n;
+}
+
 struct Kv4Args {
   const bf16* q;            // [T, hq, 128], token stride qs
   const bf16* k;            // append: [T, hkv, 128]
@@ -47,8 +64,10 @@ struct Kv4Args {
   bf16* out2;               // read: values
   int64_t num_blocks, max_blocks, max_pos;
   int64_t T;
+  int32_t kmax;             // keys of a table
   int32_t nseq, L, hq, hkv, G;
   int32_t tpp;              // tiles of a page
+  FastDiv by_g, by_hkv, by_tpp;
   float scale;
   // attention: records of parts; workgroups that run at once
   float* part;
@@ -222,7 +241,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
 // part, merged by kv4_combine_kernel.
 struct SeqInfo {
   int t0, n, rb;
-  int64_t len, steps;  // steps of the longest row
+  int len, steps;  // steps of the longest row
 };
 
 template <int RB, int KS>
@@ -231,13 +250,13 @@ __device__ __forceinline__ SeqInfo seq_info(const Kv4Args& a, int i) {
   if (i >= a.nseq) return r;
   r.t0 = a.cu ? a.cu[i] : i * a.L;
   r.n = a.cu ? a.cu[i + 1] - r.t0 : a.L;
-  r.len = a.seqlens[i];
+  r.len = min(a.seqlens[i], 1 << 30);  // (tables end at 2^30)
   if (r.t0 < 0 || r.n < 0 || (int64_t)r.t0 + r.n > a.T) r.n = 0;  // offsets that are none
-  const int64_t rows = (int64_t)r.n * a.G;
+  const int rows = r.n * a.G;
   if (rows <= a.row_lo || rows > a.row_hi) return r;
-  r.rb = (int)((rows + RB - 1) / RB);
-  const int64_t kend = min<int64_t>(max<int64_t>(r.len + r.n, 0), a.max_blocks * a.tpp * kTile);
-  r.steps = max<int64_t>((kend + KS - 1) / KS, 1);
+  r.rb = (int)((uint32_t)(rows + RB - 1) / RB);
+  const int kend = (int)min<int64_t>(max<int64_t>((int64_t)r.len + r.n, 0), a.kmax);
+  r.steps = max((kend + KS - 1) / KS, 1);
   return r;
 }
 
@@ -302,9 +321,18 @@ __device__ __forceinline__ int steps_per_part(const Kv4Args& a, int lane, const 
 }
 
 struct Unit {
-  int s, h, b, p, parts, t0, n;
-  int64_t len, rec;  // rec: the block's first record (where parts > 1)
+  int s, h, b, p, parts, t0, n, len;
+  int64_t rec;  // the block's first record (where parts > 1)
 };
+
+// ceil(n / d) for n >= 1 by a float reciprocal, off by one at most before it is
+// put right (quotients under 2^22)
+__device__ __forceinline__ int ceil_div(int n, int d, float inv) {
+  int q = (int)((float)(n - 1) * inv);
+  const int r = n - 1 - q * d;
+  q += r >= d ? 1 : r < 0 ? -1 : 0;
+  return q + 1;
+}
 
 __device__ __forceinline__ int64_t lane64(int64_t v, int l) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v & 0xffffffff), l) |
@@ -317,12 +345,14 @@ template <int RB, int KS, bool CUT>
 __device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int lane, int& spp, Unit& o) {
   SeqInfo r = seq_info<RB, KS>(a, lane);
   spp = steps_per_part<RB, KS>(a, lane, r);
-  const uint32_t uw = (uint32_t)u / (uint32_t)a.hkv;
+  const uint32_t uw = (uint32_t)u / a.by_hkv;
   o.h = (int)((uint32_t)u - uw * (uint32_t)a.hkv);
-  const int64_t want = uw;
-  int64_t before = 0, rec = 0;
+  const float inv = 1.f / (float)spp;
+  const int want = (int)uw;
+  int before = 0;
+  int64_t rec = 0;
   for (int i0 = 0;;) {
-    const int parts = r.steps <= spp ? 1 : (int)((r.steps + spp - 1) / spp);
+    const int parts = ceil_div(max(r.steps, 1), spp, inv);
     const int units = r.rb * parts, recs = parts > 1 ? units : 0, mine = CUT ? (parts > 1 ? r.rb : 0) : units;
     const int inc = wave_prefix(mine), rinc = wave_prefix(recs);
     const uint64_t hit = __ballot(before + inc > want);
@@ -332,14 +362,14 @@ __device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int lane,
       o.parts = __builtin_amdgcn_readlane(parts, l);
       o.t0 = __builtin_amdgcn_readlane(r.t0, l);
       o.n = __builtin_amdgcn_readlane(r.n, l);
-      o.len = lane64(r.len, l);
+      o.len = __builtin_amdgcn_readlane(r.len, l);
       const int rb = __builtin_amdgcn_readlane(r.rb, l);
-      const int local = (int)(want - before) - __builtin_amdgcn_readlane(inc - mine, l);
-      const int blk = CUT ? local : local / o.parts;
+      const int local = want - before - __builtin_amdgcn_readlane(inc - mine, l);
+      const int blk = CUT || o.parts == 1 ? local : local / o.parts;
       o.b = rb - 1 - blk;  // the blocks with the most keys first
       o.p = CUT ? 0 : local - blk * o.parts;
       if (local < 0 || o.b < 0 || o.p < 0) return false;  // (counts past 32 bits: offsets that are none)
-      o.rec = (rec + __builtin_amdgcn_readlane(rinc - recs, l) + (int64_t)o.b * o.parts) * a.hkv + o.h;
+      o.rec = (int64_t)(rec + __builtin_amdgcn_readlane(rinc - recs, l) + (int64_t)o.b * o.parts) * a.hkv + o.h;
       return true;
     }
     before += __builtin_amdgcn_readlane(inc, 63);
@@ -348,6 +378,11 @@ __device__ __forceinline__ bool find_unit(const Kv4Args& a, int64_t u, int lane,
     if (i0 >= a.nseq) return false;
     r = seq_info<RB, KS>(a, i0 + lane);
   }
+}
+
+// Keys that row r of the unit's sequence sees.
+__device__ __forceinline__ int last_key(const Kv4Args& a, const Unit& u, int r) {
+  return min(max(u.len + (int)((uint32_t)r / a.by_g) + 1, 0), a.kmax);
 }
 
 // A record: 16 rows as [dim % 8][row-dim slot 256] sums, then the rows' maxima
@@ -459,6 +494,24 @@ __device__ __forceinline__ float max_groups(float v) {  // over the four lane gr
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// Sums whose reference was not the largest score: outside [2^-60, 2^100), or
+// not finite.
+__device__ __forceinline__ bool bad_sums(float L, const f32x4 (&acc)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int d = 0; d < 8; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(acc[d][i]) & 0x7fffffffu);
+  return !(L >= 0x1p-60f && L < 0x1p100f) || top >= 0x7f800000u;
+}
+// The factor that takes a sum L to [1, 2); m becomes the reference of that.
+__device__ __forceinline__ float rebase(float L, float& m) {
+  if (!(L > 0.f && L < INFINITY)) return 1.f;
+  const int x = (int)(__float_as_uint(L) >> 23) - 127;  // (L at least 2^-60, or 1 with a running maximum)
+  m = (m == -INFINITY ? 0.f : m) + (float)x;
+  return __uint_as_float((uint32_t)(127 - x) << 23);
+}
+
 // Takes the NaN groups out of a tile's values where some row does not see
 // their token (0 times a NaN is one); flags gets 0xff in the bytes of theirs.
 __device__ __forceinline__ void take_nan(u32x4& v, uint32_t& vs, uint32_t& flags) {
@@ -496,7 +549,7 @@ __device__ __forceinline__ float merge_factor(float m, float M) {
 // dims 32 g + 8 i .. + 7 of a row; slot = (16 g + row % 16) * 4 + i
 __device__ __forceinline__ void write_row(const Kv4Args& a, const Unit& u, int r, int slot, float L,
                                           const float (&o)[8]) {
-  const int tok = r / a.G, head = u.h * a.G + r - tok * a.G;
+  const int tok = (uint32_t)r / a.by_g, head = u.h * a.G + r - tok * a.G;
   // (L is 0 where the row sees no key, NaN where a score is)
   const float inv = L == 0.f ? 0.f : 1.f / L;
   bf16x8 y;
@@ -527,11 +580,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
   Unit u;
   if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
   const int rows = u.n * a.G, r0 = u.b * RB;
-  const int64_t kmax = a.max_blocks * a.tpp * kTile;
-  const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
-  const int64_t st0 = (int64_t)u.p * spp;                                      // the part's first step
-  const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
-  const int nst = (int)max<int64_t>(0, min<int64_t>(spp, steps - st0));
+  const int kend = last_key(a, u, min(r0 + RB, rows) - 1);
+  const int st0 = u.p * spp;                                // the part's first step
+  const int nst = max(0, min(spp, (kend + KS - 1) / KS - st0));
   if (nst == 0 && u.p > 0) return;  // (the longest row's part; this block's end before it)
   const int nw = nst > w ? (nst - w + W - 1) / W : 0;  // this wave's steps: st0 + w + j W
 
@@ -546,13 +597,14 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
   auto tile_of_lane = [&](int j) { return ((uint32_t)st0 + w + (j + (lane >> 1)) * W) * 2 + (lane & 1); };
   auto request = [&](int j) {
     const uint32_t tile = tile_of_lane(j);
-    blk_next = (int64_t)tile * kTile < kend ? bt[tile / (uint32_t)a.tpp] : -1;
+    blk_next = tile * kTile < (uint32_t)kend ? bt[tile / a.by_tpp] : -1;
   };
   auto look = [&](int j) {
     const bool there = blk_next >= 0 && blk_next < a.num_blocks;
     gone = __ballot(!there);
+    const uint32_t tile = tile_of_lane(j);
     table = (int64_t)a.pages + (there ? (((int64_t)blk_next * a.hkv + u.h) * a.tpp +
-                                         tile_of_lane(j) % (uint32_t)a.tpp) * kRec : 0);
+                                         (tile - tile / a.by_tpp * (uint32_t)a.tpp)) * kRec : 0);
     request(j + 32);
   };
   request(0);
@@ -561,12 +613,12 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
   int ctx[SETS];  // keys that the lane's rows see, from the part's first step
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
-    const int r = min(r0 + e * 16 + col, rows - 1), tok = r / a.G;
+    const int r = min(r0 + e * 16 + col, rows - 1), tok = (uint32_t)r / a.by_g;
     q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
-    ctx[e] = (int)min<int64_t>(max<int64_t>(u.len + tok + 1 - st0 * KS, 0), (int64_t)nst * KS);
+    ctx[e] = min(max(u.len + tok + 1 - st0 * KS, 0), nst * KS);
   }
-  const int all_see = (int)min<int64_t>(max<int64_t>(u.len + r0 / a.G + 1 - st0 * KS, 0), (int64_t)nst * KS);
-  const int live = (int)min<int64_t>(max<int64_t>(kend - st0 * KS, 0), (int64_t)nst * KS);
+  const int all_see = min(max(last_key(a, u, r0) - st0 * KS, 0), nst * KS);  // keys that every row sees
+  const int live = min(max(kend - st0 * KS, 0), nst * KS);                    // that any sees
 
   auto tile_at = [&](int j, int t) { return reinterpret_cast<const uint8_t*>(lane64(table, 2 * (j & 31) + t)); };
   uint32_t koff = 64 * col + 16 * g, soff = lane, voff = 16 * lane, xoff = 16 * g + (col & 12);
@@ -651,7 +703,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
         const float mx = c2 * max_groups(fmaxf(fmaxf(fmaxf(sv[e][0][0], sv[e][0][1]), fmaxf(sv[e][0][2], sv[e][0][3])),
                                                fmaxf(fmaxf(sv[e][1][0], sv[e][1][1]), fmaxf(sv[e][1][2], sv[e][1][3]))));
         // the reference the exponents are taken from moves only when the maximum
-        // has grown by 2^8 since: any reference gives the same quotient
+        // has grown by 2^8 since: any reference gives the same quotient.  (The
+        // reference of the first step alone, as in the kernel for many rows, is
+        // level or slower here: the cache's bytes are the bound.)
         if (__ballot(mx > m[e] + 8.f) != 0) {
           const float mn = fmaxf(m[e], mx);
           const float corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
@@ -777,24 +831,21 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   Unit u;
   if (!find_unit<RB, KS, false>(a, blockIdx.x, lane, spp, u)) return;  // the same for the whole workgroup
   const int rows = u.n * a.G, r0 = u.b * RB, wr0 = r0 + 32 * w;
-  const int64_t kmax = a.max_blocks * a.tpp * kTile;
-  const int64_t ctx_lo = u.len + r0 / a.G + 1;  // of the block's first row
-  const int64_t kend = min<int64_t>(u.len + (min(r0 + RB, rows) - 1) / a.G + 1, kmax);
-  const int64_t st0 = (int64_t)u.p * spp;
-  const int64_t steps = kend > 0 ? (kend + KS - 1) / KS : 0;
-  const int nst = (int)max<int64_t>(0, min<int64_t>(spp, steps - st0));
+  const int kend = last_key(a, u, min(r0 + RB, rows) - 1);
+  const int st0 = u.p * spp;
+  const int nst = max(0, min(spp, (kend + KS - 1) / KS - st0));
   if (nst == 0 && u.p > 0) return;
 
   QFrag q[2];
   int ctx[2];  // keys that the lane's rows see, from the part's first step
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int r = min(wr0 + e * 16 + col, rows - 1), tok = r / a.G;
+    const int r = min(wr0 + e * 16 + col, rows - 1), tok = (uint32_t)r / a.by_g;
     q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
-    ctx[e] = (int)min<int64_t>(max<int64_t>(u.len + tok + 1 - st0 * KS, 0), (int64_t)nst * KS);
+    ctx[e] = min(max(u.len + tok + 1 - st0 * KS, 0), nst * KS);
   }
-  const int all_see = (int)min<int64_t>(max<int64_t>(ctx_lo - st0 * KS, 0), (int64_t)nst * KS);  // by every row
-  const int live = (int)min<int64_t>(max<int64_t>(kend - st0 * KS, 0), (int64_t)nst * KS);       // by any
+  const int all_see = min(max(last_key(a, u, r0) - st0 * KS, 0), nst * KS);  // by every row
+  const int live = min(max(kend - st0 * KS, 0), nst * KS);                    // by any
 
   // lane 4 i + t: address of the record of tile t of step j0 + i (the first
   // record's where it is past the keys or has no page: `gone` tells), a table of
@@ -805,14 +856,14 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   int32_t blk_next = -1;
   auto request = [&](int j) {
     const uint32_t tile = (uint32_t)(st0 + j) * 4 + lane;  // (fewer than 2^26)
-    blk_next = (int64_t)tile * kTile < kend ? bt[tile / (uint32_t)a.tpp] : -1;
+    blk_next = tile * kTile < (uint32_t)kend ? bt[tile / a.by_tpp] : -1;
   };
   auto look = [&](int j) {
     const uint32_t tile = (uint32_t)(st0 + j) * 4 + lane;
     const bool there = blk_next >= 0 && blk_next < a.num_blocks;
     gone = __ballot(!there);
     table = (int64_t)a.pages +
-            (there ? (((int64_t)blk_next * a.hkv + u.h) * a.tpp + tile % (uint32_t)a.tpp) * kRec : 0);
+            (there ? (((int64_t)blk_next * a.hkv + u.h) * a.tpp + (tile - tile / a.by_tpp * (uint32_t)a.tpp)) * kRec : 0);
     request(j + 16);
   };
   auto tile_at = [&](int j, int t) { return reinterpret_cast<const uint8_t*>(lane64(table, 4 * (j & 15) + t)); };
@@ -1017,15 +1068,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   pass(std::false_type{});
   bool bad = false;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    bad |= !(l[e][0] >= 0x1p-60f && l[e][0] < 0x1p100f);
-    float t = 0.f;  // (a NaN or an infinity stays one)
-#pragma unroll
-    for (int d = 0; d < 8; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t = fmaxf(t, fabsf(acc[e][d][i])) + 0.f * acc[e][d][i];
-    bad |= !(t < INFINITY);
-  }
+  for (int e = 0; e < 2; ++e) bad |= bad_sums(l[e][0], acc[e]);
   const bool any = __ballot(bad) != 0;
   if (lane == 0) again[w] = any ? 1 : 0;
   __syncthreads();
@@ -1038,17 +1081,10 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt_kernel(Kv4Args a) {
   for (int e = 0; e < 2; ++e) {
     const int r = wr0 + e * 16 + col;
     if (r >= rows) continue;
-    // sums to [1, 2): their reference may be far from the largest score
-    float L = l[e][0], f = 1.f;
+    const float f = rebase(l[e][0], m[e]), L = l[e][0] * f;
     if (nan_v[e])
 #pragma unroll
       for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{NAN, NAN, NAN, NAN};
-    if (L > 0.f && L < INFINITY) {
-      const int x = (int)(__float_as_uint(L) >> 23) - 127;  // (L >= 2^-60, or >= 1 with a running maximum)
-      f = __uint_as_float((uint32_t)(127 - x) << 23);
-      L *= f;
-      m[e] += (float)x;
-    }
     if (u.parts == 1) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1083,8 +1119,8 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
   if (!find_unit<RB, KS, true>(a, blockIdx.x / SETS, lane, spp, u)) return;
   const int rows = u.n * a.G, row = threadIdx.x >> 2 & 15, r = u.b * RB + e * 16 + row;
   // the block's own parts: its last row may see fewer keys than the sequence's
-  const int64_t kend = min<int64_t>(u.len + (min((u.b + 1) * RB, rows) - 1) / a.G + 1, a.max_blocks * a.tpp * kTile);
-  const int parts = (int)max<int64_t>(1, (max<int64_t>(kend, 0) + (int64_t)spp * KS - 1) / ((int64_t)spp * KS));
+  const int steps = (last_key(a, u, min((u.b + 1) * RB, rows) - 1) + KS - 1) / KS;
+  const int parts = ceil_div(max(steps, 1), spp, 1.f / (float)spp);
   if (r >= rows || u.rec + (int64_t)(parts - 1) * a.hkv >= a.max_rec) return;
   const float* rec = a.part + (u.rec * SETS + e) * kRecF;
   const int64_t next = (int64_t)a.hkv * SETS * kRecF;
@@ -1217,7 +1253,10 @@ Kv4Args kv4_args(void* pages, int64_t num_blocks, int block_size, const int32_t*
   a.num_blocks = num_blocks;
   a.tpp = block_size / kTile;
   a.bt = block_table;
+  a.by_tpp = fast_div((uint32_t)a.tpp);
+  a.by_hkv = fast_div((uint32_t)hkv);
   a.max_blocks = max_blocks;
+  a.kmax = (int32_t)(max_blocks * block_size);  // (at most 2^30)
   a.seqlens = cache_seqlens;
   a.nseq = nseq;
   a.T = T;
@@ -1327,6 +1366,7 @@ extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq,
   a.qs = q_stride;
   a.hq = hq;
   a.G = hq / hkv;
+  a.by_g = fast_div((uint32_t)a.G);
   a.scale = softmax_scale;
   a.out = reinterpret_cast<bf16*>(out);
   if (!cu_seqlens) max_q_len = ntok / nseq;
