@@ -67,7 +67,7 @@ struct Kv4Args {
   int32_t kmax;             // keys of a table
   int32_t nseq, L, hq, hkv, G;
   int32_t tpp;              // tiles of a page
-  FastDiv by_g, by_hkv, by_tpp;
+  FastDiv by_g, by_hkv, by_tpp, by_l;
   float scale;
   // attention: records of parts; workgroups that run at once
   float* part;
@@ -75,10 +75,26 @@ struct Kv4Args {
   int64_t max_rec;
 };
 
+__device__ __forceinline__ uint32_t ldg_u8(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) uint8_t*)(p);
+}
+__device__ __forceinline__ uint32_t ldg_u32(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) uint32_t*)(p);
+}
+
+__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
+  const uint32_t x = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t y = __float_as_uint(v);
+  auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // The sequence of packed token t (the same for the whole wave): how many
 // sequences end at or before it; nseq for a token behind the last one.
 __device__ __forceinline__ int seq_of(const Kv4Args& a, int64_t t, int lane) {
-  if (!a.cu) return (int)(t / a.L);
+  if (!a.cu) return (int)((uint32_t)t / a.by_l);
   int s = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
     const int i = i0 + lane;
@@ -91,8 +107,9 @@ __device__ __forceinline__ int seq_of(const Kv4Args& a, int64_t t, int lane) {
 // has no page.
 __device__ __forceinline__ uint8_t* tile_of(const Kv4Args& a, int s, int h, int64_t p) {
   if (p < 0) return nullptr;
-  const int64_t tile = p / kTile, bi = tile / a.tpp;
-  if (bi >= a.max_blocks) return nullptr;
+  const int64_t tile = p / kTile;
+  if (p >= a.kmax) return nullptr;
+  const int64_t bi = (uint32_t)tile / a.by_tpp;
   const int32_t blk = a.bt[(int64_t)s * a.max_blocks + bi];
   if (blk < 0 || blk >= a.num_blocks) return nullptr;
   return a.pages + (((int64_t)blk * a.hkv + h) * a.tpp + (tile - bi * a.tpp)) * kRec;
@@ -203,29 +220,56 @@ __device__ __forceinline__ u32x4 values8(uint32_t codes, uint32_t b) {
   return u32x4{pair_bf16<0>(codes, s), pair_bf16<1>(codes, s), pair_bf16<2>(codes, s), pair_bf16<3>(codes, s)};
 }
 
-// Cached tokens as bf16: sixteen threads a (token, head) row of keys and of
-// values, a wave four tokens of a head.  Tokens without a page are zeros.
+// (written once and not read here: kept out of the caches' way)
+__device__ __forceinline__ void stg16_nt(bf16* p, u32x4 v) {
+  __builtin_nontemporal_store(v, (__attribute__((address_space(1))) u32x4*)p);
+}
+
+// Cached tokens as bf16: sixteen lanes a (token, head) row of keys and of
+// values (four tokens a wave at a time, sixteen in flight), so that a store
+// covers whole rows.  Tokens without a page are zeros.
+constexpr int kReadTokens = 16;  // of a wave
+
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
-  const int lane = threadIdx.x & 63, c = lane & 15;
-  const int h = blockIdx.y;
-  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4;
-  for (int u = 0; u < 4; ++u) {
-    const int64_t tu = t0 + u;  // the sequence is found for a token at a time by the whole wave
-    if (tu >= a.T) return;
-    const int s = seq_of(a, tu, lane);
-    if (s >= a.nseq || (lane >> 4) != u) continue;
-    const int64_t p = (int64_t)a.seqlens[s] + tu - (a.cu ? (int64_t)a.cu[s] : (int64_t)s * a.L);
-    const uint8_t* rec = tile_of(a, s, h, p);
-    u32x4 k = u32x4{0u, 0u, 0u, 0u}, v = k;
-    if (rec) {
-      const int tk = (int)(p & 15);
-      k = values8(*reinterpret_cast<const uint32_t*>(rec + 64 * tk + 4 * c), rec[kRecKs + 16 * (c >> 2) + tk]);
-      v = values8(*reinterpret_cast<const uint32_t*>(rec + kRecV + 256 * (tk >> 2) + 16 * c + 4 * (tk & 3)),
-                  rec[kRecVs + 16 * (tk >> 2) + 4 * (c >> 2) + (tk & 3)]);
+  const int lane = threadIdx.x & 63, c = lane & 15, h = blockIdx.y;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kReadTokens;
+  if (t0 >= a.T) return;
+  constexpr int N = kReadTokens / 4;
+  // sequences of the wave's tokens: how many end at or before each
+  int seq[kReadTokens] = {};
+  if (a.cu)
+    for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+      const int i = i0 + lane;
+      const int end = i < a.nseq ? a.cu[i + 1] : 0x7fffffff;
+#pragma unroll
+      for (int k = 0; k < kReadTokens; ++k) seq[k] += __popcll(__ballot(end <= t0 + k));
     }
-    const int64_t at = (tu * a.hkv + h) * kD + 8 * c;
-    *reinterpret_cast<u32x4*>(a.out + at) = k;
-    *reinterpret_cast<u32x4*>(a.out2 + at) = v;
+  uint32_t kq[N], vq[N], kb[N], vb[N];
+  bool in[N], there[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int64_t t = t0 + 4 * n + (lane >> 4);
+    const int q = lane >> 4;
+    int s = q == 0 ? seq[4 * n] : q == 1 ? seq[4 * n + 1] : q == 2 ? seq[4 * n + 2] : seq[4 * n + 3];
+    if (!a.cu) s = (int)min<int64_t>((uint32_t)t / a.by_l, a.nseq);
+    in[n] = t < a.T && s < a.nseq;
+    const int64_t p = in[n] ? (int64_t)a.seqlens[s] + t - (a.cu ? (int64_t)a.cu[s] : (int64_t)s * a.L) : -1;
+    const uint8_t* rec = tile_of(a, s, h, p);
+    there[n] = rec != nullptr;
+    if (!rec) rec = a.pages;
+    const int tk = (int)(p & 15);
+    kq[n] = ldg_u32(rec + 64 * tk + 4 * c);
+    vq[n] = ldg_u32(rec + kRecV + 256 * (tk >> 2) + 16 * c + 4 * (tk & 3));
+    kb[n] = ldg_u8(rec + kRecKs + 16 * (c >> 2) + tk);
+    vb[n] = ldg_u8(rec + kRecVs + 16 * (tk >> 2) + 4 * (c >> 2) + (tk & 3));
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (!in[n]) continue;
+    const int64_t at = ((t0 + 4 * n + (lane >> 4)) * a.hkv + h) * kD + 8 * c;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    stg16_nt(a.out + at, there[n] ? values8(kq[n], kb[n]) : zero);
+    stg16_nt(a.out2 + at, there[n] ? values8(vq[n], vb[n]) : zero);
   }
 }
 
@@ -476,22 +520,6 @@ __device__ __forceinline__ void v_pairs(u32x4 v, uint32_t vs, uint32_t (&f)[8][2
   put(4, x);
   v_pair<3>(v, vs, x);
   put(6, x);
-}
-
-__device__ __forceinline__ uint32_t ldg_u8(const uint8_t* p) {
-  return *(const __attribute__((address_space(1))) uint8_t*)(p);
-}
-__device__ __forceinline__ uint32_t ldg_u32(const uint8_t* p) {
-  return *(const __attribute__((address_space(1))) uint32_t*)(p);
-}
-
-__device__ __forceinline__ float max_groups(float v) {  // over the four lane groups
-  const uint32_t x = __float_as_uint(v);
-  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const uint32_t y = __float_as_uint(v);
-  auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // Sums whose reference was not the largest score: outside [2^-60, 2^100), or
@@ -1262,6 +1290,7 @@ Kv4Args kv4_args(void* pages, int64_t num_blocks, int block_size, const int32_t*
   a.T = T;
   a.cu = cu;
   a.L = (int32_t)(nseq > 0 ? T / nseq : 0);
+  a.by_l = fast_div((uint32_t)std::max(a.L, 1));
   a.hkv = hkv;
   return a;
 }
@@ -1327,7 +1356,7 @@ extern "C" int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int bloc
                        cu_seqlens, hkv);
   a.out = reinterpret_cast<bf16*>(k_out);
   a.out2 = reinterpret_cast<bf16*>(v_out);
-  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((ntok + 15) / 16), (unsigned)hkv), dim3(256), 0,
+  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((ntok + 4 * kReadTokens - 1) / (4 * kReadTokens)), (unsigned)hkv), dim3(256), 0,
                      (hipStream_t)stream, a);
   SWL_LAUNCH_CHECK("kv4_read_kernel launch");
   return SWL_OK;
