@@ -8,11 +8,17 @@
 // the last draft where none was: its distribution is the target's.  A drafter
 // without probabilities counts as certain of its draft (q = 1 at d_j).
 //
-// Probabilities are held in 64 bits: with 128256 tokens a cumulative sum that is
-// off by 1e-7 of the total picks another token once in about forty draws.
-// Three launches: statistics of every row (maximum, sum; a workgroup per slice
-// of a row); acceptance and the weight of every slice of the sequence's last
-// row; the slice and token the random number falls in.
+// What decides is held in 64 bits: with 128256 tokens a cumulative sum that is
+// off by 1e-7 of the total picks another token once in about forty draws.  A
+// 64-bit exponential costs fifteen times an fp32 one, though (28 sequences of 1
+// to 5 drafts, 128256 tokens: 77 us with 64 bits throughout, 37 now), and most rows only
+// have to show that their draft is accepted: u q < p is clear in fp32 unless the
+// two are within 2^-14 of each other.  So, in two launches: every row's maximum
+// and sum in fp32, a workgroup per slice of a row (the logits' bytes are its
+// bound); then a workgroup per slice of every sequence's last row: acceptance
+// (each for itself; a comparison that is not clear again in 64 bits over the
+// whole row), the slice's weight in 64 bits, and by the workgroup that ends last
+// the slice and token that the random number falls in.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -24,17 +30,15 @@
 namespace {
 
 struct RowStat {
-  double z;       // sum of exp((x - max) / temperature) over the slice
-  uint32_t key;   // order key of the slice's largest logit
-  int32_t idx;    // its first index
+  float z;        // sum of e^((x - max) / temperature) over the slice
+  float mx;       // its largest logit
+  int32_t idx;    // the first index of that (greedy rows)
+  int32_t pad;
 };
-struct SeqPick {
-  double p_inv, q_inv;  // 1 / sum
-  float p_max, q_max;
-  int64_t row;          // last row (target), -1: nothing to draw, the token is set
-  int64_t q_row;        // draft row subtracted from it, -1: none
-  int64_t skip;         // token whose weight is 0, -1: none
-  int64_t best;         // first index of the row's largest logit
+// A slice of a sequence's last row: sums of the target's and the drafter's
+// e^(..), and of the residual and the drafter's part of it at a given ratio.
+struct SliceSum {
+  double p, q, res, act;
 };
 
 struct VerifyArgs {
@@ -48,10 +52,13 @@ struct VerifyArgs {
   const float* u_last;
   int64_t* tok;         // [nseq, max_drafts + 1]
   int32_t* acc;
-  int32_t nseq, per, max_drafts, slices, slice;  // slice: logits of one
-  RowStat* stat;        // [T + nseq rows, then T rows][slices]
-  SeqPick* pick;        // [nseq]
-  double* mass;         // [nseq][slices]
+  int32_t nseq, per, max_drafts;
+  int32_t stats, slices;  // slices of a row: of its statistics, of a sequence's last row
+  int32_t chunks;
+  RowStat* stat;        // [T + nseq rows, then T rows][stats]
+  SliceSum* sum;        // [nseq][slices]
+  uint32_t* done;       // [nseq] slices that are (set to 0 by the first launch)
+  double* pow;          // [256] 2^(k / 256) (made by it)
 };
 
 // order-preserving maps of a bf16's bits to 16 bits and back, a NaN of either
@@ -91,20 +98,86 @@ __device__ __forceinline__ uint32_t bits_at(const u32x4& q, int e) {
 }
 __device__ __forceinline__ bool row_vec(const bf16* row) { return (reinterpret_cast<uintptr_t>(row) & 15) == 0; }
 
-// e^((x - max) / temperature)
-__device__ __forceinline__ double weight(uint32_t bits, float mx, double invt) {
-  return exp(((double)__uint_as_float(bits << 16) - (double)mx) * invt);
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kPow = 256;  // entries of the table of 2^(k / 256)
+
+// e^((x - max) / temperature) in 64 bits; rate = 256 log2(e) / temperature, tab
+// the 256 powers 2^(k / 256) (made by the first launch).  The series of 2^f for
+// the rest |f| <= 1/512 to the fourth power (the next term is under 4e-17).
+// -inf gives 0, a NaN itself.
+__device__ __forceinline__ double weight(uint32_t bits, float mx, double rate, const double* tab) {
+  constexpr double c = 0.693147180559945309417232121458 / kPow;  // ln 2 / 256
+  constexpr double c2 = c * c;
+  const double x = __uint_as_float(bits == 0xff80u ? 0xff7f0000u : bits << 16);  // (-inf: the lowest number)
+  const double y = (x - (double)mx) * rate, n = rint(y), f = y - n;
+  const int k = (int)n;
+  double r = c2 * c2 / 24;
+  r = fma(r, f, c2 * c / 6);
+  r = fma(r, f, c2 / 2);
+  r = fma(r, f, c);
+  r = fma(r, f, 1.0);
+  return ldexp(r * tab[k & (kPow - 1)], k >> 8);
+}
+__device__ __forceinline__ double rate_of(float temp) {
+  return kPow * 1.44269504088896340735992468100 / (double)temp;
+}
+
+// Sum over the workgroup's 256 threads, the same order always.
+__device__ __forceinline__ double block_sum(double v, double* sh) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+__device__ __forceinline__ void block_sum2(double& v, double& w, double* sh) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    v += __shfl_xor(v, o, 64);
+    w += __shfl_xor(w, o, 64);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    sh[threadIdx.x >> 6] = v;
+    sh[4 + (threadIdx.x >> 6)] = w;
+  }
+  __syncthreads();
+  v = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  w = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+}
+// Inclusive prefix over them, likewise.
+__device__ __forceinline__ double block_prefix(double v, double* sh) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh[wv] = v;
+  __syncthreads();
+  for (int w = 0; w < wv; ++w) v += sh[w];
+  return v;
 }
 
 // Slices of a row, 256 threads with E logits each.
 template <int E>
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   __shared__ uint32_t shk[4];
-  __shared__ double shz[4];
+  __shared__ float shz[4];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t R = a.T + a.nseq;
   const int64_t r = blockIdx.y, t = r - R;  // target rows, then draft rows
   const bool draft = t >= 0;
+  if (blockIdx.x == 0 && r < a.nseq && tid == 0) a.done[r] = 0;
+  if (blockIdx.x == 0 && r == 0) a.pow[tid] = exp2((double)tid / kPow);
+  const bf16* row = draft ? a.drf + t * a.ld_d : a.tgt + r * a.ld_t;
+  const bool vec = row_vec(row);
+  const int64_t base = (int64_t)blockIdx.x * (256 * E);
+  u32x4 q[E / 8];  // (requested before the sequence is looked for)
+#pragma unroll
+  for (int j = 0; j < E / 8; ++j) q[j] = logits8(row, base + (j * 256 + tid) * 8, a.vocab, vec);
   int s = 0;
   if (a.cu) {
     for (int i0 = 0; i0 < a.nseq; i0 += 64) {
@@ -117,309 +190,442 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   if (s >= a.nseq) return;  // (rows behind the last sequence)
   const float temp = a.temp[s];
   if (draft && temp <= 0.f) return;
-  const bf16* row = draft ? a.drf + t * a.ld_d : a.tgt + r * a.ld_t;
-  const bool vec = row_vec(row);
-  const int64_t base = (int64_t)blockIdx.x * a.slice;
-  u32x4 q[E / 8];
+  if (temp <= 0.f) {  // greedy: the largest and its first index are all there is to know
+    uint32_t best = 0;  // order key, then the index counted down
 #pragma unroll
-  for (int j = 0; j < E / 8; ++j) q[j] = logits8(row, base + (j * 256 + tid) * 8, a.vocab, vec);
-  uint32_t best = 0;  // order key, then the index counted down
+    for (int j = 0; j < E / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = (j * 256 + tid) * 8 + e;
+        if (base + at < a.vocab) best = max(best, vkey16(bits_at(q[j], e)) << 13 | (uint32_t)(8191 - at));
+      }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, o, 64));
+    if (lane == 0) shk[wv] = best;
+    __syncthreads();
+    best = max(max(shk[0], shk[1]), max(shk[2], shk[3]));
+    if (tid == 0)
+      a.stat[r * a.stats + blockIdx.x] = RowStat{0.f, vkey_value(best >> 13), (int32_t)(base + 8191 - (best & 8191)), 0};
+    return;
+  }
+  float mx = -INFINITY;  // (a NaN is passed over, and met again in the sum)
 #pragma unroll
   for (int j = 0; j < E / 8; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = (j * 256 + tid) * 8 + e;
-      if (base + at < a.vocab) best = max(best, vkey16(bits_at(q[j], e)) << 13 | (uint32_t)(8191 - at));
-    }
+    for (int e = 0; e < 4; ++e)
+      mx = fmaxf(mx, fmaxf(__uint_as_float(q[j][e] << 16), __uint_as_float(q[j][e] & 0xffff0000u)));
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, o, 64));
-  if (lane == 0) shk[wv] = best;
+  for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  if (lane == 0) shk[wv] = __float_as_uint(mx);
   __syncthreads();
-  best = max(max(shk[0], shk[1]), max(shk[2], shk[3]));
-  const float mx = vkey_value(best >> 13);
-  double z = 0;
-  if (temp > 0.f || temp != temp) {
-    const double invt = 1.0 / (double)temp;
-    if (mx != -INFINITY) {  // (a slice of nothing but -inf weighs 0)
+  mx = fmaxf(fmaxf(__uint_as_float(shk[0]), __uint_as_float(shk[1])),
+             fmaxf(__uint_as_float(shk[2]), __uint_as_float(shk[3])));
+  float z = 0.f;
+  if (mx != -INFINITY) {  // (a slice of nothing but -inf weighs 0; so does what is past the row)
+    const float c = kLog2e / temp;
 #pragma unroll
-      for (int j = 0; j < E / 8; ++j)
+    for (int j = 0; j < E / 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (base + (j * 256 + tid) * 8 + e < a.vocab) z += weight(bits_at(q[j], e), mx, invt);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o, 64);
-    if (lane == 0) shz[wv] = z;
-    __syncthreads();
-    z = (shz[0] + shz[1]) + (shz[2] + shz[3]);
-  }
-  if (tid == 0) a.stat[r * a.slices + blockIdx.x] = RowStat{z, best >> 13, (int32_t)(base + 8191 - (best & 8191))};
-}
-
-// A row's statistics from its slices', by sixteen lanes.
-struct RowAll {
-  double z;
-  float mx;
-  int64_t best;
-};
-__device__ __forceinline__ RowAll row_all(const VerifyArgs& a, int64_t r, double invt, int l16) {
-  const RowStat* st = a.stat + r * a.slices;
-  uint64_t best = 0;
-  for (int c = l16; c < a.slices; c += 16)
-    best = max(best, (uint64_t)st[c].key << 32 | (uint32_t)~(uint32_t)st[c].idx);
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) best = max(best, (uint64_t)__shfl_xor((long long)best, o, 16));
-  RowAll x;
-  x.mx = vkey_value((uint32_t)(best >> 32));
-  x.best = (int64_t)(uint32_t)~(uint32_t)best;
-  x.z = 0;
-  for (int c = l16; c < a.slices; c += 16)
-    x.z += st[c].z * exp(((double)vkey_value(st[c].key) - (double)x.mx) * invt);
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) x.z += __shfl_xor(x.z, o, 16);
-  return x;
-}
-
-// Acceptance of a sequence's drafts (sixteen lanes a draft, sixteen drafts at a
-// time; every workgroup of the sequence for itself) and the weight of one slice
-// of its last row.
-template <int E>
-__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a) {
-  __shared__ int first_bad;
-  __shared__ double shz[4];
-  __shared__ SeqPick sp;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, l16 = tid & 15;
-  const int s = blockIdx.y;
-  int64_t t0;
-  int n;
-  drafts_of(a, s, t0, n);
-  const float temp = a.temp[s];
-  const bool greedy = temp <= 0.f;
-  const double invt = 1.0 / (double)temp;
-  const int64_t R = a.T + a.nseq, row0 = t0 + s;
-  if (tid == 0) first_bad = n;
-  __syncthreads();
-  for (int j0 = 0; j0 < n; j0 += 16) {
-    const int j = j0 + (tid >> 4);
-    if (j < n) {  // (the sixteen lanes together)
-      const int64_t d = a.ids[t0 + j];
-      bool ok = d >= 0 && d < a.vocab;
-      const RowAll p = row_all(a, row0 + j, invt, l16);
-      if (greedy) {
-        ok = ok && d == p.best;
-      } else if (ok) {
-        const uint16_t pb = *reinterpret_cast<const uint16_t*>(a.tgt + (row0 + j) * a.ld_t + d);
-        double qd = 1.0;
-        if (a.drf) {
-          const RowAll q = row_all(a, R + t0 + j, invt, l16);
-          const uint16_t qb = *reinterpret_cast<const uint16_t*>(a.drf + (t0 + j) * a.ld_d + d);
-          qd = weight(qb, q.mx, invt) / q.z;
-        }
-        ok = (double)a.u[t0 + j] * qd < weight(pb, p.mx, invt) / p.z;
+      for (int e = 0; e < 4; ++e) {
+        z += __builtin_amdgcn_exp2f((__uint_as_float(q[j][e] << 16) - mx) * c);
+        z += __builtin_amdgcn_exp2f((__uint_as_float(q[j][e] & 0xffff0000u) - mx) * c);
       }
-      if (!ok && l16 == 0) atomicMin(&first_bad, j);
-    }
-    __syncthreads();
-    const int bad = first_bad;
-    __syncthreads();  // read by all before the next drafts change it
-    if (bad < n) break;
-  }
-  const int take = first_bad;
-  if (tid < 16) {
-    SeqPick x{};
-    const RowAll p = row_all(a, row0 + take, invt, l16);
-    x.row = greedy ? -1 : row0 + take;
-    x.best = p.best;
-    x.p_max = p.mx;
-    x.p_inv = 1.0 / p.z;
-    x.q_row = x.skip = -1;
-    if (!greedy && take < n) {
-      const int64_t d = a.ids[t0 + take];
-      if (d >= 0 && d < a.vocab) {
-        if (a.drf) {
-          const RowAll q = row_all(a, R + t0 + take, invt, l16);
-          x.q_row = t0 + take;
-          x.q_max = q.mx;
-          x.q_inv = 1.0 / q.z;
-        } else {
-          x.skip = d;
-        }
-      }
-    }
-    if (tid == 0) {
-      sp = x;
-      if (blockIdx.x == 0) {
-        a.pick[s] = x;
-        a.acc[s] = take;
-      }
-    }
-  }
-  if (blockIdx.x == 0)
-    for (int j = tid; j <= a.max_drafts; j += 256) a.tok[(int64_t)s * (a.max_drafts + 1) + j] = j < take ? a.ids[t0 + j] : -1;
-  if (greedy) return;
-  __syncthreads();
-  const bf16* prow = a.tgt + sp.row * a.ld_t;
-  const bf16* qrow = sp.q_row >= 0 ? a.drf + sp.q_row * a.ld_d : nullptr;
-  const int64_t base = (int64_t)blockIdx.x * a.slice;
-  double z = 0;
-  for (int j = 0; j < E / 8; ++j) {
-    const int64_t i = base + (j * 256 + tid) * 8;
-    if (i >= a.vocab) break;
-    const u32x4 p = logits8(prow, i, a.vocab, row_vec(prow));
-    u32x4 q = p;
-    if (qrow) q = logits8(qrow, i, a.vocab, row_vec(qrow));
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double w = weight(bits_at(p, e), sp.p_max, invt) * sp.p_inv;
-      if (qrow) {
-        w -= weight(bits_at(q, e), sp.q_max, invt) * sp.q_inv;
-        w = w < 0 ? 0 : w;  // (a NaN stays one)
-      }
-      if (i + e == sp.skip) w = 0;
-      if (i + e < a.vocab) z += w;
-    }
+    for (int j = 0; j < E / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((bits_at(q[j], e) & 0x7fffu) > 0x7f80u) z = NAN;
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o, 64);
   if (lane == 0) shz[wv] = z;
   __syncthreads();
-  if (tid == 0) a.mass[(int64_t)s * a.slices + blockIdx.x] = (shz[0] + shz[1]) + (shz[2] + shz[3]);
+  if (tid == 0) a.stat[r * a.stats + blockIdx.x] = RowStat{(shz[0] + shz[1]) + (shz[2] + shz[3]), mx, 0, 0};
 }
 
-// The slice that u * (sum of all) falls in, then the token of it: the first
-// whose cumulative weight is above that.  1024 threads, E / 4 logits each.
-template <int E>
-__global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
-  constexpr int N = E / 4;  // 8, or 2 (then 8 logits for every fourth thread)
-  __shared__ double shz[16];
-  __shared__ double shm[1024];
-  __shared__ int slot, first, last_any;
-  __shared__ double below;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int s = blockIdx.x;
-  const SeqPick x = a.pick[s];
-  int64_t* out = a.tok + (int64_t)s * (a.max_drafts + 1) + a.acc[s];
-  if (x.row < 0) {
-    if (tid == 0) *out = x.best;
-    return;
+// A row's statistics from its slices', by sixteen lanes.
+struct RowAll {
+  float z, mx;
+  int64_t best;  // (greedy rows)
+};
+__device__ __forceinline__ RowAll row_all(const VerifyArgs& a, int64_t r, float c, bool greedy, int l16) {
+  const RowStat* st = a.stat + r * a.stats;
+  RowAll x{0.f, -INFINITY, 0};
+  RowStat own{0.f, -INFINITY, 0x7fffffff, 0};  // (sixteen slices hold 131072 logits: no round of the loops, mostly)
+  if (l16 < a.stats) own = st[l16];
+  if (greedy) {
+    auto key = [](const RowStat& v) {
+      return (uint64_t)vkey16(__float_as_uint(v.mx) >> 16) << 32 | (uint32_t)~(uint32_t)v.idx;
+    };
+    uint64_t best = key(own);
+    for (int i = 16 + l16; i < a.stats; i += 16) best = max(best, key(st[i]));
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) best = max(best, (uint64_t)__shfl_xor((long long)best, o, 16));
+    x.best = (int64_t)(uint32_t)~(uint32_t)best;
+    return x;
   }
-  const double* mass = a.mass + (int64_t)s * a.slices;
-  const double invt = 1.0 / (double)a.temp[s];
-  // the masses 1024 at a time through LDS: their sum, then where it passes u of it
-  double total = 0, sum = 0, before = 0;
-  int at = -1;
-  bool found = false;
-  for (int pass = 0; pass < 2; ++pass)
-    for (int c0 = 0; c0 < a.slices; c0 += 1024) {
-      __syncthreads();
-      if (c0 + tid < a.slices) shm[tid] = mass[c0 + tid];
-      __syncthreads();
-      if (tid == 0) {
-        const int m = min(1024, a.slices - c0);
-        const double want = (double)a.u_last[s] * total;
-        for (int c = 0; c < m && !found; ++c) {
-          if (pass == 0) {
-            total += shm[c];
-          } else {
-            if (shm[c] > 0) {  // the last slice of any weight where none passes it
-              at = c0 + c;
-              before = sum;
-              found = sum + shm[c] > want;
-            }
-            sum += shm[c];
+  x.mx = own.mx;
+  for (int i = 16 + l16; i < a.stats; i += 16) x.mx = fmaxf(x.mx, st[i].mx);
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) x.mx = fmaxf(x.mx, __shfl_xor(x.mx, o, 16));
+  // (slices of nothing but -inf weigh 0, or are a NaN)
+  auto part = [&](const RowStat& v) { return v.z == 0.f ? 0.f : v.z * __builtin_amdgcn_exp2f((v.mx - x.mx) * c); };
+  if (l16 < a.stats) x.z = part(own);
+  for (int i = 16 + l16; i < a.stats; i += 16) x.z += part(st[i]);
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) x.z += __shfl_xor(x.z, o, 16);
+  return x;
+}
+
+// What a sequence's last row is, and what is taken from it.
+struct Last {
+  const bf16* p;  // target row
+  const bf16* q;  // draft row subtracted from it, or null
+  int64_t skip;   // token whose weight is 0, -1: none
+  float p_max, q_max;
+  double ratio;   // the target's sum over the drafter's
+};
+// f(e, e^(..) of the target, of the drafter) for the eight tokens from i, in
+// order; 0 at `skip` and past the row.  (Not unrolled: these kernels run once
+// through their code, and its fetching would be their time.)
+template <typename F>
+__device__ __forceinline__ void weights8(const VerifyArgs& a, const Last& x, int64_t i, double rate,
+                                         const double* tab, F f) {
+  u32x4 p = logits8(x.p, i, a.vocab, row_vec(x.p)), q = p;
+  if (x.q) q = logits8(x.q, i, a.vocab, row_vec(x.q));
+#pragma unroll 1
+  for (int e = 0; e < 8; e += 2) {
+    double wp[2], wq[2] = {0, 0};
+    wp[0] = weight(p[0] & 0xffffu, x.p_max, rate, tab);
+    wp[1] = weight(p[0] >> 16, x.p_max, rate, tab);
+    if (x.q) {
+      wq[0] = weight(q[0] & 0xffffu, x.q_max, rate, tab);
+      wq[1] = weight(q[0] >> 16, x.q_max, rate, tab);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bool in = i + e + k < a.vocab;
+      f(e + k, in && i + e + k != x.skip ? wp[k] : 0.0, in ? wq[k] : 0.0);
+    }
+    p = u32x4{p[1], p[2], p[3], p[0]};
+    q = u32x4{q[1], q[2], q[3], q[0]};
+  }
+}
+
+// The two rows' sums in 64 bits, by the workgroup (q 0 without a draft row).
+__device__ __forceinline__ void row_sums64(const VerifyArgs& a, const Last& x, double rate, const double* tab,
+                                           double* sh, double (&z)[2]) {
+  z[0] = z[1] = 0;
+  for (int64_t i = threadIdx.x * 8; i < a.vocab; i += 2048)
+    weights8(a, x, i, rate, tab, [&](int, double p, double q) {
+      z[0] += p;
+      z[1] += q;
+    });
+  block_sum2(z[0], z[1], sh);
+}
+
+// The first largest logit of a row, a NaN above all: for rows whose weights are
+// no numbers.
+__device__ int64_t row_best(const bf16* row, int64_t vocab, unsigned long long* sh) {
+  if (threadIdx.x == 0) *sh = 0;
+  __syncthreads();
+  unsigned long long best = 0;
+  for (int64_t i = threadIdx.x * 8; i < vocab; i += 2048) {
+    const u32x4 q = logits8(row, i, vocab, row_vec(row));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < vocab)
+        best = max(best, (unsigned long long)vkey16(bits_at(q, e)) << 32 | (uint32_t)~(uint32_t)(i + e));
+  }
+  atomicMax(sh, best);
+  __syncthreads();
+  return (int64_t)(uint32_t)~(uint32_t)*sh;
+}
+
+// Device-scope accesses, past the caches that other XCDs do not see.
+__device__ __forceinline__ void put(double* p, double v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Acceptance of a sequence's drafts (sixteen lanes for a draft's target row and
+// sixteen for the drafter's, eight drafts at a time), one slice's weight of its
+// last row, and by the last workgroup of the
+// sequence the token: the first whose cumulative weight is above u * (sum of
+// all); where rounding leaves none, the last of any weight.
+//
+// The residual max(p - q, 0) needs the two rows' sums, which are known only when
+// all slices are: its weight is added up at the fp32 sums' ratio (off by a
+// relative d of under 2^-14, 1e-6 as a rule) together with the drafter's part F
+// of it, and put right by - d F at the end.  What that leaves out are the tokens
+// between the two ratios, d of themselves each and about d of all: d^2.
+constexpr int kChunk = 2048;  // logits of a workgroup at a time; a slice is a.chunks of them
+
+__global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
+  constexpr int kNone = 0x7fffffff;
+  __shared__ int first_bad, ended;
+  __shared__ double tab[kPow], sh[8], wt[8][256], below, first;
+  __shared__ int sh_hit[4], sh_any[4];
+  __shared__ float sh_mx[16], sh_z[16];  // maxima and sums of the eight drafts: target, drafter
+  __shared__ int64_t sh_best[8];
+  __shared__ unsigned long long shb;
+  const int tid = threadIdx.x, l16 = tid & 15, s = blockIdx.y;
+  tab[tid] = a.pow[tid];  // (a barrier follows)
+  int64_t t0;
+  int n;
+  drafts_of(a, s, t0, n);
+  const float temp = a.temp[s];
+  const bool greedy = temp <= 0.f;
+  const float c = kLog2e / temp;
+  const double rate = rate_of(temp);
+  const float u_last = a.u_last[s];
+  const int64_t R = a.T + a.nseq, row0 = t0 + s;
+  Last x;
+  // Drafts before `sure` are accepted; index n, behind the last draft, is where
+  // it ends at the latest.
+  int take, sure = 0;
+  int64_t d;
+  for (int j0 = 0;;) {
+    __syncthreads();
+    if (tid == 0) first_bad = kNone;
+    __syncthreads();
+    const int j = j0 + (tid >> 5);
+    const bool second = tid >> 4 & 1;
+    if (j <= n) {  // (the 32 lanes together)
+      const bool draft = j < n;
+      d = draft ? a.ids[t0 + j] : -1;
+      const bool in = d >= 0 && d < a.vocab;
+      const bf16* row = second && draft && a.drf ? a.drf + (t0 + j) * a.ld_d : a.tgt + (row0 + j) * a.ld_t;
+      const float lg = in ? bf2f(ldg(row + d)) : 0.f;
+      const float u = draft ? a.u[t0 + j] : 0.f;
+      const RowAll r = row_all(a, second && draft && a.drf && !greedy ? R + t0 + j : row0 + j, c, greedy, l16);
+      const float prob = __builtin_amdgcn_exp2f((lg - r.mx) * c) / r.z, other = __shfl_xor(prob, 16, 32);
+      if (l16 == 0) {
+        sh_mx[tid >> 4] = r.mx;
+        sh_z[tid >> 4] = r.z;
+        if (!second) {
+          sh_best[tid >> 5] = r.best;
+          bool ok = false, clear = true;
+          if (j < sure) {
+            ok = true;
+          } else if (greedy) {
+            ok = in && d == r.best;
+          } else if (in) {
+            const float v = a.drf ? u * other : u;
+            // (fp32: the exponents' roundings, under 2^-16 of a term that counts)
+            ok = v < prob * (1.f - 0x1p-14f) && prob > 0x1p-100f;
+            clear = ok || (v > prob * (1.f + 0x1p-14f) && v > 0x1p-100f && v < INFINITY);
           }
+          if (!ok) atomicMin(&first_bad, 2 * j + (clear ? 0 : 1));
         }
       }
     }
+    __syncthreads();
+    const int bad = first_bad;
+    if (bad == kNone) {
+      j0 += 8;
+      continue;
+    }
+    take = bad >> 1;
+    d = take < n ? a.ids[t0 + take] : -1;  // the refused draft
+    const bool subtract = d >= 0 && d < a.vocab;
+    x.p = a.tgt + (row0 + take) * a.ld_t;
+    x.q = subtract && a.drf ? a.drf + (t0 + take) * a.ld_d : nullptr;
+    x.skip = -1;
+    x.p_max = sh_mx[2 * (take - j0)];
+    x.q_max = sh_mx[2 * (take - j0) + 1];
+    const float zp = sh_z[2 * (take - j0)], zq = sh_z[2 * (take - j0) + 1];
+    x.ratio = (double)zp / (double)zq;
+    // A comparison that is not clear, or sums that fp32 does not have (an
+    // infinite rate, a NaN): from the whole rows, in 64 bits.
+    const bool poor = !greedy && x.q && !(zp >= 0.5f && zp < INFINITY && zq >= 0.5f && zq < INFINITY);
+    if (bad & 1 || poor) {
+      double z[2];
+      row_sums64(a, x, rate, tab, sh, z);
+      x.ratio = z[0] / z[1];
+      if (bad & 1) {
+        const double qd =
+            x.q ? weight(*reinterpret_cast<const uint16_t*>(x.q + d), x.q_max, rate, tab) / z[1] : 1.0;
+        const double pd = weight(*reinterpret_cast<const uint16_t*>(x.p + d), x.p_max, rate, tab) / z[0];
+        if ((double)a.u[t0 + take] * qd < pd) {
+          sure = take + 1;
+          continue;  // the same drafts again, this one taken
+        }
+      }
+    }
+    if (subtract && !x.q) x.skip = d;
+    break;
+  }
+  const int64_t best = sh_best[take & 7];  // (batches begin at multiples of eight)
+  int64_t* out = a.tok + (int64_t)s * (a.max_drafts + 1);
+  if (blockIdx.x == 0) {
+    if (tid == 0) a.acc[s] = take;
+    for (int j = tid; j <= a.max_drafts; j += 256)
+      if (j != take || greedy) out[j] = j < take ? a.ids[t0 + j] : j == take ? best : -1;
+  }
+  if (greedy) return;
+  SliceSum own{0, 0, 0, 0};
+  const int64_t slice = (int64_t)a.chunks * kChunk;
+#pragma unroll 1
+  for (int64_t i = blockIdx.x * slice + tid * 8; i < min((blockIdx.x + 1) * slice, a.vocab); i += kChunk)
+    weights8(a, x, i, rate, tab, [&](int, double p, double q) {
+      own.p += p;
+      own.q += q;
+      const double v = p - x.ratio * q;
+      if (x.q && !(v < 0)) {
+        own.res += v;
+        own.act += q;
+      }
+    });
+  if (x.q) {
+    block_sum2(own.p, own.q, sh);
+    block_sum2(own.res, own.act, sh);
+  } else {
+    own.p = block_sum(own.p, sh);
+  }
+  // The slice's sums are in memory, for every XCD, before it is counted: device-
+  // scope stores, waited for.  (A release fence would write back the XCD's whole
+  // L2, once a workgroup, and an acquire empty it.)
+  SliceSum* sums = a.sum + (int64_t)s * a.slices;
   if (tid == 0) {
-    slot = total > 0 ? at : -1;  // a NaN, or nothing left: the largest logit
-    below = (double)a.u_last[s] * total - before;
-    first = 1 << 30;
-    last_any = -1;
+    put(&sums[blockIdx.x].p, own.p);
+    if (x.q) {
+      put(&sums[blockIdx.x].q, own.q);
+      put(&sums[blockIdx.x].res, own.res);
+      put(&sums[blockIdx.x].act, own.act);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    ended = (int)__hip_atomic_fetch_add(&a.done[s], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (slot < 0) {
-    if (tid == 0) *out = x.best;
+  if (ended != a.slices - 1) return;
+  SliceSum v{0, 0, 0, 0};  // of slice tid (there are at most 256)
+  if (tid < a.slices) {
+    v.p = get(&sums[tid].p);
+    if (x.q) v = SliceSum{v.p, get(&sums[tid].q), get(&sums[tid].res), get(&sums[tid].act)};
+  }
+  double m = v.p;
+  if (x.q) {  // the exact ratio, and the weights put right to it
+    block_sum2(v.p, v.q, sh);
+    const double ratio = v.p / v.q;
+    m = v.res - (ratio - x.ratio) * v.act;
+    m = m < 0 ? 0 : m;
+    x.ratio = ratio;
+  }
+  // The first thread whose cumulative weight `inc` is above `goal` (where there
+  // is none, the last of any weight), by the workgroup; -1: no weight at all.
+  auto pick = [&](double w, double inc, double goal) {
+    const uint64_t over = __ballot(w > 0 && inc > goal), some = __ballot(w > 0);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+      sh_hit[tid >> 6] = over ? tid + __builtin_ctzll(over) : kNone;
+      sh_any[tid >> 6] = some ? tid + 63 - __builtin_clzll(some) : -1;
+    }
+    __syncthreads();
+    const int hit = min(min(sh_hit[0], sh_hit[1]), min(sh_hit[2], sh_hit[3]));
+    return hit != kNone ? hit : max(max(sh_any[0], sh_any[1]), max(sh_any[2], sh_any[3]));
+  };
+  double inc = block_prefix(m, sh);
+  if (tid == 255) below = inc;  // the sum of all
+  __syncthreads();
+  const double all = below, want = (double)u_last * all;
+  if (!(all > 0)) {  // a NaN, or nothing left
+    const int64_t b = row_best(x.p, a.vocab, &shb);
+    if (tid == 0) out[take] = b;
     return;
   }
-  const bf16* prow = a.tgt + x.row * a.ld_t;
-  const bf16* qrow = x.q_row >= 0 ? a.drf + x.q_row * a.ld_d : nullptr;
-  const int64_t i = (int64_t)slot * a.slice + tid * 8;
-  double w8[8];
-  sum = 0;
-  const bool in = tid < 128 * N && i < a.vocab;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w8[e] = 0;
-  if (in) {
-    const u32x4 p = logits8(prow, i, a.vocab, row_vec(prow));
-    u32x4 q = p;
-    if (qrow) q = logits8(qrow, i, a.vocab, row_vec(qrow));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double w = weight(bits_at(p, e), x.p_max, invt) * x.p_inv;
-      if (qrow) {
-        w -= weight(bits_at(q, e), x.q_max, invt) * x.q_inv;
-        w = w < 0 ? 0 : w;
-      }
-      if (i + e == x.skip || i + e >= a.vocab) w = 0;
-      w8[e] = w;
-      sum += w;
-    }
-  }
-  double inc = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += y;
-  }
-  if (lane == 63) shz[wv] = inc;
+  const int at = pick(m, inc, want);
+  if (tid == at) below = want - (inc - m);  // what is left for the slice (read behind pick's barriers)
   __syncthreads();
-  double cum = inc - sum;
-  for (int w = 0; w < wv; ++w) cum += shz[w];
-  // the first token above `below`, and the last of any weight (where rounding
-  // puts the slice's sum under it)
-  int mine = -1, last = -1;
-#pragma unroll
+  const double goal = below;
+  // the slice's chunks: the first whose weight passes that, else the last of any
+  double before = 0, w = 0;
+  int chunk = -1, who = 0, k = 0;
+  auto weigh = [&](int k) {
+    const int64_t i = at * slice + (int64_t)k * kChunk + tid * 8;
+    w = 0;
+    if (i < a.vocab)
+      weights8(a, x, i, rate, tab, [&](int e, double p, double q) {
+        const double y = x.q ? fmax(p - x.ratio * q, 0.0) : p;
+        w += y;
+        wt[e][tid] = y;
+      });
+  };
+#pragma unroll 1
+  for (;; ++k) {
+    weigh(k);
+    inc = before + block_prefix(w, sh);
+    const int t = pick(w, inc, goal);
+    if (t >= 0) {
+      chunk = k;
+      who = t;
+      if (tid == t) first = inc - w;
+      if (tid == 255) below = inc;
+      __syncthreads();
+      before = below;
+      __syncthreads();
+    }
+    if ((chunk >= 0 && before > goal) || k == a.chunks - 1) break;
+  }
+  if (chunk < 0) {  // (a weight that was the other ratio's alone: the residual is nothing)
+    const int64_t b = row_best(x.p, a.vocab, &shb);
+    if (tid == 0) out[take] = b;
+    return;
+  }
+  if (chunk != k) weigh(chunk);  // (the last chunks had no weight)
+  if (tid != who) return;
+  double cum = first;  // its tokens, one after another
+  int hit = 0;
   for (int e = 0; e < 8; ++e) {
-    cum += w8[e];
-    if (w8[e] > 0) {
-      last = tid * 8 + e;
-      if (mine < 0 && cum > below) mine = tid * 8 + e;
+    const double y = wt[e][tid];
+    cum += y;
+    if (y > 0) {
+      hit = e;
+      if (cum > goal) break;
     }
   }
-  if (mine >= 0) atomicMin(&first, mine);
-  if (last >= 0) atomicMax(&last_any, last);
-  __syncthreads();
-  if (tid == 0) *out = (int64_t)slot * a.slice + (first < (1 << 30) ? first : max(last_any, 0));
+  out[take] = at * slice + (int64_t)chunk * kChunk + tid * 8 + hit;
 }
 
-// Logits of a slice: 8192, or 2048 where that leaves under four workgroups a CU.
-int slice_of(int64_t rows, int64_t vocab) { return rows * ((vocab + 8191) / 8192) >= 1024 ? 8192 : 2048; }
+// Logits of a slice of the statistics: 8192, or 2048 where that leaves under
+// four workgroups a CU.
+int stats_slice(int64_t rows, int64_t vocab) { return rows * ((vocab + 8191) / 8192) >= 1024 ? 8192 : 2048; }
 
 struct VerifyLayout {
-  int slice;
-  int64_t slices, pick, mass, bytes;
+  int stats_slice, chunks;
+  int64_t stats, slices, sum, pow, done, bytes;
 };
 VerifyLayout verify_layout(int64_t nseq, int64_t T, int64_t vocab, bool draft) {
   VerifyLayout l;
   const int64_t rows = T + nseq + (draft ? T : 0);
-  l.slice = slice_of(rows, vocab);
-  l.slices = (vocab + l.slice - 1) / l.slice;
-  l.pick = rows * l.slices * (int64_t)sizeof(RowStat);
-  l.mass = l.pick + nseq * (int64_t)sizeof(SeqPick);
-  l.bytes = l.mass + nseq * l.slices * (int64_t)sizeof(double);
+  l.stats_slice = stats_slice(rows, vocab);
+  l.stats = (vocab + l.stats_slice - 1) / l.stats_slice;
+  // (slices of the last rows: about 1024 workgroups, which run at once, and 256
+  // of a row at most)
+  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+  l.chunks = (int)std::max((chunks + 255) / 256, (nseq * chunks + 1023) / 1024);
+  l.slices = (vocab + (int64_t)l.chunks * kChunk - 1) / ((int64_t)l.chunks * kChunk);
+  l.sum = rows * l.stats * (int64_t)sizeof(RowStat);
+  l.pow = l.sum + nseq * l.slices * (int64_t)sizeof(SliceSum);
+  l.done = l.pow + kPow * (int64_t)sizeof(double);
+  l.bytes = l.done + nseq * (int64_t)sizeof(uint32_t);
   return l;
 }
 
-template <int E>
-int launch_verify(const VerifyArgs& a, hipStream_t st) {
-  const unsigned rows = (unsigned)(a.T + a.nseq + (a.drf ? a.T : 0));
-  hipLaunchKernelGGL(verify_stats_kernel<E>, dim3((unsigned)a.slices, rows), dim3(256), 0, st, a);
+int launch_verify(const VerifyArgs& a, const VerifyLayout& l, hipStream_t st) {
+  const dim3 rows((unsigned)a.stats, (unsigned)(a.T + a.nseq + (a.drf ? a.T : 0)));
+  if (l.stats_slice == 8192)
+    hipLaunchKernelGGL(verify_stats_kernel<32>, rows, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(verify_stats_kernel<8>, rows, dim3(256), 0, st, a);
   SWL_LAUNCH_CHECK("verify_stats_kernel launch");
-  hipLaunchKernelGGL(verify_mass_kernel<E>, dim3((unsigned)a.slices, (unsigned)a.nseq), dim3(256), 0, st, a);
-  SWL_LAUNCH_CHECK("verify_mass_kernel launch");
-  hipLaunchKernelGGL(verify_pick_kernel<E>, dim3((unsigned)a.nseq), dim3(1024), 0, st, a);
-  SWL_LAUNCH_CHECK("verify_pick_kernel launch");
+  const dim3 last((unsigned)a.slices, (unsigned)a.nseq);
+  hipLaunchKernelGGL(verify_last_kernel, last, dim3(256), 0, st, a);
+  SWL_LAUNCH_CHECK("verify_last_kernel launch");
   return SWL_OK;
 }
 
@@ -467,11 +673,13 @@ extern "C" int swl_verify_drafts_bf16(const void* target, int64_t ld_target, con
   a.nseq = nseq;
   a.per = (int32_t)(ndraft / nseq);
   a.max_drafts = max_drafts;
+  a.stats = (int32_t)l.stats;
   a.slices = (int32_t)l.slices;
-  a.slice = l.slice;
+  a.chunks = l.chunks;
   char* ws = reinterpret_cast<char*>(workspace);
   a.stat = reinterpret_cast<RowStat*>(ws);
-  a.pick = reinterpret_cast<SeqPick*>(ws + l.pick);
-  a.mass = reinterpret_cast<double*>(ws + l.mass);
-  return l.slice == 8192 ? launch_verify<32>(a, (hipStream_t)stream) : launch_verify<8>(a, (hipStream_t)stream);
+  a.sum = reinterpret_cast<SliceSum*>(ws + l.sum);
+  a.pow = reinterpret_cast<double*>(ws + l.pow);
+  a.done = reinterpret_cast<uint32_t*>(ws + l.done);
+  return launch_verify(a, l, (hipStream_t)stream);
 }

@@ -7,6 +7,7 @@ raise.
 """
 
 import ctypes
+import functools
 from typing import List, Optional, Sequence
 
 import torch
@@ -641,21 +642,26 @@ def sample(logits: torch.Tensor, out_tok: Sequence[torch.Tensor], do_sample: Seq
                                            _i32_array(top_k), f32(top_p), int(seed), _stream()))
 
 
-def _logit_rows(t: torch.Tensor, name: str, packed: bool):
+def _logit_rows(t: torch.Tensor, name: str, packed: bool, dev: int):
     """Logits as (rows, vocab, row stride): [rows, vocab] where packed, else
-    [nseq, n, vocab]; rows may be strided."""
-    _need(t, name)
-    if t.dim() != (2 if packed else 3):
+    [nseq, n, vocab]; rows may be strided, evenly."""
+    _here(t, name, BF16, dev)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != (2 if packed else 3):
         raise ValueError(f"{name} must be [rows, vocab] with cu_drafts, else [nseq, n, vocab]")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    vocab, n = shape[-1], shape[-2]
+    if vocab > 1 and stride[-1] != 1:
         raise ValueError(f"{name} must have unit column stride")
-    rows, vocab = t.shape[:-1].numel(), t.shape[-1]
-    ld = max(t.stride(-2), vocab) if t.shape[-2] > 1 else max(vocab, t.stride(0) if t.dim() == 3 else 0)
-    if rows > 1 and t.shape[-2] > 1 and t.stride(-2) < vocab:
+    if packed:
+        rows, ld = n, stride[0] if n > 1 else vocab
+    else:
+        rows = shape[0] * n
+        ld = stride[1] if n > 1 else stride[0] if shape[0] > 1 else vocab
+        if shape[0] > 1 and n > 1 and stride[0] != n * stride[1]:
+            raise ValueError(f"{name} rows must be evenly strided")
+    if rows > 1 and ld < vocab:
         raise ValueError(f"{name} rows must not overlap")
-    if not packed and t.shape[0] > 1 and t.shape[1] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
-        raise ValueError(f"{name} rows must be evenly strided")
-    return rows, vocab, ld
+    return rows, vocab, max(ld, vocab)
 
 
 def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept: torch.Tensor,
@@ -672,20 +678,22 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept
     fp32 [nseq] (temperature <= 0: greedy).  Top-k or top-p: set the logits that
     are out to -inf in both.  Returns (tokens int64 [nseq, max_drafts + 1]:
     accepted drafts, the drawn token, -1; accepted int32 [nseq])."""
+    dev = _device_for(target_logits, "target_logits", BF16)
     packed = cu_drafts is not None
-    rows, vocab, ldt = _logit_rows(target_logits, "target_logits", packed)
-    _need(draft_ids, "draft_ids", torch.int64)
-    _need(u_accept, "u_accept", torch.float32)
-    _need(u_final, "u_final", torch.float32)
-    _need(temperature, "temperature", torch.float32)
+    rows, vocab, ldt = _logit_rows(target_logits, "target_logits", packed, dev)
+    _here(draft_ids, "draft_ids", torch.int64, dev)
+    for t, nm in ((u_accept, "u_accept"), (u_final, "u_final"), (temperature, "temperature")):
+        _here(t, nm, torch.float32, dev)
+        if not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous")
     nd = draft_ids.numel()
     if packed:
-        _need(cu_drafts, "cu_drafts", torch.int32)
-        if cu_drafts.dim() != 1 or cu_drafts.numel() < 1 or not cu_drafts.is_contiguous():
+        _here(cu_drafts, "cu_drafts", torch.int32, dev)
+        if cu_drafts.dim() != 1 or cu_drafts.shape[0] < 1 or not cu_drafts.is_contiguous():
             raise ValueError("cu_drafts must be contiguous [nseq + 1]")
         if max_drafts is None or max_drafts < 0:
             raise ValueError("cu_drafts needs max_drafts")
-        nseq = cu_drafts.numel() - 1
+        nseq = cu_drafts.shape[0] - 1
         if draft_ids.dim() != 1 or rows != nd + nseq:
             raise ValueError("packed drafts need draft_ids [tokens] and tokens + nseq target rows")
     else:
@@ -694,29 +702,28 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept
         nseq, n = draft_ids.shape
         if target_logits.shape[0] != nseq or target_logits.shape[1] != n + 1:
             raise ValueError("target_logits must be [nseq, n + 1, vocab]")
-        max_drafts = n if max_drafts is None else int(max_drafts)
-        if max_drafts != n:
+        if max_drafts not in (None, n):
             raise ValueError("max_drafts goes with cu_drafts")
+        max_drafts = n
+    if not draft_ids.is_contiguous():
+        raise ValueError("draft_ids must be contiguous")
     if u_accept.numel() != nd or u_final.numel() != nseq or temperature.numel() != nseq:
         raise ValueError("u_accept needs one number per draft, u_final and temperature one per sequence")
-    for t, nm in ((draft_ids, "draft_ids"), (u_accept, "u_accept"), (u_final, "u_final"), (temperature, "temperature")):
-        if not t.is_contiguous():
-            raise ValueError(f"{nm} must be contiguous")
     ldd = 0
     if draft_logits is not None:
-        dr, dv, ldd = _logit_rows(draft_logits, "draft_logits", packed)
+        dr, dv, ldd = _logit_rows(draft_logits, "draft_logits", packed, dev)
         if dr != nd or dv != vocab or (not packed and nd and draft_logits.shape[:2] != draft_ids.shape):
             raise ValueError("draft_logits need one row of the target's vocabulary per draft")
-    _same_device(target_logits, draft_ids, u_accept, u_final, temperature, draft_logits, cu_drafts)
-    dev = target_logits.device
-    tok = torch.empty(nseq, max_drafts + 1, dtype=torch.int64, device=dev)
-    acc = torch.empty(nseq, dtype=torch.int32, device=dev)
+    device = target_logits.device
+    tok = torch.empty(nseq, max_drafts + 1, dtype=torch.int64, device=device)
+    acc = torch.empty(nseq, dtype=torch.int32, device=device)
     lib = _lib.load()
     need = lib.swl_verify_drafts_workspace(nseq, nd, vocab, 1 if draft_logits is not None else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.check(lib.swl_verify_drafts_bf16(
-        _ptr(target_logits), ldt, _ptr(draft_logits), ldd, vocab, _ptr(draft_ids), _ptr(cu_drafts), nseq, nd, max_drafts,
-        _ptr(temperature), _ptr(u_accept), _ptr(u_final), _ptr(tok), _ptr(acc), _ptr(ws), need, _stream()))
+        target_logits.data_ptr(), ldt, _addr(draft_logits), ldd, vocab, draft_ids.data_ptr(), _addr(cu_drafts), nseq, nd,
+        max_drafts, temperature.data_ptr(), u_accept.data_ptr(), u_final.data_ptr(), tok.data_ptr(), acc.data_ptr(),
+        ws.data_ptr(), need, _stream()))
     return tok, acc
 
 
@@ -885,45 +892,69 @@ def kv4_pages(num_blocks: int, block_size: int, hkv: int, device) -> torch.Tenso
     return torch.zeros(num_blocks, hkv, block_size // 16, KV4_RECORD, dtype=torch.uint8, device=device)
 
 
-def _kv4_cache(pages, block_table, lens, name, nseq, cu):
-    """Checks of what the kv4 calls share; nseq None: as many as cu says."""
-    _need(pages, "pages", torch.uint8)
-    if pages.dim() != 4 or pages.shape[3] != KV4_RECORD or not pages.is_contiguous():
+# The kv4 calls are short on the GPU (a decode step's append 3.4 us), so their
+# checks read every attribute once and pass plain addresses.
+if hasattr(torch._C, "_cuda_getDevice"):
+    _current_device = torch._C._cuda_getDevice
+else:
+    _current_device = torch.cuda.current_device
+
+
+def _device_for(t, name: str, dtype) -> int:
+    """The current device's index, for a call whose first tensor is t."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _need(t, name, dtype)
+    return _current_device()
+
+
+def _here(t, name: str, dtype, dev: int):
+    """t is a tensor of `dtype` on the current device (launches go to its
+    current stream)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != dev:
+        _need(t, name, dtype)
+        raise ValueError(f"{name} must be on the current device (cuda:{dev}), got {t.device}")
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def _kv4_cache(pages, block_table, lens, name, nseq, cu, dev):
+    """Checks of what the kv4 calls share; nseq is cu's where it is given.
+    Returns (nseq, blocks, kv heads, block size, table width)."""
+    _here(pages, "pages", torch.uint8, dev)
+    shape = pages.shape
+    if len(shape) != 4 or shape[3] != KV4_RECORD or not pages.is_contiguous():
         raise ValueError(f"pages must be contiguous [num_blocks, hkv, block_size / 16, {KV4_RECORD}]")
-    _need(block_table, "block_table", torch.int32)
-    _need(lens, name, torch.int32)
+    _here(block_table, "block_table", torch.int32, dev)
+    _here(lens, name, torch.int32, dev)
     if cu is not None:
-        _need(cu, "cu_seqlens", torch.int32)
-        if cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+        _here(cu, "cu_seqlens", torch.int32, dev)
+        if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
             raise ValueError("cu_seqlens must be contiguous [nseq + 1]")
-        nseq = cu.numel() - 1
-    if block_table.dim() != 2 or block_table.shape[0] < nseq or not block_table.is_contiguous():
+        nseq = cu.shape[0] - 1
+    bt = block_table.shape
+    if len(bt) != 2 or bt[0] < nseq or not block_table.is_contiguous():
         raise ValueError("block_table must be contiguous [nseq, max_blocks]")
-    if lens.dim() != 1 or lens.numel() < nseq or not lens.is_contiguous():
+    if lens.dim() != 1 or lens.shape[0] < nseq or not lens.is_contiguous():
         raise ValueError(f"{name} must be contiguous with nseq entries")
-    _same_device(pages, block_table, lens, cu)
-    return nseq
+    return nseq, shape[0], shape[1], shape[2] * 16, bt[1]
 
 
-def _same_device(*ts):
-    """All tensors on the current device (launches go to its current stream)."""
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.device.index != dev:
-            raise ValueError(f"tensors must be on the current device (cuda:{dev}), got {t.device}")
-
-
-def _packed_rows(t: torch.Tensor, name: str, cu):
+def _packed_rows(t: torch.Tensor, name: str, cu, dev):
     """Token rows as (tokens, heads, token stride): [nseq, L, heads, 128]
     without cu_seqlens, [tokens, heads, 128] with."""
-    _need(t, name)
-    if t.dim() != (4 if cu is None else 3) or t.shape[-1] != 128:
+    _here(t, name, BF16, dev)
+    shape = t.shape
+    if len(shape) != (4 if cu is None else 3) or shape[-1] != 128:
         raise ValueError(f"{name} must be [nseq, q_len, heads, 128], or [tokens, heads, 128] with cu_seqlens")
     if cu is None:
-        return t.shape[0] * t.shape[1], t.shape[2], _token_rows(t, name, t.shape[2], 128)
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128)):
+        return shape[0] * shape[1], shape[2], _token_rows(t, name, shape[2], 128)
+    n, heads, _ = shape
+    s0, s1, s2 = t.stride()
+    if n and heads and (s2 != 1 or (heads > 1 and s1 != 128)):
         raise ValueError(f"{name} heads must be contiguous within a token")
-    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * 128
+    return n, heads, s0 if n > 1 else heads * 128
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
@@ -938,20 +969,21 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
     (contiguous, q's shape; may be q itself) or a new tensor; k and v are left
     as they are.  Tokens behind the last sequence are not stored and their rows
     of q_out are left as they were."""
-    ntok, hkv, ks = _packed_rows(k, "k", cu_seqlens)
-    nv, hv, vs = _packed_rows(v, "v", cu_seqlens)
+    dev = _device_for(k, "k", BF16)
+    ntok, hkv, ks = _packed_rows(k, "k", cu_seqlens, dev)
+    _, _, vs = _packed_rows(v, "v", cu_seqlens, dev)
     if v.shape != k.shape:
         raise ValueError("k and v must have one shape")
-    nseq = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", None if cu_seqlens is not None else
-                      k.shape[0], cu_seqlens)
-    if pages.shape[1] != hkv:
+    nseq, nb, cache_heads, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", k.shape[0], cu_seqlens,
+                                               dev)
+    if cache_heads != hkv:
         raise ValueError("cache geometry mismatch")
     if (positions is None) != (cos_sin is None):
         raise ValueError("positions and cos_sin go together")
     max_pos = 0
     if positions is not None:
-        _need(positions, "positions", torch.int64)
-        _need(cos_sin, "cos_sin")
+        _here(positions, "positions", torch.int64, dev)
+        _here(cos_sin, "cos_sin", BF16, dev)
         if positions.numel() != ntok or not positions.is_contiguous():
             raise ValueError("positions must be contiguous with one entry per token")
         if cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous():
@@ -959,22 +991,21 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
         max_pos = cos_sin.shape[0]
     hq = qs = 0
     if q is not None:
-        nq, hq, qs = _packed_rows(q, "q", cu_seqlens)
+        _, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
         if q.shape[:-2] != k.shape[:-2]:
             raise ValueError("q, k and v must have the same tokens")
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
         else:
-            _need(q_out, "q_out")
+            _here(q_out, "q_out", BF16, dev)
             if q_out.shape != q.shape or not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous with q's shape")
     elif q_out is not None:
         raise ValueError("q_out needs q")
-    _same_device(k, v, positions, cos_sin, q, q_out)
     _lib.check(_lib.load().swl_kv4_append_bf16(
-        _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(q_out), nseq, ntok, _ptr(cu_seqlens), hq, hkv, 128, _ptr(pages),
-        pages.shape[0], pages.shape[2] * 16, _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens),
-        _ptr(positions), _ptr(cos_sin), max_pos, _stream()))
+        _addr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _addr(q_out), nseq, ntok, _addr(cu_seqlens), hq, hkv, 128,
+        pages.data_ptr(), nb, bs, block_table.data_ptr(), mb, cache_seqlens.data_ptr(), _addr(positions),
+        _addr(cos_sin), max_pos, _stream()))
     return q_out
 
 
@@ -987,17 +1018,22 @@ def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tenso
     sequence hold anything."""
     if count < 0:
         raise ValueError("count must not be negative")
-    _need(starts, "starts", torch.int32)
-    nseq = _kv4_cache(pages, block_table, starts, "starts", starts.numel(), cu_seqlens)
-    hkv = pages.shape[1]
+    dev = _device_for(starts, "starts", torch.int32)
+    _here(starts, "starts", torch.int32, dev)
+    nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, starts, "starts", starts.numel(), cu_seqlens, dev)
     shape = (count, hkv, 128) if cu_seqlens is not None else (nseq, count, hkv, 128)
     ntok = count if cu_seqlens is not None else nseq * count
     k = torch.empty(shape, dtype=BF16, device=pages.device)
-    v = torch.empty(shape, dtype=BF16, device=pages.device)
+    v = torch.empty_like(k)
     _lib.check(_lib.load().swl_kv4_read_bf16(
-        _ptr(pages), pages.shape[0], pages.shape[2] * 16, _ptr(block_table), block_table.shape[1], _ptr(starts), nseq,
-        ntok, _ptr(cu_seqlens), hkv, 128, _ptr(k), _ptr(v), _stream()))
+        pages.data_ptr(), nb, bs, block_table.data_ptr(), mb, starts.data_ptr(), nseq, ntok, _addr(cu_seqlens), hkv, 128,
+        k.data_ptr(), v.data_ptr(), _stream()))
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace(nseq: int, ntok: int, packed: int, max_q_len: int, hq: int, hkv: int, max_keys: int) -> int:
+    return _lib.load().swl_kv4_attention_workspace(nseq, ntok, packed, max_q_len, hq, hkv, max_keys)
 
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
@@ -1010,33 +1046,30 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     [tokens, hq * 128], rows behind the last sequence left as they were in
     `out`.  max_q_len: the most new tokens of a sequence where the host knows
     it (a hint for speed alone)."""
-    ntok, hq, qs = _packed_rows(q, "q", cu_seqlens)
-    nseq = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", None if cu_seqlens is not None else
-                      q.shape[0], cu_seqlens)
-    hkv = pages.shape[1]
+    dev = _device_for(q, "q", BF16)
+    ntok, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
+    nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", q.shape[0], cu_seqlens, dev)
     if hq < 1 or hkv < 1 or hq % hkv:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if cu_seqlens is None:
         max_q_len = q.shape[1]
-    elif max_q_len is None:
-        max_q_len = ntok
-    max_q_len = max(int(max_q_len), 1)
-    shape = (*q.shape[:-2], hq * 128)
-    if out is None:
-        out = torch.empty(shape, dtype=BF16, device=q.device)
+        shape = (*q.shape[:2], hq * 128)
     else:
-        _need(out, "out")
+        max_q_len = ntok if max_q_len is None else int(max_q_len)
+        shape = (ntok, hq * 128)
+    max_q_len = max(max_q_len, 1)
+    device = q.device
+    if out is None:
+        out = torch.empty(shape, dtype=BF16, device=device)
+    else:
+        _here(out, "out", BF16, dev)
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be contiguous [.., hq * 128] with q's tokens")
-    _same_device(q, out)
-    lib = _lib.load()
-    bs = pages.shape[2] * 16
-    need = lib.swl_kv4_attention_workspace(nseq, ntok, 0 if cu_seqlens is None else 1, max_q_len, hq, hkv,
-                                           block_table.shape[1] * bs)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.check(lib.swl_kv4_attention_bf16(
-        _ptr(q), qs, nseq, ntok, _ptr(cu_seqlens), max_q_len, hq, hkv, 128, _ptr(pages), pages.shape[0], bs,
-        _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens), float(softmax_scale), _ptr(out), _ptr(ws), need,
+    need = _kv4_workspace(nseq, ntok, 0 if cu_seqlens is None else 1, max_q_len, hq, hkv, mb * bs)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _lib.check(_lib.load().swl_kv4_attention_bf16(
+        q.data_ptr(), qs, nseq, ntok, _addr(cu_seqlens), max_q_len, hq, hkv, 128, pages.data_ptr(), nb, bs,
+        block_table.data_ptr(), mb, cache_seqlens.data_ptr(), float(softmax_scale), out.data_ptr(), _addr(ws), need,
         _stream()))
     return out
 

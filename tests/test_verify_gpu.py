@@ -198,6 +198,16 @@ def test_rows_that_are_no_numbers_and_drafts_outside_the_vocabulary(dev):
     assert got[0][0, 1] == 700 and got[0][1, 0] == 9 and got[0][2, 2] == 0
     c["temp"][:] = 0.0
     _same(c, dev)
+    # a NaN among masked logits, in a slice of nothing else
+    new, V = [1, 1], 20000
+    c = _case(13, new, V, True, [1.0])
+    c["u"][:] = 0.0
+    c["tgt"][:, 8:] = -math.inf
+    c["tgt"][1, 15000] = math.nan
+    c["tgt"][2, 15001] = math.nan
+    c["ids"][:] = 3
+    got = _same(c, dev)
+    assert got[0].tolist() == [[3, 15000], [15001, -1]]
 
 
 def test_drawn_tokens_follow_the_target(dev):
@@ -249,3 +259,28 @@ def test_captured_call_on_another_stream(dev):
         assert torch.equal(tok.cpu(), want[0]) and torch.equal(acc.cpu(), want[1])
         eager = call()
         assert torch.equal(eager[0], tok)
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+def test_random_numbers_next_to_the_border(dev, drafter):
+    """u so near to p / q that only 64 bits tell them apart (2^-15 to 2^-20 of
+    it, either side; u itself is rounded by 2^-24)."""
+    new, V = [5, 4, 20, 1, 3, 6], 4001
+    c = _case(41, new, V, drafter, [0.9, 1.4], near=0.8)
+    at = row = 0
+    edge = [2.0 ** -15, -2.0 ** -17, 2.0 ** -20, -2.0 ** -15, -2.0 ** -20, 2.0 ** -17]
+    near = 0
+    for s, n in enumerate(new):
+        t = float(c["temp"][s])
+        for j in range(n):
+            p, d = _soft(c["tgt"][row + j], t), int(c["ids"][at + j])
+            q = float(_soft(c["drf"][at + j], t)[d]) if drafter else 1.0
+            r = float(p[d]) / q
+            if r < 0.95:
+                # the last one refused; those before it accepted, however nearly
+                c["u"][at + j] = r * (1 + (-abs(edge[(at + j) % 6]) if j < n - 1 else edge[s]))
+                near += 1
+        at += n
+        row += n + 1
+    got = _same(c, dev)
+    assert near >= 12 and int(got[1].sum()) >= 12
