@@ -24,6 +24,7 @@ from .. import ext_unified_barrier as ub
 from .. import ops
 from .model_builder import OP_DOWN_PROJ, OP_EMBED, OP_GATE_UP_FUSED, OP_LM_HEAD, OP_O_PROJ, OP_QKV_FUSED
 from .model_builder import SyncRemoteLoRALinear
+from .paged_attention import PagedKVCache4
 
 
 class _NoStage:
@@ -109,7 +110,8 @@ class WorkerBatchedOps:
         GQA attention over the pages; returns {slot: [1, q_len, hidden]}.
         q/k/v may be views of the fused QKV output (read in place).  out (an
         addition): {slot: [1, q_len, hidden] bf16} to write a lone slot's
-        result into (a staged slot input buffer)."""
+        result into (a staged slot input buffer).  With a PagedKVCache4 the
+        tokens are stored in, and attended to from, 4 bits."""
         q_len = attn_meta["bufs_q"].shape[1]
         n = len(slot_ids)
 
@@ -121,6 +123,11 @@ class WorkerBatchedOps:
         k = gather(1, num_kv_heads)
         v = gather(2, num_kv_heads)
         dst = out.get(slot_ids[0]) if out is not None and n == 1 else None
+        if isinstance(paged_kv, PagedKVCache4):
+            pages, bt, lens = paged_kv.pages[layer_idx], attn_meta["block_tables"], attn_meta["cache_seqlens"]
+            q = ops.kv4_append(k, v, pages, bt, lens, attn_meta["positions"], cos_sin_cache, q=q)
+            out = ops.kv4_attention(q, pages, bt, lens, 1.0 / (head_dim ** 0.5), out=dst)
+            return {sid: out[i:i + 1] for i, sid in enumerate(slot_ids)}
         out = ops.paged_attention(q, k, v, paged_kv.key_caches[layer_idx], paged_kv.value_caches[layer_idx],
                                   attn_meta["block_tables"], attn_meta["cache_seqlens"], attn_meta["positions"],
                                   cos_sin_cache, 1.0 / (head_dim ** 0.5), out=dst)

@@ -4,7 +4,8 @@ Same class, constructor and methods as the reference's
 src/worker/paged_attention.py (PagedKVCache :7-128,
 build_vllm_cos_sin_cache :131-142).  Pages use the flash-attn layout
 [num_blocks, block_size, num_kv_heads, head_dim] the libswl attention kernel
-reads; freed pages are zeroed by a libswl kernel.
+reads; freed pages are zeroed by a libswl kernel.  PagedKVCache4 (an addition)
+holds the same cache in 4 bits.
 """
 
 import math
@@ -30,12 +31,19 @@ class PagedKVCache:
         self.dtype = dtype
         self.max_blocks_per_seq = (max_seq_len + block_size - 1) // block_size
         self.num_blocks = max_slots * self.max_blocks_per_seq
-        shape = (self.num_blocks, block_size, num_kv_heads, head_dim)
-        self.key_caches = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(num_layers)]
-        self.value_caches = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(num_layers)]
+        self._make_pools()
         self.free_blocks = list(range(self.num_blocks - 1, -1, -1))
         self.slot_block_tables: Dict[int, List[int]] = {}
         self.slot_seq_lens: Dict[int, int] = {}
+
+    def _make_pools(self):
+        shape = (self.num_blocks, self.block_size, self.num_kv_heads, self.head_dim)
+        self.key_caches = [torch.zeros(shape, device=self.device, dtype=self.dtype) for _ in range(self.num_layers)]
+        self.value_caches = [torch.zeros(shape, device=self.device, dtype=self.dtype) for _ in range(self.num_layers)]
+
+    def _pools(self) -> List[torch.Tensor]:
+        """Every pool as bf16 [num_blocks, ...]."""
+        return self.key_caches + self.value_caches
 
     def allocate_blocks(self, slot_id: int, num_blocks: int):
         if len(self.free_blocks) < num_blocks:
@@ -62,7 +70,7 @@ class PagedKVCache:
         if blocks:
             assert all(0 <= b < self.num_blocks for b in blocks)
             ids = torch.tensor(blocks, dtype=torch.int64, device=self.device)
-            ops.zero_blocks(self.key_caches + self.value_caches, ids)
+            ops.zero_blocks(self._pools(), ids)
         self.free_blocks.extend(blocks)
         self.slot_seq_lens.pop(slot_id, None)
 
@@ -85,6 +93,38 @@ class PagedKVCache:
     def advance_seq_lens_by(self, slot_ids: List[int], counts: List[int]):
         for sid, c in zip(slot_ids, counts):
             self.slot_seq_lens[sid] += c
+
+
+class PagedKVCache4(PagedKVCache):
+    """PagedKVCache whose pages hold keys and values in 4 bits (ops.kv4_pages:
+    codes with a scale per 32 dims, 68 bytes a token and head instead of 256
+    each): same methods, `pages` per layer in place of key_caches and
+    value_caches.  WorkerBatchedOps.batch_flash_attention and WorkerEngine take
+    it in place of the bf16 cache.  head_dim 128, block_size a multiple of 16."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int, max_slots: int,
+                 max_seq_len: int, device, dtype: torch.dtype = torch.bfloat16):
+        if head_dim != 128 or dtype != torch.bfloat16:
+            raise ValueError("the 4-bit cache takes bf16 heads of 128 dims")
+        super().__init__(num_layers, num_kv_heads, head_dim, block_size, max_slots, max_seq_len, device, dtype)
+
+    def _make_pools(self):
+        self.pages = [ops.kv4_pages(self.num_blocks, self.block_size, self.num_kv_heads, self.device)
+                      for _ in range(self.num_layers)]
+
+    def _pools(self) -> List[torch.Tensor]:
+        return [p.view(torch.bfloat16) for p in self.pages]
+
+    def read(self, slot_id: int, layer_idx: int, start: int = 0, count: Optional[int] = None):
+        """(k, v) bf16 [count, num_kv_heads, head_dim] of a slot's cached tokens
+        start .. (all by default): what the 4 bits stand for, exactly."""
+        if count is None:
+            count = self.slot_seq_lens[slot_id] - start
+        if start < 0 or count < 0 or start + count > self.slot_seq_lens[slot_id]:
+            raise ValueError("tokens outside the slot's length")
+        k, v = ops.kv4_read(self.pages[layer_idx], self.get_block_table_tensor([slot_id]),
+                            torch.tensor([start], dtype=torch.int32).to(self.device), count)
+        return k[0], v[0]
 
 
 def build_vllm_cos_sin_cache(rotary_emb, max_seq_len: int, device, dtype: torch.dtype) -> torch.Tensor:

@@ -124,3 +124,27 @@ def test_oracle_encoding_is_nearest_and_least():
                 seen.add((_kv4.scale_at(t, g, value), 0))
                 seen.add((_kv4.scale_at(t, g, value), 4))
     assert len(seen) == 2 * _kv4.REC
+
+
+def test_cache_of_four_bits_allocates_as_the_bf16_one():
+    from swarmlora_amd.worker.paged_attention import PagedKVCache, PagedKVCache4
+    c4 = PagedKVCache4(2, 2, 128, 16, 3, 100, "cpu")
+    c16 = PagedKVCache(2, 2, 128, 16, 3, 100, "cpu", torch.bfloat16)
+    assert len(c4.pages) == 2 and c4.pages[0].shape == (21, 2, 1, 2176)
+    for c in (c4, c16):
+        c.ensure_blocks_for_length(1, 17)
+        c.ensure_blocks_for_length(0, 100)
+        c.ensure_blocks_for_length(1, 33)
+        c.advance_seq_lens([0, 1], 5)
+    assert c4.slot_block_tables == c16.slot_block_tables and c4.slot_seq_lens == c16.slot_seq_lens
+    assert torch.equal(c4.get_block_table_tensor([1, 0]), c16.get_block_table_tensor([1, 0]))
+    with pytest.raises(RuntimeError, match="max_seq_len"):
+        c4.ensure_blocks_for_length(0, 113)
+    with pytest.raises(ValueError, match="128 dims"):
+        PagedKVCache4(1, 2, 64, 16, 1, 64, "cpu")
+    with pytest.raises(ValueError, match="128 dims"):
+        PagedKVCache4(1, 2, 128, 16, 1, 64, "cpu", torch.float16)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        PagedKVCache4(1, 2, 128, 24, 1, 64, "cpu")
+    with pytest.raises(ValueError, match="outside"):
+        c4.read(0, 0, 3, 3)

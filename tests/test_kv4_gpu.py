@@ -279,6 +279,30 @@ def test_attention_uniform_strided_and_a_wrong_hint(dev, L):
     _check(low, want, wt, 2.0 ** -7)
 
 
+def test_prompt_attention_whose_reference_is_left_far_behind(dev):
+    """Rows of many: scores that grow along the keys by far more than 2^100,
+    scores far below those of the first keys, and first pages that are missing
+    in front of scores far below zero (the running maximum has to take over)."""
+    ops = _ops()
+    L, hq, hkv = 200, 4, 1
+    for kind in range(3):
+        bt, nb = _tables([L], 16, 61 + kind)
+        k, v, q = randn((L, hkv, 128), 1), randn((L, hkv, 128), 2), randn((L, hq, 128), 3).abs()
+        ramp = torch.linspace(0.0, 60.0, L).view(-1, 1, 1)
+        sign = 1.0 if kind == 0 else -1.0
+        k = (k.abs() * ramp * sign if kind < 2 else -k.abs() * 60).to(BF16)
+        pages = ops.kv4_pages(nb, 16, hkv, "cuda")
+        zero = torch.zeros(1, dtype=torch.int32, device=dev)
+        cu = torch.tensor([0, L], dtype=torch.int32, device=dev)
+        ops.kv4_append(k.to(dev), v.to(dev), pages, bt.to(dev), zero, cu_seqlens=cu)
+        if kind == 2:
+            bt[0, :3] = -1
+        out = ops.kv4_attention(q.to(dev), pages, bt.to(dev), zero, SCALE, cu_seqlens=cu)
+        want, wt = _kv4.attend(q, pages.cpu(), bt, [0], [0, L], SCALE)
+        # sum |q k| up to 0.8 * 0.8 * 60 * 128 * scale = 440 before log2: its fp32 rounding, 2^-22 of it, moves p
+        _check(out, want, wt, 2.0 ** -7 + 2.0 ** -22 * 440 * 8)
+
+
 def test_attention_over_missing_pages_and_empty_rows(dev):
     ops = _ops()
     ctx, new = [300, 40, 20, 64], [1, 6, 40, 3]
@@ -455,3 +479,43 @@ def test_two_streams_at_once(dev):
         for o in outs[i]:
             assert torch.equal(o, outs[i][0])
         _check(outs[i][0], *res[i], 2.0 ** -7)
+
+
+def test_worker_attention_over_a_cache_of_four_bits(dev):
+    """WorkerBatchedOps.batch_flash_attention with a PagedKVCache4: prompts of
+    two slots, then single tokens, one slot read back and freed."""
+    from swarmlora_amd.worker.batched_ops import WorkerBatchedOps
+    from swarmlora_amd.worker.paged_attention import PagedKVCache4
+    hq, hkv, layers = 8, 2, 2
+    kv = PagedKVCache4(layers, hkv, 128, 16, 3, 128, dev)
+    cs = _cos_sin(128)
+    refs = [p.cpu() for p in kv.pages]
+    for step, q_len in enumerate([33, 1, 1]):
+        sids = [2, 0]
+        for s in sids:
+            kv.ensure_blocks_for_length(s, kv.slot_seq_lens.get(s, 0) + q_len)
+        lens = kv.get_seq_lens_tensor(sids)
+        bt = kv.get_block_table_tensor(sids)
+        pos = (lens.long().unsqueeze(1) + torch.arange(q_len, device=dev)).reshape(-1)
+        meta = {"cache_seqlens": lens, "block_tables": bt, "positions": pos, "bufs_q": torch.empty(2, q_len, 0, device=dev)}
+        for layer in range(layers):
+            rows = {s: randn((1, q_len, (hq + 2 * hkv) * 128), 100 * step + 10 * layer + s) for s in sids}
+            qkv = {s: r.to(dev).split([hq * 128, hkv * 128, hkv * 128], -1) for s, r in rows.items()}
+            got = WorkerBatchedOps.batch_flash_attention(sids, qkv, kv, cs.to(dev), layer, hq, hkv, 128, meta)
+            q, k, v = (torch.cat([rows[s][0] for s in sids]).split([hq * 128, hkv * 128, hkv * 128], -1)[i].unflatten(1, (-1, 128))
+                       for i in range(3))
+            at = pos.cpu()
+            kr, qr = _kv4.rotate(k, cs[at]), _kv4.rotate(q, cs[at]).to(BF16)
+            for t in range(2 * q_len):
+                _kv4.store(refs[layer], bt.cpu(), t // q_len, int(at[t]), kr[t], v[t].double())
+            assert torch.equal(kv.pages[layer].cpu(), refs[layer])
+            want, wt = _kv4.attend(qr, refs[layer], bt.cpu(), lens.tolist(), [0, q_len, 2 * q_len], SCALE)
+            _check(torch.cat([got[s] for s in sids]).view(2 * q_len, -1), want, wt, 2.0 ** -7)
+        kv.advance_seq_lens(sids, q_len)
+    k, v = kv.read(0, 1, 30)
+    rk, rv, _ = _kv4.load(refs[1], kv.get_block_table_tensor([0]).cpu(), 0, 35)
+    assert torch.equal(k.cpu().double(), rk[30:]) and torch.equal(v.cpu().double(), rv[30:])
+    blocks = list(kv.slot_block_tables[2])
+    kv.free_slot(2)
+    for p in kv.pages:
+        assert not bool(p[blocks].any()) and bool(p[kv.slot_block_tables[0]].any())
