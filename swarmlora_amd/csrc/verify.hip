@@ -108,7 +108,7 @@ constexpr int kPow = 256;  // entries of the table of 2^(k / 256)
 __device__ __forceinline__ double weight(uint32_t bits, float mx, double rate, const double* tab) {
   constexpr double c = 0.693147180559945309417232121458 / kPow;  // ln 2 / 256
   constexpr double c2 = c * c;
-  const double x = __uint_as_float(bits == 0xff80u ? 0xff7f0000u : bits << 16);  // (-inf: the lowest number)
+  const double x = __uint_as_float(bits == 0xff80u ? 0xff7f0000u : bits << 16);  // (-inf: no NaN from a rate of 0)
   const double y = (x - (double)mx) * rate, n = rint(y), f = y - n;
   const int k = (int)n;
   double r = c2 * c2 / 24;
@@ -116,7 +116,7 @@ __device__ __forceinline__ double weight(uint32_t bits, float mx, double rate, c
   r = fma(r, f, c2 / 2);
   r = fma(r, f, c);
   r = fma(r, f, 1.0);
-  return ldexp(r * tab[k & (kPow - 1)], k >> 8);
+  return bits == 0xff80u ? 0.0 : ldexp(r * tab[k & (kPow - 1)], k >> 8);
 }
 __device__ __forceinline__ double rate_of(float temp) {
   return kPow * 1.44269504088896340735992468100 / (double)temp;

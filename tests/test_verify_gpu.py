@@ -210,6 +210,28 @@ def test_rows_that_are_no_numbers_and_drafts_outside_the_vocabulary(dev):
     assert got[0].tolist() == [[3, 15000], [15001, -1]]
 
 
+@pytest.mark.parametrize("temp", [3e38, math.inf])
+def test_masked_tokens_stay_out_whatever_the_temperature(dev, temp):
+    """-inf logits weigh 0 where the temperature makes all others alike."""
+    ops, V = _ops(), 1003
+    keep = torch.tensor([5, 17, 400, 1002])
+    tgt = torch.full((2, V), -math.inf, dtype=BF16)
+    tgt[:, keep] = torch.tensor([1.0, -3.0, 2.0, 0.5]).to(BF16)
+    for u_last, want in ((0.1, 5), (0.3, 17), (0.6, 400), (0.9, 1002)):
+        for drf in (None, tgt[:1].to(dev)):
+            for d, u in ((400, 0.2), (3, 0.0)):  # accepted (p = 1 / 4); refused, and p is drawn from
+                tok, acc = ops.verify_drafts(
+                    tgt.to(dev).view(1, 2, V), torch.tensor([[d]], device=dev), torch.tensor([u], device=dev),
+                    torch.tensor([u_last], device=dev), torch.tensor([temp], device=dev),
+                    drf.view(1, 1, V) if drf is not None else None)
+                if d == 400:
+                    assert tok.tolist() == [[400, want]] and acc.tolist() == [1]
+                elif drf is None:
+                    assert tok.tolist() == [[want, -1]] and acc.tolist() == [0]
+                else:  # p - q leaves nothing: the first largest logit
+                    assert tok.tolist() == [[400, -1]] and acc.tolist() == [0]
+
+
 def test_drawn_tokens_follow_the_target(dev):
     """Over 20000 requests of the same two rows the first token (draft or
     drawn) has the target's distribution whatever the drafter's is: every
