@@ -125,7 +125,7 @@ def _same(c, dev, max_drafts=None):
     ([1, 5, 3, 2], 128256, [0.6, 1.0, 0.0], 0),
     ([2] * 70, 3000, [1.0, 0.9, 0.0, 2.0], 0),               # more than 64 sequences
     ([40, 17, 33], 500, [3.0, 8.0], 3),                      # more drafts than sixteen
-    ([3] * 180, 16500, [0.9], 0),                            # slices of 8192
+    ([3] * 180, 16500, [0.9], 0),                            # rows of more than one slice
 ])
 def test_tokens_and_counts_equal_the_rule(dev, new, vocab, temps, pad, drafter):
     for seed in range(3):
