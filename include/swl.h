@@ -415,10 +415,10 @@ int swl_paged_attention_rows_bf16(void* const* qkv_rows, void* const* out_rows, 
  *   2112 + 16 (t / 4) + 4 (d / 32) + t % 4          value scales
  * Zeroed pages hold zeros.
  * New tokens are packed: sequence s has tokens cu_seqlens[s] ..
- * cu_seqlens[s + 1] - 1 of the ntok (device int32 [nseq + 1], ascending from
- * 0; sequences may be empty, tokens from cu_seqlens[nseq] on belong to none and
- * their outputs are left as they were); cu_seqlens NULL: ntok / nseq tokens
- * each.  cache_seqlens [nseq] int32: tokens of the sequence before its new
+ * cu_seqlens[s + 1] - 1 of the ntok (under 2^25; device int32 [nseq + 1],
+ * ascending from 0; sequences may be empty, tokens from cu_seqlens[nseq] on
+ * belong to none and their outputs are left as they were); cu_seqlens NULL:
+ * ntok / nseq tokens each.  cache_seqlens [nseq] int32: tokens of the sequence before its new
  * ones; new token i of sequence s is token cache_seqlens[s] + i, in page
  * block_table[s][that / block_size] (int32 [nseq, max_blocks]).  A token whose
  * page is outside the table, or outside 0 .. num_blocks - 1, has no place: it
@@ -450,15 +450,16 @@ int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, con
 /* Causal attention of the new tokens (already appended) over the cache: query
  * i of sequence s sees tokens 0 .. cache_seqlens[s] + i; query head j reads kv
  * head j / (hq / hkv), any hq that is a multiple of hkv.  out [ntok, hq *
- * 128].  Sums and softmax in fp32.  A query that sees no token gets zeros, one
- * with an infinity or a NaN, or that sees a NaN key, NaN; a NaN value group
- * reaches the queries that see it.  Values must leave room for their sum (under
- * 2^118 / tokens).
+ * 128], not q's memory.  Sums and softmax in fp32.  A query that sees no token
+ * gets zeros, one with an infinity or a NaN, or that sees a NaN key, NaN; a NaN
+ * value group reaches the queries that see it.  Values must leave room for
+ * their sum (under 2^118 / tokens).
  * max_q_len: the most new tokens of a sequence (a hint for speed alone: it
  * chooses between kernels, any value >= 1 gives a right result).
  * workspace: swl_kv4_attention_workspace(nseq, ntok, cu_seqlens != NULL,
- * max_q_len, hq, hkv, max_blocks * block_size) bytes of device memory, 16-byte aligned, owned by
- * the call until its kernels have run; its contents do not matter. */
+ * max_q_len, hq, hkv, max_blocks * block_size) bytes of device memory, 16-byte
+ * aligned, owned by the call until its kernels have run; its contents do not
+ * matter. */
 int64_t swl_kv4_attention_workspace(int nseq, int64_t ntok, int packed, int64_t max_q_len, int hq, int hkv,
                                     int64_t max_keys);
 int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t ntok, const int32_t* cu_seqlens,

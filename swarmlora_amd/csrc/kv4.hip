@@ -1313,7 +1313,7 @@ int kv4_check_pages(const char* what, const void* pages, int64_t num_blocks, int
                     const int32_t* block_table, int64_t max_blocks, const int32_t* cache_seqlens, int nseq, int64_t T,
                     const int32_t* cu, int hkv) {
   auto bad = [&](const char* m) { return swl::fail(SWL_ERR_INVALID, std::string(what) + ": " + m); };
-  if (nseq < 0 || T < 0 || T >= ((int64_t)1 << 31)) return bad("bad sequence or token count");
+  if (nseq < 0 || T < 0 || T >= ((int64_t)1 << 25)) return bad("bad sequence or token count");
   if (hkv < 1 || hkv > 4096) return bad("bad head counts");
   if (block_size < 16 || block_size % 16 != 0 || block_size > (1 << 20))
     return bad("block_size must be a multiple of 16");
@@ -1372,6 +1372,8 @@ extern "C" int swl_kv4_append_bf16(const void* q, int64_t q_stride, const void* 
   SWL_CHECK(k && v, SWL_ERR_INVALID, "swl_kv4_append_bf16: null argument");
   SWL_CHECK((!q || q_stride >= (int64_t)hq * d) && k_stride >= (int64_t)hkv * d && v_stride >= (int64_t)hkv * d,
             SWL_ERR_INVALID, "swl_kv4_append_bf16: token strides smaller than a token row");
+  SWL_CHECK(q != q_out || !q || q_stride == (int64_t)hq * d, SWL_ERR_INVALID,
+            "swl_kv4_append_bf16: q_out may be q only where its rows are hq * 128 apart");
   SWL_CHECK(aligned16(k) && aligned16(v) && (k_stride & 7) == 0 && (v_stride & 7) == 0 &&
                 (!q || (aligned16(q) && aligned16(q_out) && (q_stride & 7) == 0)) && aligned16(cos_sin),
             SWL_ERR_INVALID, "swl_kv4_append_bf16: q, k, v rows and cos_sin must be 16-byte aligned");
@@ -1440,6 +1442,7 @@ extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq,
   SWL_CHECK(ntok * (int64_t)(hq / hkv) < ((int64_t)1 << 31), SWL_ERR_INVALID,
             "swl_kv4_attention_bf16: too many rows");
   SWL_CHECK(q && out, SWL_ERR_INVALID, "swl_kv4_attention_bf16: null argument");
+  SWL_CHECK(q != out, SWL_ERR_INVALID, "swl_kv4_attention_bf16: out must not be q");
   SWL_CHECK(q_stride >= (int64_t)hq * d && (q_stride & 7) == 0 && aligned16(q) && aligned16(out), SWL_ERR_INVALID,
             "swl_kv4_attention_bf16: q and out rows must be 16-byte aligned, a token's heads together");
   Kv4Args a = kv4_args(const_cast<void*>(pages), num_blocks, block_size, block_table, max_blocks, cache_seqlens, nseq,
@@ -1453,7 +1456,7 @@ extern "C" int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq,
   a.out = reinterpret_cast<bf16*>(out);
   if (!cu_seqlens) max_q_len = ntok / nseq;
   const Kv4Plan p = kv4_plan(nseq, ntok, cu_seqlens != nullptr, max_q_len, hq, hkv, max_blocks * block_size);
-  SWL_CHECK(p.few.units + p.many.units < ((int64_t)1 << 31), SWL_ERR_INVALID,
+  SWL_CHECK(p.few.units + p.many.units < ((int64_t)1 << 24), SWL_ERR_INVALID,
             "swl_kv4_attention_bf16: too many rows");
   const int64_t need = p.few.bytes + p.many.bytes;
   SWL_CHECK(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), SWL_ERR_INVALID,

@@ -44,7 +44,8 @@ def _append(lib, **kw):
     (dict(pos=None), "go together"), (dict(mp=0), "go together"), (dict(k=None), "null"), (dict(pages=None), "null"),
     (dict(lens=None), "null"), (dict(ks=255), "strides"), (dict(qs=1016), "strides"), (dict(vs=260), "aligned"),
     (dict(k=P + 2), "aligned"), (dict(pages=P + 8), "aligned"), (dict(ntok=5), "as many tokens"), (dict(nseq=-1), "count"),
-    (dict(cs=P + 4), "aligned"), (dict(mb=1 << 40), "page geometry"),
+    (dict(cs=P + 4), "aligned"), (dict(mb=1 << 40), "page geometry"), (dict(qs=1280, qo=P), "rows are hq"),
+    (dict(ntok=1 << 25), "token count"),
 ])
 def test_append_refusals(kw, text):
     lib = _lib().load()
@@ -63,11 +64,12 @@ def test_nothing_to_do_is_no_error():
     (dict(scale=-1.0), "softmax_scale"), (dict(scale=math.inf), "softmax_scale"), (dict(scale=math.nan), "softmax_scale"),
     (dict(mq=0), "max_q_len"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(qs=1000), "aligned"),
     (dict(ws=None), "workspace"), (dict(wsb=100), "workspace"), (dict(bs=8), "multiple of 16"), (dict(q=P + 2), "aligned"),
+    (dict(out=P), "must not be q"), (dict(nseq=1, ntok=1 << 24, hq=256, hkv=256, qs=1 << 15), "too many rows"),
 ])
 def test_attention_refusals(kw, text):
     lib = _lib().load()
     a = dict(q=P, qs=1024, nseq=2, ntok=4, cu=None, mq=2, hq=8, hkv=2, d=128, pages=P, nb=4, bs=16, bt=P, mb=4096, lens=P,
-             scale=0.1, out=P, ws=P, wsb=1 << 40)
+             scale=0.1, out=2 * P, ws=P, wsb=1 << 40)
     a.update(kw)
     rc = lib.swl_kv4_attention_bf16(a["q"], a["qs"], a["nseq"], a["ntok"], a["cu"], a["mq"], a["hq"], a["hkv"], a["d"],
                                     a["pages"], a["nb"], a["bs"], a["bt"], a["mb"], a["lens"], a["scale"], a["out"], a["ws"],
