@@ -1221,9 +1221,7 @@ __global__ __launch_bounds__(256) void kv4_combine_mixed_kernel(Kv4Args many, Kv
 
 // ------------------------------------------------------------- launchers ---
 // Geometry of one attention call, from shapes alone: bounds that hold for
-// every set of lengths (steps_per_part).  Sequences of at most kSplitRows rows
-// go to the kernel for few rows, the others to the one for many; a call whose
-// hint says that there are none of the others leaves them all to the first.
+// every set of lengths (steps_per_part).
 struct Kv4Launch {
   bool on;
   int rb, slots, min_spp, row_lo, row_hi;
@@ -1232,10 +1230,20 @@ struct Kv4Launch {
 struct Kv4Plan {
   Kv4Launch few, many;
 };
+// Sequences of at most kSplitRows rows go to the kernel for few rows: 28 with
+// 64 rows over 4000 keys 53 us there, 71 in the one for many; 8 with 96 over
+// 16000 keys 91 and 75, over 4000 37 and 35.  So do all sequences of a call
+// that cannot have more than kFewScores scores (tokens x keys of a table x query
+// heads), for it starts sooner and is cut finer: one sequence of 512 tokens over
+// 1500 keys (2^24.6 scores) 30 and 40 us, 128 over 4000 (2^24) 28 and 35, 64
+// over 16000 (2^25) 38 and 44; but 300 over 4000 (2^25.2) 51 and 45, two of 64
+// over 16000 (2^26) 55 and 50.
 constexpr int kSplitRows = 64;
+constexpr double kFewScores = 0x1p25;
 constexpr int kCus = 256;  // of an MI355X
-// Workgroups of a CU (registers), and steps of a part at least (16 of 32 keys:
-// four a wave; 28 single tokens over 128 to 2048 keys with 8: 21.8 us, 16: 17)
+// Workgroups of a CU (registers), and steps of a part at least.  16 of 32 keys,
+// four a wave: 28 single tokens over 128 to 2048 keys 17 us, with 8 21.8.  8 of
+// 64 keys: 300 tokens alone 14 us, with 4 18.5; over 500 keys 25 and 28.
 constexpr int kSplit1PerCu = 4, kSplit2PerCu = 2, kPromptPerCu = 2, kSplitSteps = 16, kPromptSteps = 8;
 
 Kv4Launch kv4_launch(int64_t nseq, int64_t T, int G, int hkv, int64_t max_keys, int64_t max_rows, int rb, int ks,
@@ -1258,10 +1266,11 @@ Kv4Plan kv4_plan(int64_t nseq, int64_t T, bool packed, int64_t max_q_len, int hq
   Kv4Plan p{};
   const int G = hq / hkv;
   const int64_t most = std::min(max_q_len, T) * G;
-  if (most <= kSplitRows || packed)  // (a packed call's hint may be too small: its rows are bounded by T alone)
-    p.few = kv4_launch(nseq, T, G, hkv, max_keys, most > kSplitRows ? kSplitRows : packed ? T * G : most,
-                       most <= 16 ? 16 : 32, 32, most <= 16 ? kSplit1PerCu : kSplit2PerCu, kSplitSteps);
-  if (most > kSplitRows) {
+  const bool few = most <= kSplitRows || (double)T * (double)max_keys * hq <= kFewScores;
+  if (few || packed)  // (a packed call's hint may be too small: its rows are bounded by T alone)
+    p.few = kv4_launch(nseq, T, G, hkv, max_keys, !few ? kSplitRows : packed ? T * G : most, most <= 16 ? 16 : 32, 32,
+                       most <= 16 ? kSplit1PerCu : kSplit2PerCu, kSplitSteps);
+  if (!few) {
     p.many = kv4_launch(nseq, T, G, hkv, max_keys, T * G, kPromptRows, kPromptKeys, kPromptPerCu, kPromptSteps);
     p.few.row_hi = p.many.row_lo = packed ? kSplitRows : 0;
   }

@@ -5,8 +5,8 @@ Stored bytes are compared exactly: products of two bf16 are exact in fp32, so
 the kernel's rotated keys carry one fp32 rounding, and a code differs from the
 64-bit rule's only where that moves a value across a border (the seeds here
 have none).  Attention, per element: half a step of the result's bf16 (2^-8 of
-it), and relative to A = sum p |v|: the probabilities' rounding (2^-17 for two
-bf16, 2^-8 for one, in kernels of many rows), fp32 scores (128 products of up
+it), and relative to A = sum p |v|: the probabilities' rounding to bf16 (2^-8,
+of the terms and of their sum 2^-7 together at most), fp32 scores (128 products of up
 to 6 * 4 in units that sum to under 200 before the scale: 2^-24 * 200 * 4 twice,
 under 2^-12) and sums over the keys (2^-24 * keys, under 2^-11 for 8192).
 """
@@ -39,6 +39,12 @@ def _tables(total, page, seed, spare=2):
         bt[s, :n] = perm[at:at + n]
         at += n
     return bt, nb
+
+
+def _wide(bt, wide=True):
+    """The table with columns of no page, to 2^21 keys and more: a call that could
+    be large by its shapes, which takes the kernels for many rows."""
+    return torch.cat([bt, bt.new_full((bt.shape[0], (1 << 17) - bt.shape[1]), -1)], 1) if wide else bt
 
 
 def _prefix(counts):
@@ -248,12 +254,12 @@ def test_attention_matches_the_definition(dev, ctx, new, hq, hkv, page):
     cu = _prefix(new)
     out = torch.full((T + extra, hq * 128), 5.0, dtype=BF16, device=dev)
     lens = torch.tensor(ctx, dtype=torch.int32)
-    for hint in (max(new), None):
+    want, wt = _kv4.attend(q[:T], pages.cpu(), bt, ctx, cu.tolist(), SCALE)
+    for hint, wide in ((max(new), False), (None, False), (max(new), True), (None, True)):
         out.fill_(5.0)
-        got = ops.kv4_attention(q.to(dev), pages, bt.to(dev), lens.to(dev), SCALE, cu_seqlens=cu.to(dev), max_q_len=hint,
-                                out=out)
+        got = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), lens.to(dev), SCALE, cu_seqlens=cu.to(dev),
+                                max_q_len=hint, out=out)
         assert got is out
-        want, wt = _kv4.attend(q[:T], pages.cpu(), bt, ctx, cu.tolist(), SCALE)
         _check(out[:T], want, wt, 2.0 ** -7)
         assert bool((out[T:] == 5.0).all())
 
@@ -269,10 +275,10 @@ def test_attention_uniform_strided_and_a_wrong_hint(dev, L):
     rows = randn((n, L, (hq + 4) * 128), 4, 2.0)
     q = rows.to(dev)[..., :hq * 128].unflatten(-1, (hq, 128))
     lens = torch.tensor(ctx, dtype=torch.int32, device=dev)
-    out = ops.kv4_attention(q, pages, bt.to(dev), lens, SCALE)
     cu = [i * L for i in range(n + 1)]
     want, wt = _kv4.attend(q.cpu().reshape(n * L, hq, 128), pages.cpu(), bt, ctx, cu, SCALE)
-    _check(out, want, wt, 2.0 ** -7)
+    for wide in (False, True):
+        _check(ops.kv4_attention(q, pages, _wide(bt, wide).to(dev), lens, SCALE), want, wt, 2.0 ** -7)
     packed = q.reshape(n * L, hq, 128)
     low = ops.kv4_attention(packed, pages, bt.to(dev), lens, SCALE, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev),
                             max_q_len=1)
@@ -297,10 +303,11 @@ def test_prompt_attention_whose_reference_is_left_far_behind(dev):
         ops.kv4_append(k.to(dev), v.to(dev), pages, bt.to(dev), zero, cu_seqlens=cu)
         if kind == 2:
             bt[0, :3] = -1
-        out = ops.kv4_attention(q.to(dev), pages, bt.to(dev), zero, SCALE, cu_seqlens=cu)
         want, wt = _kv4.attend(q, pages.cpu(), bt, [0], [0, L], SCALE)
-        # sum |q k| up to 0.8 * 0.8 * 60 * 128 * scale = 440 before log2: its fp32 rounding, 2^-22 of it, moves p
-        _check(out, want, wt, 2.0 ** -7 + 2.0 ** -22 * 440 * 8)
+        for wide in (False, True):
+            out = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), zero, SCALE, cu_seqlens=cu)
+            # sum |q k| up to 0.8 * 0.8 * 60 * 128 * scale = 440 before log2: its fp32 rounding, 2^-22 of it, moves p
+            _check(out, want, wt, 2.0 ** -7 + 2.0 ** -22 * 440 * 8)
 
 
 def test_attention_over_missing_pages_and_empty_rows(dev):
@@ -311,11 +318,12 @@ def test_attention_over_missing_pages_and_empty_rows(dev):
     bt[3, 2] = pages.shape[0] + 5  # past the pool
     q = randn((sum(new), 8, 128), 3, 2.0)
     cu = _prefix(new)
-    out = ops.kv4_attention(q.to(dev), pages, bt.to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev), SCALE,
-                            cu_seqlens=cu.to(dev))
     want, wt = _kv4.attend(q, pages.cpu(), bt, ctx, cu.tolist(), SCALE)
-    _check(out, want, wt, 2.0 ** -7)
-    assert bool((out[1:7] == 0).all())  # the second sequence has no page at all
+    for wide in (False, True):
+        out = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev),
+                                SCALE, cu_seqlens=cu.to(dev))
+        _check(out, want, wt, 2.0 ** -7)
+        assert bool((out[1:7] == 0).all())  # the second sequence has no page at all
 
 
 def test_attention_lengths_past_the_table_or_negative(dev):
@@ -351,10 +359,11 @@ def test_attention_nan_reaches_only_the_rows_that_see_it(dev, new):
     q = randn((sum(new), hq, 128), 3, 2.0)
     q[0, 7, 3] = math.nan
     cu = _prefix(new)
-    out = ops.kv4_attention(q.to(dev), pages, bt.to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev), SCALE,
-                            cu_seqlens=cu.to(dev))
     want, wt = _kv4.attend(q, pages.cpu(), bt, ctx, cu.tolist(), SCALE)
-    _check(out, want, wt.nan_to_num(0.0), 2.0 ** -7)
+    for wide in (False, True):
+        out = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev),
+                                SCALE, cu_seqlens=cu.to(dev))
+        _check(out, want, wt.nan_to_num(0.0), 2.0 ** -7)
     assert bool(torch.isnan(want).any()) and not bool(torch.isnan(want).all())
 
 
@@ -403,7 +412,8 @@ def test_chunks_tokens_and_drafts_of_one_cache(dev):
         dr = rows.to(dev)
         dq, dk, dv = (x.unflatten(1, (-1, 128)) for x in dr.split([hq * 128, hkv * 128, hkv * 128], 1))
         rot = ops.kv4_append(dk, dv, pages, bt.to(dev), lens.to(dev), pos.to(dev), cs.to(dev), q=dq, cu_seqlens=cu.to(dev))
-        out = ops.kv4_attention(rot, pages, bt.to(dev), lens.to(dev), SCALE, cu_seqlens=cu.to(dev), max_q_len=max(new))
+        out = ops.kv4_attention(rot, pages, _wide(bt, i == 0).to(dev), lens.to(dev), SCALE, cu_seqlens=cu.to(dev),
+                                max_q_len=max(new))
         kr = _kv4.rotate(k, cs[pos])
         for t in range(T):
             _kv4.store(ref, bt, seq[t], int(pos[t]), kr[t], v[t].double())
