@@ -153,7 +153,9 @@ __device__ __forceinline__ uint32_t top8(const float (&x)[8]) {
 // as 4-bit groups to the pages.  A 128-thread workgroup per (token, 16 heads),
 // eight threads a head with 16-byte accesses: thread c has dims 8 c .. + 7 and
 // the same of the other half, so that a quad of threads holds two whole groups
-// of 32.  Keys are rounded once, from the fp32 rotation.
+// of 32.  Keys are rounded once, from the fp32 rotation.  Bytes bound it where
+// there are many tokens (10639 of 32 + 2 * 8 heads, 232 MB, 41 us: 5.7 TB/s),
+// the launch and one trip to memory where there are few (28: 3.4 us).
 __global__ __launch_bounds__(128) void kv4_append_kernel(Kv4Args a) {
   const int64_t t = blockIdx.x;
   const int lane = threadIdx.x & 63;
@@ -227,7 +229,9 @@ __device__ __forceinline__ void stg16_nt(bf16* p, u32x4 v) {
 
 // Cached tokens as bf16: sixteen lanes a (token, head) row of keys and of
 // values (four tokens a wave at a time, sixteen in flight), so that a store
-// covers whole rows.  Tokens without a page are zeros.
+// covers whole rows.  Tokens without a page are zeros.  Its bytes bound it: 69
+// thousand tokens of 8 heads, 358 MB, 55 us (6.5 TB/s; with stores through the
+// caches and four tokens a wave 188 us); a request of 300 tokens 5.3 us.
 constexpr int kReadTokens = 16;  // of a wave
 
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
@@ -595,6 +599,12 @@ __device__ __forceinline__ void write_row(const Kv4Args& a, const Unit& u, int r
 // lane the keys 4 g .. + 3 of both tiles of its row, which is the B operand of
 // O^T = V^T P^T as it is.  The probabilities enter as one bf16 and are summed as
 // they are, as in the kernel for many rows.
+//
+// The cache's bytes bound it once they are many: 32 tokens over 8192 to 32767
+// keys each (742 MB) take 124 us, 6.0 TB/s; 1 to 6 drafted tokens of 28 requests
+// over 128 to 8192 keys (122 MB) 30 us, with a second step of loads in flight a
+// wave 33.  Under that the chain of dependent loads (lengths, table, records)
+// does: 7 us for four tokens over 300 keys, 14.5 for 28 over 128 to 2048.
 constexpr int kSplitWaves = 4;
 
 struct SplitLds {
@@ -854,6 +864,12 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
 // number.  That, an infinity or NaN, or a row without a key in its first 32
 // leaves sums outside [2^-60, 2^100); the unit is then done again with a
 // running maximum.
+//
+// Matrix and vector work bound it about alike: five prompts up to 8192 tokens
+// (600 GFLOP of visible scores and sums, 32 heads) take 517 us, 1160 TFLOP/s,
+// the matrix units busy 54 % of the time; with a running maximum and the
+// compiler's own order 1171 us.  128 rows a workgroup: with 32 every record
+// would be made bf16 four times as often.
 constexpr int kPromptRows = 128, kPromptKeys = 64;
 
 struct PromptLds {
@@ -1167,7 +1183,9 @@ __global__ __launch_bounds__(256, 2) void kv4_mixed_kernel(Kv4Args many, Kv4Args
 }
 
 // Merges the parts of 16 rows of a block that was cut: a workgroup per (block,
-// kv head, set of 16 rows), thread (g, row, i) as above, parts in order.
+// kv head, set of 16 rows), thread (g, row, i) as above, parts in order.  Its
+// launch and the records bound it: 4 us for 28 single tokens, 13 for the 34 MB
+// of two prompt chunks of 512 cut in two.
 template <int RB, int KS>
 __device__ __forceinline__ void combine_set(const Kv4Args& a, uint32_t set) {
   constexpr int SETS = RB / 16;
