@@ -36,9 +36,10 @@ struct RowStat {
   int32_t pad;
 };
 // A slice of a sequence's last row: sums of the target's and the drafter's
-// e^(..), and of the residual and the drafter's part of it at a given ratio.
+// e^(..), of the residual and the drafter's part of it at a given ratio, and the
+// target's part that is next to no residual.
 struct SliceSum {
-  double p, q, res, act;
+  double p, q, res, act, near;
 };
 
 struct VerifyArgs {
@@ -366,12 +367,15 @@ __device__ __forceinline__ double get(const double* p) {
 // all slices are: its weight is added up at the fp32 sums' ratio (off by a
 // relative d of under 2^-14, 1e-6 as a rule) together with the drafter's part F
 // of it, and put right by - d F at the end.  What that leaves out are the tokens
-// between the two ratios, d of themselves each and about d of all: d^2.
+// between the two ratios, d of themselves each and mostly about d of all: d^2.
+// Where it could be more than 2^-30 of the residual (rows that are nearly the
+// same) the last workgroup adds the slices up again at the exact ratio.
 //
-// 10.5 us for one sequence of 4 drafts, 25 for 28 of up to 5 (128256 tokens, with
+// 10.8 us for one sequence of 4 drafts, 27 for 28 of up to 5 (128256 tokens, with
 // a drafter): a chain of loads, sums over the workgroup and one count in memory,
-// and 64-bit arithmetic of about 5 us spread over the card; a call with every
-// slice in one pass of the whole card, so that this chain is met once.
+// and 64-bit arithmetic of some 6 us by its count, spread over the card; every
+// slice is there at once, so that this chain is met once.
+constexpr double kNear = 0x1p-18;  // (the fp32 sums' ratio is nearer than half of it but for rows out of the way)
 constexpr int kChunk = 2048;  // logits of a workgroup at a time; a slice is a.chunks of them
 
 __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
@@ -381,7 +385,7 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
   __shared__ int sh_hit[4], sh_any[4];
   __shared__ float sh_mx[16], sh_z[16];  // maxima and sums of the eight drafts: target, drafter
   __shared__ int64_t sh_best[8];
-  __shared__ unsigned long long shb;
+  __shared__ unsigned long long shb, sh_near;
   const int tid = threadIdx.x, l16 = tid & 15, s = blockIdx.y;
   tab[tid] = a.pow[tid];  // (a barrier follows)
   int64_t t0;
@@ -477,7 +481,8 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       if (j != take || greedy) out[j] = j < take ? a.ids[t0 + j] : j == take ? best : -1;
   }
   if (greedy) return;
-  SliceSum own{0, 0, 0, 0};
+  SliceSum own{0, 0, 0, 0, 0};
+  if (tid == 0) sh_near = 0;
   const int64_t slice = (int64_t)a.chunks * kChunk;
 #pragma unroll 1
   for (int64_t i = blockIdx.x * slice + tid * 8; i < min((blockIdx.x + 1) * slice, a.vocab); i += kChunk)
@@ -489,10 +494,14 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
         own.res += v;
         own.act += q;
       }
+      if (x.q && fabs(v) < p * kNear) own.near += p;
     });
   if (x.q) {
-    block_sum2(own.p, own.q, sh);
+    block_sum2(own.p, own.q, sh);  // (a barrier: sh_near is 0)
+    // (a bound: whole numbers, so that the order of the atomics does not show)
+    if (own.near > 0) atomicAdd(&sh_near, (unsigned long long)(own.near * 0x1p40) + 1);
     block_sum2(own.res, own.act, sh);
+    own.near = (double)sh_near * 0x1p-40;
   } else {
     own.p = block_sum(own.p, sh);
   }
@@ -506,6 +515,7 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       put(&sums[blockIdx.x].q, own.q);
       put(&sums[blockIdx.x].res, own.res);
       put(&sums[blockIdx.x].act, own.act);
+      put(&sums[blockIdx.x].near, own.near);
     }
     __builtin_amdgcn_s_waitcnt(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -513,17 +523,20 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
   }
   __syncthreads();
   if (ended != a.slices - 1) return;
-  SliceSum v{0, 0, 0, 0};  // of slice tid (there are at most 256)
+  SliceSum v{0, 0, 0, 0, 0};  // of slice tid (there are at most 256)
   if (tid < a.slices) {
     v.p = get(&sums[tid].p);
-    if (x.q) v = SliceSum{v.p, get(&sums[tid].q), get(&sums[tid].res), get(&sums[tid].act)};
+    if (x.q)
+      v = SliceSum{v.p, get(&sums[tid].q), get(&sums[tid].res), get(&sums[tid].act), get(&sums[tid].near)};
   }
-  double m = v.p;
+  double m = v.p, off = 0;  // off: how far all may be off, by the slice's share
   if (x.q) {  // the exact ratio, and the weights put right to it
     block_sum2(v.p, v.q, sh);
     const double ratio = v.p / v.q;
     m = v.res - (ratio - x.ratio) * v.act;
     m = m < 0 ? 0 : m;
+    const double d = fabs(ratio - x.ratio) / ratio;
+    off = d < kNear / 2 ? d * v.near : v.p;
     x.ratio = ratio;
   }
   // The first thread whose cumulative weight `inc` is above `goal` (where there
@@ -542,6 +555,21 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
   double inc = block_prefix(m, sh);
   if (tid == 255) below = inc;  // the sum of all
   __syncthreads();
+  if (__syncthreads_or(off > below * 0x1p-38)) {  // (256 slices at most: 2^-30 together)
+    m = 0;
+#pragma unroll 1
+    for (int k = 0; k < a.slices; ++k) {
+      double y = 0;
+#pragma unroll 1
+      for (int64_t i = k * slice + tid * 8; i < min((k + 1) * slice, a.vocab); i += kChunk)
+        weights8(a, x, i, rate, tab, [&](int, double p, double q) { y += fmax(p - x.ratio * q, 0.0); });
+      y = block_sum(y, sh);
+      if (tid == k) m = y;
+    }
+    inc = block_prefix(m, sh);
+    if (tid == 255) below = inc;
+    __syncthreads();
+  }
   const double all = below, want = (double)u_last * all;
   if (!(all > 0)) {  // a NaN, or nothing left
     const int64_t b = row_best(x.p, a.vocab, &shb);

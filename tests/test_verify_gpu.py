@@ -232,6 +232,29 @@ def test_masked_tokens_stay_out_whatever_the_temperature(dev, temp):
                     assert tok.tolist() == [[400, -1]] and acc.tolist() == [0]
 
 
+@pytest.mark.parametrize("raised", [True, False])
+def test_a_residual_far_smaller_than_the_rows(dev, raised):
+    """Rows that differ in the draft and five tokens of little weight, so that
+    their sums agree to under 3e-8 (raised: the residual is those five alone;
+    lowered: every other token has a hundred-millionth of its weight left)."""
+    n, V = 64, 20000
+    g = torch.Generator().manual_seed(6)
+    drf = (2.5 * torch.randn(V, generator=g)).to(BF16)
+    few = [1500, 3333, 9001, 12345, 19000]  # slices of 2048: five of them
+    drf[few] = torch.tensor([-6.0, -5.5, -6.5, -5.0, -7.0], dtype=BF16)
+    tgt = drf.clone()
+    drf[7], tgt[7] = -9.0, -10.0  # the draft
+    tgt[few] = (drf[few].float() + (1.0 if raised else -1.0) * torch.tensor([0.25, 0.5, 0.25, 0.125, 0.5])).to(BF16)
+    r = float(torch.exp(tgt.double()).sum() / torch.exp(drf.double()).sum()) - 1
+    assert 5e-9 < abs(r) < 3e-8 and (r > 0) == raised
+    c = {"tgt": tgt.expand(2 * n, V).contiguous(), "drf": drf.expand(n, V).contiguous(), "ids": torch.full((n,), 7),
+         "temp": torch.ones(n), "u": torch.full((n,), 0.9), "u_last": (torch.arange(n) + 0.37) / n, "new": [1] * n}
+    got = _same(c, dev)
+    assert bool((got[1] == 0).all())
+    seen = len(got[0][:, 0].unique())
+    assert seen == 5 if raised else seen > 20
+
+
 def test_drawn_tokens_follow_the_target(dev):
     """Over 20000 requests of the same two rows the first token (draft or
     drawn) has the target's distribution whatever the drafter's is: every
