@@ -714,16 +714,15 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept
         dr, dv, ldd = _logit_rows(draft_logits, "draft_logits", packed, dev)
         if dr != nd or dv != vocab or (not packed and nd and draft_logits.shape[:2] != draft_ids.shape):
             raise ValueError("draft_logits need one row of the target's vocabulary per draft")
-    device = target_logits.device
-    tok = torch.empty(nseq, max_drafts + 1, dtype=torch.int64, device=device)
-    acc = torch.empty(nseq, dtype=torch.int32, device=device)
+    tok = draft_ids.new_empty((nseq, max_drafts + 1))
+    acc = draft_ids.new_empty(nseq, dtype=torch.int32)
     lib = _lib.load()
     need = lib.swl_verify_drafts_workspace(nseq, nd, vocab, 1 if draft_logits is not None else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    ws = draft_ids.new_empty(need, dtype=torch.uint8)
     _lib.check(lib.swl_verify_drafts_bf16(
         target_logits.data_ptr(), ldt, _addr(draft_logits), ldd, vocab, draft_ids.data_ptr(), _addr(cu_drafts), nseq, nd,
         max_drafts, temperature.data_ptr(), u_accept.data_ptr(), u_final.data_ptr(), tok.data_ptr(), acc.data_ptr(),
-        ws.data_ptr(), need, _stream()))
+        ws.data_ptr(), need, _stream_of(dev)))
     return tok, acc
 
 
@@ -892,12 +891,17 @@ def kv4_pages(num_blocks: int, block_size: int, hkv: int, device) -> torch.Tenso
     return torch.zeros(num_blocks, hkv, block_size // 16, KV4_RECORD, dtype=torch.uint8, device=device)
 
 
-# The kv4 calls are short on the GPU (a decode step's append 3.4 us), so their
-# checks read every attribute once and pass plain addresses.
-if hasattr(torch._C, "_cuda_getDevice"):
+# The kv4 calls are short on the GPU (a decode step's append 3.4 us), so the host
+# is their time: the checks read every attribute once and pass plain addresses.
+if hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_getDevice"):
     _current_device = torch._C._cuda_getDevice
+    _stream_of = torch._C._cuda_getCurrentRawStream
 else:
     _current_device = torch.cuda.current_device
+
+    def _stream_of(dev: int) -> int:
+        return torch.cuda.current_stream(dev).cuda_stream
+_Tensor, _U8, _I32 = torch.Tensor, torch.uint8, torch.int32
 
 
 def _device_for(t, name: str, dtype) -> int:
@@ -910,7 +914,7 @@ def _device_for(t, name: str, dtype) -> int:
 def _here(t, name: str, dtype, dev: int):
     """t is a tensor of `dtype` on the current device (launches go to its
     current stream)."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != dev:
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != dev:
         _need(t, name, dtype)
         raise ValueError(f"{name} must be on the current device (cuda:{dev}), got {t.device}")
 
@@ -922,39 +926,48 @@ def _addr(t: Optional[torch.Tensor]):
 def _kv4_cache(pages, block_table, lens, name, nseq, cu, dev):
     """Checks of what the kv4 calls share; nseq is cu's where it is given.
     Returns (nseq, blocks, kv heads, block size, table width)."""
-    _here(pages, "pages", torch.uint8, dev)
+    _here(pages, "pages", _U8, dev)
     shape = pages.shape
     if len(shape) != 4 or shape[3] != KV4_RECORD or not pages.is_contiguous():
         raise ValueError(f"pages must be contiguous [num_blocks, hkv, block_size / 16, {KV4_RECORD}]")
-    _here(block_table, "block_table", torch.int32, dev)
-    _here(lens, name, torch.int32, dev)
+    _here(block_table, "block_table", _I32, dev)
+    _here(lens, name, _I32, dev)
     if cu is not None:
-        _here(cu, "cu_seqlens", torch.int32, dev)
-        if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
+        _here(cu, "cu_seqlens", _I32, dev)
+        offsets = cu.shape
+        if len(offsets) != 1 or offsets[0] < 1 or not cu.is_contiguous():
             raise ValueError("cu_seqlens must be contiguous [nseq + 1]")
-        nseq = cu.shape[0] - 1
-    bt = block_table.shape
+        nseq = offsets[0] - 1
+    bt, ln = block_table.shape, lens.shape
     if len(bt) != 2 or bt[0] < nseq or not block_table.is_contiguous():
         raise ValueError("block_table must be contiguous [nseq, max_blocks]")
-    if lens.dim() != 1 or lens.shape[0] < nseq or not lens.is_contiguous():
+    if len(ln) != 1 or ln[0] < nseq or not lens.is_contiguous():
         raise ValueError(f"{name} must be contiguous with nseq entries")
-    return nseq, shape[0], shape[1], shape[2] * 16, bt[1]
+    nb, hkv, tiles, _ = shape
+    return nseq, nb, hkv, tiles * 16, bt[1]
 
 
 def _packed_rows(t: torch.Tensor, name: str, cu, dev):
-    """Token rows as (tokens, heads, token stride): [nseq, L, heads, 128]
+    """Token rows as (shape, tokens, heads, token stride): [nseq, L, heads, 128]
     without cu_seqlens, [tokens, heads, 128] with."""
     _here(t, name, BF16, dev)
-    shape = t.shape
+    shape, stride = t.shape, t.stride()
     if len(shape) != (4 if cu is None else 3) or shape[-1] != 128:
         raise ValueError(f"{name} must be [nseq, q_len, heads, 128], or [tokens, heads, 128] with cu_seqlens")
     if cu is None:
-        return shape[0] * shape[1], shape[2], _token_rows(t, name, shape[2], 128)
-    n, heads, _ = shape
-    s0, s1, s2 = t.stride()
-    if n and heads and (s2 != 1 or (heads > 1 and s1 != 128)):
+        nseq, L, heads, _ = shape
+        s0, s1, s2, s3 = stride
+        n = nseq * L
+        if L > 1:
+            if nseq > 1 and s0 != L * s1:
+                raise ValueError(f"{name} tokens must be evenly strided")
+            s0 = s1
+    else:
+        n, heads, _ = shape
+        s0, s2, s3 = stride
+    if n and heads and (s3 != 1 or (heads > 1 and s2 != 128)):
         raise ValueError(f"{name} heads must be contiguous within a token")
-    return n, heads, s0 if n > 1 else heads * 128
+    return shape, n, heads, s0 if n > 1 else heads * 128
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
@@ -970,11 +983,11 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
     as they are.  Tokens behind the last sequence are not stored and their rows
     of q_out are left as they were."""
     dev = _device_for(k, "k", BF16)
-    ntok, hkv, ks = _packed_rows(k, "k", cu_seqlens, dev)
-    _, _, vs = _packed_rows(v, "v", cu_seqlens, dev)
-    if v.shape != k.shape:
+    shape, ntok, hkv, ks = _packed_rows(k, "k", cu_seqlens, dev)
+    vshape, _, _, vs = _packed_rows(v, "v", cu_seqlens, dev)
+    if vshape != shape:
         raise ValueError("k and v must have one shape")
-    nseq, nb, cache_heads, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", k.shape[0], cu_seqlens,
+    nseq, nb, cache_heads, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", shape[0], cu_seqlens,
                                                dev)
     if cache_heads != hkv:
         raise ValueError("cache geometry mismatch")
@@ -986,26 +999,27 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
         _here(cos_sin, "cos_sin", BF16, dev)
         if positions.numel() != ntok or not positions.is_contiguous():
             raise ValueError("positions must be contiguous with one entry per token")
-        if cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous():
+        table = cos_sin.shape
+        if len(table) != 2 or table[1] != 128 or not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be contiguous [max_pos, 128]")
-        max_pos = cos_sin.shape[0]
+        max_pos = table[0]
     hq = qs = 0
     if q is not None:
-        _, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
-        if q.shape[:-2] != k.shape[:-2]:
+        qshape, _, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
+        if qshape[:-2] != shape[:-2]:
             raise ValueError("q, k and v must have the same tokens")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
+            q_out = q.new_empty(qshape)
         else:
             _here(q_out, "q_out", BF16, dev)
-            if q_out.shape != q.shape or not q_out.is_contiguous():
+            if q_out.shape != qshape or not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous with q's shape")
     elif q_out is not None:
         raise ValueError("q_out needs q")
     _lib.check(_lib.load().swl_kv4_append_bf16(
         _addr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _addr(q_out), nseq, ntok, _addr(cu_seqlens), hq, hkv, 128,
         pages.data_ptr(), nb, bs, block_table.data_ptr(), mb, cache_seqlens.data_ptr(), _addr(positions),
-        _addr(cos_sin), max_pos, _stream()))
+        _addr(cos_sin), max_pos, _stream_of(dev)))
     return q_out
 
 
@@ -1019,15 +1033,14 @@ def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tenso
     if count < 0:
         raise ValueError("count must not be negative")
     dev = _device_for(starts, "starts", torch.int32)
-    _here(starts, "starts", torch.int32, dev)
     nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, starts, "starts", starts.numel(), cu_seqlens, dev)
     shape = (count, hkv, 128) if cu_seqlens is not None else (nseq, count, hkv, 128)
     ntok = count if cu_seqlens is not None else nseq * count
-    k = torch.empty(shape, dtype=BF16, device=pages.device)
+    k = pages.new_empty(shape, dtype=BF16)
     v = torch.empty_like(k)
     _lib.check(_lib.load().swl_kv4_read_bf16(
         pages.data_ptr(), nb, bs, block_table.data_ptr(), mb, starts.data_ptr(), nseq, ntok, _addr(cu_seqlens), hkv, 128,
-        k.data_ptr(), v.data_ptr(), _stream()))
+        k.data_ptr(), v.data_ptr(), _stream_of(dev)))
     return k, v
 
 
@@ -1047,30 +1060,30 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     `out`.  max_q_len: the most new tokens of a sequence where the host knows
     it (a hint for speed alone)."""
     dev = _device_for(q, "q", BF16)
-    ntok, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
-    nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", q.shape[0], cu_seqlens, dev)
+    qshape, ntok, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
+    nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", qshape[0], cu_seqlens, dev)
     if hq < 1 or hkv < 1 or hq % hkv:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if cu_seqlens is None:
-        max_q_len = q.shape[1]
-        shape = (*q.shape[:2], hq * 128)
+        max_q_len = qshape[1]
+        shape = (nseq, max_q_len, hq * 128)
     else:
         max_q_len = ntok if max_q_len is None else int(max_q_len)
         shape = (ntok, hq * 128)
-    max_q_len = max(max_q_len, 1)
-    device = q.device
+    if max_q_len < 1:
+        max_q_len = 1
     if out is None:
-        out = torch.empty(shape, dtype=BF16, device=device)
+        out = q.new_empty(shape)
     else:
         _here(out, "out", BF16, dev)
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be contiguous [.., hq * 128] with q's tokens")
     need = _kv4_workspace(nseq, ntok, 0 if cu_seqlens is None else 1, max_q_len, hq, hkv, mb * bs)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    ws = pages.new_empty(need) if need else None
     _lib.check(_lib.load().swl_kv4_attention_bf16(
         q.data_ptr(), qs, nseq, ntok, _addr(cu_seqlens), max_q_len, hq, hkv, 128, pages.data_ptr(), nb, bs,
         block_table.data_ptr(), mb, cache_seqlens.data_ptr(), float(softmax_scale), out.data_ptr(), _addr(ws), need,
-        _stream()))
+        _stream_of(dev)))
     return out
 
 
