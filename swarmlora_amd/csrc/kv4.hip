@@ -1182,59 +1182,67 @@ __global__ __launch_bounds__(256, 2) void kv4_mixed_kernel(Kv4Args many, Kv4Args
     split_unit<2>(few, blockIdx.x - n_many, sh.split);
 }
 
-// Merges the parts of 16 rows of a block that was cut: a workgroup per (block,
-// kv head, set of 16 rows), thread (g, row, i) as above, parts in order.  Its
-// launch and the records bound it: 4 us for 28 single tokens, 13 for the 34 MB
-// of two prompt chunks of 512 cut in two.
+// Merges the parts of the blocks that were cut: a workgroup per (block, kv head,
+// combine_sets of 16 rows), thread (g, row, i) as above, parts in order.  Its
+// launch, the unit's search and the records bound it: 4 us for 28 single tokens,
+// 9 for the 34 MB of two prompt chunks of 512 cut in two (with one set a
+// workgroup, and so four times the searches, 13.5; with all eight 12.5).
+constexpr int combine_sets(int rb) { return rb == 128 ? 4 : 1; }
+
 template <int RB, int KS>
-__device__ __forceinline__ void combine_set(const Kv4Args& a, uint32_t set) {
-  constexpr int SETS = RB / 16;
+__device__ __forceinline__ void combine_unit(const Kv4Args& a, uint32_t unit) {
+  constexpr int SETS = RB / 16, EACH = combine_sets(RB);
   const int lane = threadIdx.x & 63;
-  const int e = set % SETS;
   int spp;
   Unit u;
-  if (!find_unit<RB, KS, true>(a, set / SETS, lane, spp, u)) return;
-  const int rows = u.n * a.G, row = threadIdx.x >> 2 & 15, r = u.b * RB + e * 16 + row;
+  if (!find_unit<RB, KS, true>(a, unit / (SETS / EACH), lane, spp, u)) return;
+  const int rows = u.n * a.G, row = threadIdx.x >> 2 & 15;
   // the block's own parts: its last row may see fewer keys than the sequence's
   const int steps = (last_key(a, u, min((u.b + 1) * RB, rows) - 1) + KS - 1) / KS;
   const int parts = ceil_div(max(steps, 1), spp, 1.f / (float)spp);
-  if (r >= rows || u.rec + (int64_t)(parts - 1) * a.hkv >= a.max_rec) return;
-  const float* rec = a.part + (u.rec * SETS + e) * kRecF;
+  if (u.rec + (int64_t)(parts - 1) * a.hkv >= a.max_rec) return;
   const int64_t next = (int64_t)a.hkv * SETS * kRecF;
-  float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  constexpr int B = 4;  // records in flight together
-  for (int p0 = 0; p0 < parts; p0 += B) {
-    float pm[B], pl[B], po[B][8];
+#pragma unroll 1
+  for (int e = unit % (SETS / EACH) * EACH, e1 = e + EACH; e < e1; ++e) {
+    const int r = u.b * RB + e * 16 + row;
+    if (r >= rows) return;
+    const float* rec = a.part + (u.rec * SETS + e) * kRecF;
+    float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    constexpr int B = 4;  // records in flight together
+    for (int p0 = 0; p0 < parts; p0 += B) {
+      float pm[B], pl[B], po[B][8];
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const float* rp = rec + min(p0 + b, parts - 1) * next;
-      pm[b] = rp[2048 + row];
-      pl[b] = rp[2064 + row];
+      for (int b = 0; b < B; ++b) {
+        if (p0 + b >= parts) break;
+        const float* rp = rec + (p0 + b) * next;
+        pm[b] = rp[2048 + row];
+        pl[b] = rp[2064 + row];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) po[b][d] = rp[d * 256 + threadIdx.x];
+        for (int d = 0; d < 8; ++d) po[b][d] = rp[d * 256 + threadIdx.x];
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (p0 + b >= parts) break;
+        const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
+        L = L * fa + pl[b] * fb;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] = o[d] * fa + po[b][d] * fb;
+        M = mn;
+      }
     }
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      if (p0 + b >= parts) break;
-      const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
-      L = L * fa + pl[b] * fb;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) o[d] = o[d] * fa + po[b][d] * fb;
-      M = mn;
-    }
+    write_row(a, u, r, threadIdx.x, L, o);
   }
-  write_row(a, u, r, threadIdx.x, L, o);
 }
 
 template <int RB, int KS>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Args a) {
-  combine_set<RB, KS>(a, blockIdx.x);
+  combine_unit<RB, KS>(a, blockIdx.x);
 }
 __global__ __launch_bounds__(256) void kv4_combine_mixed_kernel(Kv4Args many, Kv4Args few, uint32_t n_many) {
   if (blockIdx.x < n_many)
-    combine_set<kPromptRows, kPromptKeys>(many, blockIdx.x);
+    combine_unit<kPromptRows, kPromptKeys>(many, blockIdx.x);
   else
-    combine_set<32, 32>(few, blockIdx.x - n_many);
+    combine_unit<32, 32>(few, blockIdx.x - n_many);
 }
 
 // ------------------------------------------------------------- launchers ---
@@ -1306,7 +1314,7 @@ Kv4Args kv4_part_args(Kv4Args a, const Kv4Launch& p, void* ws) {
 }
 // Workgroups of the combine: cut blocks, 16 rows each.
 unsigned kv4_sets(const Kv4Launch& p) {
-  return p.recs ? (unsigned)(std::min<int64_t>(p.blocks, p.slots) * (p.rb / 16)) : 0;
+  return p.recs ? (unsigned)(std::min<int64_t>(p.blocks, p.slots) * (p.rb / 16 / combine_sets(p.rb))) : 0;
 }
 
 int kv4_launch_attention(const Kv4Args& a, const Kv4Plan& p, void* ws, hipStream_t st) {
