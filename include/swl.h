@@ -450,10 +450,10 @@ int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, con
 /* Causal attention of the new tokens (already appended) over the cache: query
  * i of sequence s sees tokens 0 .. cache_seqlens[s] + i; query head j reads kv
  * head j / (hq / hkv), any hq that is a multiple of hkv.  out [ntok, hq *
- * 128], not q's memory.  Sums and softmax in fp32.  A query that sees no token
- * gets zeros, one with an infinity or a NaN, or that sees a NaN key, NaN; a NaN
- * value group reaches the queries that see it.  Values must leave room for
- * their sum (under 2^118 / tokens).
+ * 128], not q's memory; softmax_scale positive and finite.  Sums and softmax in
+ * fp32.  A query that sees no token gets zeros, one with an infinity or a NaN, or
+ * that sees a NaN key, NaN; a NaN value group reaches the queries that see it.
+ * Values must leave room for their sum (under 2^118 / tokens).
  * max_q_len: the most new tokens of a sequence (a hint for speed alone: it
  * chooses between kernels, any value >= 1 gives a right result).
  * workspace: swl_kv4_attention_workspace(nseq, ntok, cu_seqlens != NULL,

@@ -264,6 +264,45 @@ def test_attention_matches_the_definition(dev, ctx, new, hq, hkv, page):
         assert bool((out[T:] == 5.0).all())
 
 
+def test_more_sequences_than_lanes(dev):
+    """150 sequences, some without new tokens, appended, read back and attended
+    to in packed calls; the long ones behind the first 64."""
+    ops = _ops()
+    n, hq, hkv, page = 150, 4, 2, 16
+    g = torch.Generator().manual_seed(9)
+    ctx = torch.randint(0, 60, (n,), generator=g).tolist()
+    new = torch.randint(0, 3, (n,), generator=g).tolist()
+    ctx[70], ctx[140], new[70], new[130], new[149] = 1500, 700, 1, 50, 2
+    pages, bt = _filled([c + m for c, m in zip(ctx, new)], hkv, page, 91)
+    T, cu, lens = sum(new), _prefix(new), torch.tensor(ctx, dtype=torch.int32)
+    k, v, q = randn((T, hkv, 128), 1), randn((T, hkv, 128), 2), randn((T, hq, 128), 3, 2.0)
+    ops.kv4_append(k.to(dev), v.to(dev), pages, bt.to(dev), lens.to(dev), cu_seqlens=cu.to(dev))
+    gk, gv = ops.kv4_read(pages, bt.to(dev), lens.to(dev), T, cu_seqlens=cu.to(dev))
+    assert torch.equal(gk.cpu().double(), _kv4.decode(*_kv4.encode(k.double())))
+    assert torch.equal(gv.cpu().double(), _kv4.decode(*_kv4.encode(v.double())))
+    want, wt = _kv4.attend(q, pages.cpu(), bt, ctx, cu.tolist(), SCALE)
+    for hint, wide in ((50, False), (None, True), (1, False)):
+        out = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), lens.to(dev), SCALE, cu_seqlens=cu.to(dev),
+                                max_q_len=hint)
+        _check(out, want, wt, 2.0 ** -7)
+
+
+def test_one_token_of_any_stride(dev):
+    """A lone token's own strides do not matter (an expanded or cut view)."""
+    ops = _ops()
+    pages, bt = _filled([20], 2, 16, 95)
+    lens = torch.tensor([19], dtype=torch.int32, device=dev)
+    q, k = randn((1, 1, 4, 128), 1).to(dev), randn((1, 1, 2, 128), 2).to(dev)
+    a = pages.clone()
+    ops.kv4_append(k, k, a, bt.to(dev), lens)
+    b = pages.clone()
+    odd = torch.as_strided(k, (1, 1, 2, 128), (1, 3, 128, 1))
+    ops.kv4_append(odd, odd, b, bt.to(dev), lens)
+    assert torch.equal(a, b)
+    qo = torch.as_strided(q, (1, 1, 4, 128), (0, 5, 128, 1))
+    assert torch.equal(ops.kv4_attention(qo, a, bt.to(dev), lens, SCALE), ops.kv4_attention(q, a, bt.to(dev), lens, SCALE))
+
+
 @pytest.mark.parametrize("L", [1, 4, 33])
 def test_attention_uniform_strided_and_a_wrong_hint(dev, L):
     """Queries in place in fused rows, [nseq, L, ..] without offsets; a
@@ -464,6 +503,48 @@ def test_captured_step_follows_the_lengths(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, got)
         lens += 1
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_captured_packed_call_follows_the_offsets(dev, wide):
+    """One captured call of append and attention over 80 token rows, replayed
+    with other offsets and lengths: prompts beside single tokens, empty
+    sequences, rows behind the last one left as they were."""
+    ops = _ops()
+    hq, hkv, page, T = 8, 2, 16, 80
+    pages, bt = _filled([600, 400, 200], hkv, page, 73)
+    bt_d = _wide(bt, wide).to(dev)
+    q, k, v = (randn((T, h, 128), 5 + i).to(dev) for i, h in enumerate((hq, hkv, hkv)))
+    cu, lens = (torch.zeros(n, dtype=torch.int32, device=dev) for n in (4, 3))
+    out = torch.empty(T, hq * 128, dtype=BF16, device=dev)
+
+    def step():
+        ops.kv4_append(k, v, pages, bt_d, lens, cu_seqlens=cu)
+        ops.kv4_attention(q, pages, bt_d, lens, SCALE, cu_seqlens=cu, out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i, (new, ctx) in enumerate([([1, 70, 9], [500, 0, 100]), ([40, 0, 40], [0, 300, 160]), ([79, 1, 0], [510, 399, 7]),
+                                    ([2, 2, 2], [3, 4, 5]), ([0, 0, 0], [1, 1, 1])]):
+        q.copy_(randn((T, hq, 128), 50 + i, 2.0))
+        k.copy_(randn((T, hkv, 128), 60 + i))
+        cu.copy_(_prefix(new))
+        lens.copy_(torch.tensor(ctx, dtype=torch.int32))
+        out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, n = out.clone(), sum(new)
+        assert bool((got[n:] == 5.0).all())
+        want, wt = _kv4.attend(q[:n].cpu(), pages.cpu(), bt, ctx, _prefix(new).tolist(), SCALE)
+        _check(got[:n], want, wt, 2.0 ** -7)
+        step()
+        assert torch.equal(out, got)
 
 
 def test_two_streams_at_once(dev):
