@@ -11,7 +11,7 @@
 // What decides is held in 64 bits: with 128256 tokens a cumulative sum that is
 // off by 1e-7 of the total picks another token once in about forty draws.  A
 // 64-bit exponential costs fifteen times an fp32 one, though (28 sequences of 1
-// to 5 drafts, 128256 tokens: 77 us with 64 bits throughout, 37 now), and most rows only
+// to 5 drafts, 128256 tokens: 77 us with 64 bits throughout, 35 now), and most rows only
 // have to show that their draft is accepted: u q < p is clear in fp32 unless the
 // two are within 2^-14 of each other.  So, in two launches: every row's maximum
 // and sum in fp32, a workgroup per slice of a row (the logits' bytes are its
@@ -35,10 +35,10 @@ struct RowStat {
   int32_t idx;    // the first index of that (greedy rows)
   int32_t pad;
 };
-// A slice of a sequence's last row: sums of the target's and the drafter's
+// A wave's share of a sequence's last row: sums of the target's and the drafter's
 // e^(..), of the residual and the drafter's part of it at a given ratio, and the
 // target's part that is next to no residual.
-struct SliceSum {
+struct ShareSum {
   double p, q, res, act, near;
 };
 
@@ -55,9 +55,9 @@ struct VerifyArgs {
   int32_t* acc;
   int32_t nseq, per, max_drafts;
   int32_t stats, slices;  // slices of a row: of its statistics, of a sequence's last row
-  int32_t chunks;
+  int32_t share;          // logits of a wave of a slice
   RowStat* stat;        // [T + nseq rows, then T rows][stats]
-  SliceSum* sum;        // [nseq][slices]
+  ShareSum* sum;        // [nseq][4 slices]
   uint32_t* done;       // [nseq] slices that are (set to 0 by the first launch)
   double* pow;          // [256] 2^(k / 256) (made by it)
 };
@@ -146,6 +146,11 @@ __device__ __forceinline__ void block_sum2(double& v, double& w, double* sh) {
   __syncthreads();
   v = (sh[0] + sh[1]) + (sh[2] + sh[3]);
   w = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
 }
 // Inclusive prefix over them, likewise.
 __device__ __forceinline__ double block_prefix(double v, double* sh) {
@@ -358,10 +363,12 @@ __device__ __forceinline__ double get(const double* p) {
 }
 
 // Acceptance of a sequence's drafts (sixteen lanes for a draft's target row and
-// sixteen for the drafter's, eight drafts at a time), one slice's weight of its
-// last row, and by the last workgroup of the
-// sequence the token: the first whose cumulative weight is above u * (sum of
-// all); where rounding leaves none, the last of any weight.
+// sixteen for the drafter's, eight drafts at a time), the weight of a slice of
+// its last row, every wave's share of the slice for itself, and by the last
+// workgroup of the sequence the token: the share that the random number falls
+// in, then the thread and the token of that share: the first whose cumulative
+// weight is above u * (sum of all); where rounding leaves none, the last of any
+// weight.  Shares lie in index order, at most 256 of a row, one a thread.
 //
 // The residual max(p - q, 0) needs the two rows' sums, which are known only when
 // all slices are: its weight is added up at the fp32 sums' ratio (off by a
@@ -369,23 +376,25 @@ __device__ __forceinline__ double get(const double* p) {
 // of it, and put right by - d F at the end.  What that leaves out are the tokens
 // between the two ratios, d of themselves each and mostly about d of all: d^2.
 // Where it could be more than 2^-30 of the residual (rows that are nearly the
-// same) the last workgroup adds the slices up again at the exact ratio.
+// same) the last workgroup adds the shares up again at the exact ratio.
 //
-// 10.8 us for one sequence of 4 drafts, 27 for 28 of up to 5 (128256 tokens, with
-// a drafter): a chain of loads, sums over the workgroup and one count in memory,
-// and 64-bit arithmetic of some 6 us by its count, spread over the card; every
-// slice is there at once, so that this chain is met once.
+// 10.5 us for one sequence of 4 drafts, 22 for 28 of up to 5 (128256 tokens, with
+// a drafter): a chain of loads, sums and one count in memory (5 us until the
+// weights, 6 behind them), and 64-bit arithmetic of some 6 us by its count, spread
+// over the card; every slice is there at once, so that this chain is met once.
+// Sums of whole slices, 4096 logits instead of 1024 to look through at the end:
+// 27 us.
 constexpr double kNear = 0x1p-18;  // (the fp32 sums' ratio is nearer than half of it but for rows out of the way)
-constexpr int kChunk = 2048;  // logits of a workgroup at a time; a slice is a.chunks of them
+constexpr int kPiece = 1024;  // logits of a share that the last workgroup looks at together, four a thread
 
 __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
   constexpr int kNone = 0x7fffffff;
   __shared__ int first_bad, ended;
-  __shared__ double tab[kPow], sh[8], wt[8][256], below, first;
+  __shared__ double tab[kPow], sh[8], wt[4][256], below, first;
   __shared__ int sh_hit[4], sh_any[4];
   __shared__ float sh_mx[16], sh_z[16];  // maxima and sums of the eight drafts: target, drafter
   __shared__ int64_t sh_best[8];
-  __shared__ unsigned long long shb, sh_near;
+  __shared__ unsigned long long shb;
   const int tid = threadIdx.x, l16 = tid & 15, s = blockIdx.y;
   tab[tid] = a.pow[tid];  // (a barrier follows)
   int64_t t0;
@@ -481,11 +490,11 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       if (j != take || greedy) out[j] = j < take ? a.ids[t0 + j] : j == take ? best : -1;
   }
   if (greedy) return;
-  SliceSum own{0, 0, 0, 0, 0};
-  if (tid == 0) sh_near = 0;
-  const int64_t slice = (int64_t)a.chunks * kChunk;
+  ShareSum own{0, 0, 0, 0, 0};
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t from = ((int64_t)blockIdx.x * 4 + wave) * a.share, end = min(from + a.share, a.vocab);
 #pragma unroll 1
-  for (int64_t i = blockIdx.x * slice + tid * 8; i < min((blockIdx.x + 1) * slice, a.vocab); i += kChunk)
+  for (int64_t i = from + (tid & 63) * 8; i < end; i += 512)
     weights8(a, x, i, rate, tab, [&](int, double p, double q) {
       own.p += p;
       own.q += q;
@@ -496,40 +505,40 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       }
       if (x.q && fabs(v) < p * kNear) own.near += p;
     });
+  own.p = wave_sum(own.p);
   if (x.q) {
-    block_sum2(own.p, own.q, sh);  // (a barrier: sh_near is 0)
-    // (a bound: whole numbers, so that the order of the atomics does not show)
-    if (own.near > 0) atomicAdd(&sh_near, (unsigned long long)(own.near * 0x1p40) + 1);
-    block_sum2(own.res, own.act, sh);
-    own.near = (double)sh_near * 0x1p-40;
-  } else {
-    own.p = block_sum(own.p, sh);
+    own.q = wave_sum(own.q);
+    own.res = wave_sum(own.res);
+    own.act = wave_sum(own.act);
+    if (__ballot(own.near > 0) != 0) own.near = wave_sum(own.near);
   }
-  // The slice's sums are in memory, for every XCD, before it is counted: device-
-  // scope stores, waited for.  (A release fence would write back the XCD's whole
-  // L2, once a workgroup, and an acquire empty it.)
-  SliceSum* sums = a.sum + (int64_t)s * a.slices;
-  if (tid == 0) {
-    put(&sums[blockIdx.x].p, own.p);
+  // The shares' sums are in memory, for every XCD, before the slice is counted:
+  // device-scope stores, waited for.  (A release fence would write back the XCD's
+  // whole L2, once a workgroup, and an acquire empty it.)
+  ShareSum* sums = a.sum + (int64_t)s * 4 * a.slices;
+  if ((tid & 63) == 0) {
+    ShareSum* mine = sums + blockIdx.x * 4 + wave;
+    put(&mine->p, own.p);
     if (x.q) {
-      put(&sums[blockIdx.x].q, own.q);
-      put(&sums[blockIdx.x].res, own.res);
-      put(&sums[blockIdx.x].act, own.act);
-      put(&sums[blockIdx.x].near, own.near);
+      put(&mine->q, own.q);
+      put(&mine->res, own.res);
+      put(&mine->act, own.act);
+      put(&mine->near, own.near);
     }
     __builtin_amdgcn_s_waitcnt(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    ended = (int)__hip_atomic_fetch_add(&a.done[s], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
+  if (tid == 0) ended = (int)__hip_atomic_fetch_add(&a.done[s], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
   if (ended != a.slices - 1) return;
-  SliceSum v{0, 0, 0, 0, 0};  // of slice tid (there are at most 256)
-  if (tid < a.slices) {
+  ShareSum v{0, 0, 0, 0, 0};  // of share tid
+  if (tid < 4 * a.slices) {
     v.p = get(&sums[tid].p);
     if (x.q)
-      v = SliceSum{v.p, get(&sums[tid].q), get(&sums[tid].res), get(&sums[tid].act), get(&sums[tid].near)};
+      v = ShareSum{v.p, get(&sums[tid].q), get(&sums[tid].res), get(&sums[tid].act), get(&sums[tid].near)};
   }
-  double m = v.p, off = 0;  // off: how far all may be off, by the slice's share
+  double m = v.p, off = 0;  // off: how far all may be off, by this share of it
   if (x.q) {  // the exact ratio, and the weights put right to it
     block_sum2(v.p, v.q, sh);
     const double ratio = v.p / v.q;
@@ -555,13 +564,13 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
   double inc = block_prefix(m, sh);
   if (tid == 255) below = inc;  // the sum of all
   __syncthreads();
-  if (__syncthreads_or(off > below * 0x1p-38)) {  // (256 slices at most: 2^-30 together)
+  if (__syncthreads_or(off > below * 0x1p-38)) {  // (256 shares at most: 2^-30 together)
     m = 0;
 #pragma unroll 1
-    for (int k = 0; k < a.slices; ++k) {
+    for (int k = 0; k < 4 * a.slices; ++k) {
       double y = 0;
 #pragma unroll 1
-      for (int64_t i = k * slice + tid * 8; i < min((k + 1) * slice, a.vocab); i += kChunk)
+      for (int64_t i = (int64_t)k * a.share + tid * 8; i < min((int64_t)(k + 1) * a.share, a.vocab); i += 2048)
         weights8(a, x, i, rate, tab, [&](int, double p, double q) { y += fmax(p - x.ratio * q, 0.0); });
       y = block_sum(y, sh);
       if (tid == k) m = y;
@@ -577,21 +586,33 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
     return;
   }
   const int at = pick(m, inc, want);
-  if (tid == at) below = want - (inc - m);  // what is left for the slice (read behind pick's barriers)
+  if (tid == at) below = want - (inc - m);  // what is left for the share (read behind pick's barriers)
   __syncthreads();
   const double goal = below;
-  // the slice's chunks: the first whose weight passes that, else the last of any
+  // the share's pieces: the first whose weight passes that, else the last of any
+  const int64_t begin = (int64_t)at * a.share, stop = min(begin + a.share, a.vocab);
+  const int pieces = (a.share + kPiece - 1) / kPiece;
   double before = 0, w = 0;
-  int chunk = -1, who = 0, k = 0;
+  int piece = -1, who = 0, k = 0;
   auto weigh = [&](int k) {
-    const int64_t i = at * slice + (int64_t)k * kChunk + tid * 8;
+    const int64_t i = begin + (int64_t)k * kPiece + tid * 4;
+    uint32_t pb[4], qb[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pb[e] = qb[e] = 0xff80u;
+      if (i + e < stop) {
+        pb[e] = reinterpret_cast<const uint16_t*>(x.p)[i + e];
+        if (x.q) qb[e] = reinterpret_cast<const uint16_t*>(x.q)[i + e];
+      }
+    }
     w = 0;
-    if (i < a.vocab)
-      weights8(a, x, i, rate, tab, [&](int e, double p, double q) {
-        const double y = x.q ? fmax(p - x.ratio * q, 0.0) : p;
-        w += y;
-        wt[e][tid] = y;
-      });
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      double y = i + e < stop && i + e != x.skip ? weight(pb[e], x.p_max, rate, tab) : 0.0;
+      if (x.q) y = i + e < stop ? fmax(y - x.ratio * weight(qb[e], x.q_max, rate, tab), 0.0) : 0.0;
+      w += y;
+      wt[e][tid] = y;
+    }
   };
 #pragma unroll 1
   for (;; ++k) {
@@ -599,7 +620,7 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
     inc = before + block_prefix(w, sh);
     const int t = pick(w, inc, goal);
     if (t >= 0) {
-      chunk = k;
+      piece = k;
       who = t;
       if (tid == t) first = inc - w;
       if (tid == 255) below = inc;
@@ -607,18 +628,18 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       before = below;
       __syncthreads();
     }
-    if ((chunk >= 0 && before > goal) || k == a.chunks - 1) break;
+    if ((piece >= 0 && before > goal) || k == pieces - 1) break;
   }
-  if (chunk < 0) {  // (a weight that was the other ratio's alone: the residual is nothing)
+  if (piece < 0) {  // (a weight that was the other ratio's alone: the residual is nothing)
     const int64_t b = row_best(x.p, a.vocab, &shb);
     if (tid == 0) out[take] = b;
     return;
   }
-  if (chunk != k) weigh(chunk);  // (the last chunks had no weight)
+  if (piece != k) weigh(piece);  // (the last pieces had no weight)
   if (tid != who) return;
   double cum = first;  // its tokens, one after another
   int hit = 0;
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < 4; ++e) {
     const double y = wt[e][tid];
     cum += y;
     if (y > 0) {
@@ -626,24 +647,25 @@ __global__ __launch_bounds__(256) void verify_last_kernel(VerifyArgs a) {
       if (cum > goal) break;
     }
   }
-  out[take] = at * slice + (int64_t)chunk * kChunk + tid * 8 + hit;
+  out[take] = begin + (int64_t)piece * kPiece + tid * 4 + hit;
 }
 
 struct VerifyLayout {
-  int chunks;
+  int share;
   int64_t stats, slices, sum, pow, done, bytes;
 };
 VerifyLayout verify_layout(int64_t nseq, int64_t T, int64_t vocab, bool draft) {
   VerifyLayout l;
   const int64_t rows = T + nseq + (draft ? T : 0);
   l.stats = (vocab + kStatsSlice - 1) / kStatsSlice;
-  // (slices of the last rows: about 1024 workgroups, which run at once, and 256
-  // of a row at most)
-  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
-  l.chunks = (int)std::max((chunks + 255) / 256, (nseq * chunks + 1023) / 1024);
-  l.slices = (vocab + (int64_t)l.chunks * kChunk - 1) / ((int64_t)l.chunks * kChunk);
+  // (slices of the last rows, multiples of 2048: about 1024 workgroups, which run
+  // at once, and 64 of a row at most)
+  const int64_t chunks = (vocab + 2047) / 2048;
+  const int64_t each = std::min(chunks, std::max((chunks + 63) / 64, (nseq * chunks + 1023) / 1024));
+  l.share = (int)(each * 512);
+  l.slices = (chunks + each - 1) / each;
   l.sum = rows * l.stats * (int64_t)sizeof(RowStat);
-  l.pow = l.sum + nseq * l.slices * (int64_t)sizeof(SliceSum);
+  l.pow = l.sum + nseq * 4 * l.slices * (int64_t)sizeof(ShareSum);
   l.done = l.pow + kPow * (int64_t)sizeof(double);
   l.bytes = l.done + nseq * (int64_t)sizeof(uint32_t);
   return l;
@@ -705,10 +727,10 @@ extern "C" int swl_verify_drafts_bf16(const void* target, int64_t ld_target, con
   a.max_drafts = max_drafts;
   a.stats = (int32_t)l.stats;
   a.slices = (int32_t)l.slices;
-  a.chunks = l.chunks;
+  a.share = l.share;
   char* ws = reinterpret_cast<char*>(workspace);
   a.stat = reinterpret_cast<RowStat*>(ws);
-  a.sum = reinterpret_cast<SliceSum*>(ws + l.sum);
+  a.sum = reinterpret_cast<ShareSum*>(ws + l.sum);
   a.pow = reinterpret_cast<double*>(ws + l.pow);
   a.done = reinterpret_cast<uint32_t*>(ws + l.done);
   return launch_verify(a, (hipStream_t)stream);

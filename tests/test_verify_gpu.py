@@ -126,6 +126,8 @@ def _same(c, dev, max_drafts=None):
     ([2] * 70, 3000, [1.0, 0.9, 0.0, 2.0], 0),               # more than 64 sequences
     ([40, 17, 33], 500, [3.0, 8.0], 3),                      # more drafts than sixteen
     ([3] * 180, 16500, [0.9], 0),                            # rows of more than one slice
+    ([1] * 1100, 4100, [0.8], 0),                            # a wave's share in two pieces, and in three
+    ([1], 600001, [1.1], 0),
 ])
 def test_tokens_and_counts_equal_the_rule(dev, new, vocab, temps, pad, drafter):
     for seed in range(3):
