@@ -448,12 +448,21 @@ struct QFrag {
   i32x8 hi, lo;
   int sb;  // scale byte of hi; lo's is 4 less
 };
-__device__ __forceinline__ QFrag q_frag(const bf16* row, int g) {
+struct QRow {
+  u32x4 x[4];
+};
+__device__ __forceinline__ QRow q_row(const bf16* row, int g) {
+  QRow r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.x[j] = ldg16(row + 64 * (j >> 1) + 16 * g + 8 * (j & 1));
+  return r;
+}
+__device__ __forceinline__ QFrag q_frag(const QRow& r) {
   float x[4][8];
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    unpack8(ldg16(row + 64 * (j >> 1) + 16 * g + 8 * (j & 1)), x[j]);
+    unpack8(r.x[j], x[j]);
     top = max(top, top8(x[j]));
   }
   top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
@@ -651,12 +660,12 @@ __device__ __forceinline__ void split_unit(const Kv4Args& a, uint32_t unit, Spli
   };
   request(0);
 
-  QFrag q[SETS];
-  int ctx[SETS];  // keys that the lane's rows see, from the part's first step
+  QRow raw[SETS];  // (made operands behind the first records' requests)
+  int ctx[SETS];   // keys that the lane's rows see, from the part's first step
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
     const int r = min(r0 + e * 16 + col, rows - 1), tok = (uint32_t)r / a.by_g;
-    q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
+    raw[e] = q_row(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
     ctx[e] = min(max(u.len + tok + 1 - st0 * KS, 0), nst * KS);
   }
   const int all_see = min(max(last_key(a, u, r0) - st0 * KS, 0), nst * KS);  // keys that every row sees
@@ -701,6 +710,9 @@ __device__ __forceinline__ void split_unit(const Kv4Args& a, uint32_t unit, Spli
   look(0);
   load_k(0);
   load_v(0);
+  QFrag q[SETS];
+#pragma unroll
+  for (int e = 0; e < SETS; ++e) q[e] = q_frag(raw[e]);
   auto walk = [&](auto sets) {  // the wave's steps, for the sets that have rows
     constexpr int NS = decltype(sets)::value;
     for (int j = 0; j < nw; ++j) {
@@ -900,7 +912,7 @@ __device__ __forceinline__ void prompt_unit(const Kv4Args& a, uint32_t unit, Pro
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = min(wr0 + e * 16 + col, rows - 1), tok = (uint32_t)r / a.by_g;
-    q[e] = q_frag(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g);
+    q[e] = q_frag(q_row(a.q + (u.t0 + tok) * a.qs + (int64_t)(u.h * a.G + r - tok * a.G) * kD, g));
     ctx[e] = min(max(u.len + tok + 1 - st0 * KS, 0), nst * KS);
   }
   const int all_see = min(max(last_key(a, u, r0) - st0 * KS, 0), nst * KS);  // by every row
