@@ -63,9 +63,10 @@ struct VerifyArgs {
 };
 
 // order-preserving maps of a bf16's bits to 16 bits and back, a NaN of either
-// sign above all
+// sign above all, -0 the same as +0
 __device__ __forceinline__ uint32_t vkey16(uint32_t bits) {
   if ((bits & 0x7fffu) > 0x7f80u) return 0xffffu;
+  if (bits == 0x8000u) return 0x8000u;
   return (bits & 0x8000u) ? (~bits & 0xffffu) : (bits | 0x8000u);
 }
 __device__ __forceinline__ float vkey_value(uint32_t key) {

@@ -331,3 +331,23 @@ def test_random_numbers_next_to_the_border(dev, drafter):
         row += n + 1
     got = _same(c, dev)
     assert near >= 12 and int(got[1].sum()) >= 12
+
+
+@pytest.mark.parametrize("temp", [0.0, math.nan])
+def test_zeros_of_either_sign_are_equal(dev, temp):
+    """The first largest logit where -0 and +0 are the largest, -0 first: in one
+    thread's logits, in one slice, and in two; greedy rows, and rows whose
+    probabilities are no numbers (a temperature of NaN)."""
+    places = [(1, 2), (9, 4000), (100, 20000), (8191, 8192)]
+    V, n = 20001, 2 * len(places)
+    tgt = torch.full((n, 2, V), -1.0, dtype=BF16)
+    for i, (a, b) in enumerate(places):
+        for j, (x, y) in enumerate(((-0.0, 0.0), (0.0, -0.0))):
+            tgt[2 * i + j, :, a], tgt[2 * i + j, :, b] = x, y
+    first = torch.tensor([a for a, _ in places for _ in range(2)])
+    tok, acc = _ops().verify_drafts(tgt.to(dev), first.view(n, 1).to(dev), torch.zeros(n, 1, device=dev),
+                                    torch.full((n,), 0.5, device=dev), torch.full((n,), temp, device=dev))
+    if temp == 0.0:
+        assert acc.tolist() == [1] * n and tok.cpu().tolist() == [[f, f] for f in first.tolist()]
+    else:
+        assert acc.tolist() == [0] * n and tok.cpu().tolist() == [[f, -1] for f in first.tolist()]
