@@ -351,3 +351,27 @@ def test_zeros_of_either_sign_are_equal(dev, temp):
         assert acc.tolist() == [1] * n and tok.cpu().tolist() == [[f, f] for f in first.tolist()]
     else:
         assert acc.tolist() == [0] * n and tok.cpu().tolist() == [[f, -1] for f in first.tolist()]
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("temp", [1e-4, 1e-6, 1e-30, 1e-40])
+def test_temperatures_next_to_none(dev, temp, drafter):
+    """Positive temperatures so small that a logit's exponent leaves 32 bits:
+    all weight on the largest logits, shared where they tie."""
+    new, V = [2, 3, 1, 2], 9000
+    c = _case(17, new, V, drafter, [temp])
+    c["temp"][:] = temp
+    c["tgt"][:, 77] = -3e38
+    c["tgt"][0, [5, 4000]] = 60.0   # a tie: half each
+    c["tgt"][3, [6, 8999]] = 60.0
+    c["tgt"][2, [7, 8]] = 60.0      # behind two accepted drafts
+    c["ids"][0], c["ids"][2] = 5, 6
+    c["u"][:] = 0.4
+    if drafter:
+        c["drf"][0, 5] = c["drf"][2, 6] = 90.0
+        c["drf"][1, :] = c["tgt"][1, :]
+    c["ids"][1] = int(c["tgt"][1].float().argmax())
+    for u in (0.1, 0.7):
+        c["u_last"][:] = u
+        got = _same(c, dev)
+        assert got[1][0] == 2 and got[0][0, 2] == (7 if u < 0.5 else 8)
