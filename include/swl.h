@@ -450,8 +450,11 @@ int swl_kv4_read_bf16(const void* pages, int64_t num_blocks, int block_size, con
 /* Causal attention of the new tokens (already appended) over the cache: query
  * i of sequence s sees tokens 0 .. cache_seqlens[s] + i; query head j reads kv
  * head j / (hq / hkv), any hq that is a multiple of hkv.  out [ntok, hq *
- * 128], not q's memory; softmax_scale positive and finite.  Sums and softmax in
- * fp32.  A query that sees no token gets zeros, one with an infinity or a NaN, or
+ * 128], not q's memory; softmax_scale positive and finite.  Scores, the softmax's
+ * statistics and all sums are held in fp32.  Two operands have fewer bits: q's
+ * elements under 2^-13 of their row's largest are off by up to 2^-21 of that, and
+ * the probabilities multiply V as bf16 (each off by up to 2^-8 of itself, 0.0014 of
+ * the result, rms; the row's sum is of them as rounded).  A query that sees no token gets zeros, one with an infinity or a NaN, or
  * that sees a NaN key, NaN; a NaN value group reaches the queries that see it.
  * Values must leave room for their sum (under 2^118 / tokens).
  * max_q_len: the most new tokens of a sequence (a hint for speed alone: it
@@ -476,8 +479,11 @@ int swl_kv4_attention_bf16(const void* q, int64_t q_stride, int nseq, int64_t nt
  * (bf16 logits, row stride ld_target).  draft: the drafter's logits, a row per
  * draft (row stride ld_draft); NULL: the drafter was certain of every draft
  * (q = 1 there).
- * p, q: softmax of logits / temperature[s], held in 64 bits.  Draft j is
- * accepted while u_accept[j] * q_j(d) < p_j(d) (u in [0, 1)); the token after
+ * p, q: softmax of logits / temperature[s].  What decides is in 64 bits:
+ * comparisons that fp32 leaves open, and the weights that a token is drawn by (of
+ * max(p - q, 0) the weights of up to 256 stretches of the row are known to 2^-30
+ * of all of it together; a u_final that near to a border may give the token
+ * beyond).  Draft j is accepted while u_accept[j] * q_j(d) < p_j(d) (u in [0, 1)); the token after
  * the accepted ones is drawn from max(p - q, 0) where a draft was refused, else
  * from the row after the last one: the first index whose cumulative weight
  * exceeds u_final[s] of the whole.  temperature <= 0: greedy (a draft is

@@ -121,7 +121,7 @@ __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
 }
 
 // Scale byte of a group from the largest magnitude bits of its four lanes' 8
-// dims: the largest / 2^(b - 127) in [4, 7), so that it rounds as if the grid
+// dims: the largest / 2^(b - 127) in [3.5, 7), so that it rounds as if the grid
 // went on to 8 (5 % less of its error than with [4, 8), where up to 8 would be
 // cut to 6); [2, 252], so that every value held is a normal, finite bf16;
 // 255 (read as NaN) for a group with an infinity or a NaN.
@@ -335,10 +335,13 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // Steps of a part: the fewest (at least min_spp) that cut the call into no more
 // units than `slots`, the workgroups that run at once: a second round of a few
-// units costs as much as a whole one (28 sequences with drafted tokens, 736
-// units for 512 places 42.6 us, 496 units 34.8).  With as many blocks as
-// places, or more sequences than a wave's lanes, the steps are shared out
-// evenly instead.  Either way a part is at least steps / slots, so that there
+// units costs as much as a whole one (28 sequences with 1 to 6 drafted tokens
+// over 128 to 8192 keys 41 us, 44 with their steps shared out evenly).  With as
+// many blocks as places, or more sequences than a wave's lanes, the steps are
+// shared out evenly.  (Plans of several rounds are not looked at, though blocks
+// between half and all of the places would gain by one: four chunks of 300
+// tokens over 4000 keys, 320 blocks of 68 steps in 512 places, stay whole, 68
+// steps a place, where three parts each would be two rounds of 23.)  Either way a part is at least steps / slots, so that there
 // are at most `slots` full parts, `slots` + blocks units, `slots` blocks that
 // are cut and 2 `slots` records, whatever the lengths.  r: seq_info of the
 // lane's sequence.
@@ -442,7 +445,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // 16 rows of q as the B operand of the scaled MFMA: fp8 twice, the nearest and
 // what is left of it, both exact but for elements under 2^-13 of their row's
-// largest (off by 2^-22 of that): a bf16 has 8 significant bits, e4m3 4.  The
+// largest (off by 2^-21 of that at most: half of the second one's least step,
+// 2^-13, where the largest is 2^7): a bf16 has 8 significant bits, e4m3 4.  The
 // lane has dims 16 g .. + 15 and 64 + 16 g .. + 15, as the operand counts them.
 struct QFrag {
   i32x8 hi, lo;
@@ -607,13 +611,14 @@ __device__ __forceinline__ void write_row(const Kv4Args& a, const Unit& u, int r
 // results meet in LDS.  S^T = K Q^T (scaled MFMA, keys as stored) leaves in a
 // lane the keys 4 g .. + 3 of both tiles of its row, which is the B operand of
 // O^T = V^T P^T as it is.  The probabilities enter as one bf16 and are summed as
-// they are, as in the kernel for many rows.
+// they are, as in the kernel for many rows; a second bf16 of each would make the
+// three cases below 135, 35 and 15 us.
 //
 // The cache's bytes bound it once they are many: 32 tokens over 8192 to 32767
 // keys each (742 MB) take 124 us, 6.0 TB/s; 1 to 6 drafted tokens of 28 requests
 // over 128 to 8192 keys (122 MB) 30 us, with a second step of loads in flight a
 // wave 33.  Under that the chain of dependent loads (lengths, table, records)
-// does: 7 us for four tokens over 300 keys, 14.5 for 28 over 128 to 2048.
+// does: 7 us for four tokens over 300 keys, 14 for 28 over 128 to 2048.
 constexpr int kSplitWaves = 4;
 
 struct SplitLds {
@@ -865,10 +870,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
 // operand: no conversion, a quarter of bf16's bytes).  Values are made bf16
 // once for the four waves: wave w turns tile w of the step into MFMA operand
 // order and leaves it in LDS for the next step, one barrier a step.  The
-// probabilities enter as one bf16 (2^-9 of each, below the result's own
-// rounding where many keys share the weight; two would add half to the matrix
-// work of PV), and their sum is an MFMA row of ones over the same rounded
-// values, so that the weights sum to 1 exactly.
+// probabilities enter as one bf16 (off by 2^-8 of each at most, together 0.0014
+// of the result, rms, less than its own rounding and a hundredth of what 4 bits
+// cost; two would double the matrix work of PV: 760 us in place of 567 for the
+// prompts below, both traced), and their sum is an MFMA row of ones over the
+// same rounded values, so that the weights sum to 1 exactly.
 //
 // Exponents are taken from the row's largest score of its first 32 keys, and
 // no maximum is kept after that: a reference too low makes all terms larger by
@@ -878,10 +884,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
 // running maximum.
 //
 // Matrix and vector work bound it about alike: five prompts up to 8192 tokens
-// (600 GFLOP of visible scores and sums, 32 heads) take 517 us, 1160 TFLOP/s,
-// the matrix units busy 54 % of the time; with a running maximum and the
-// compiler's own order 1171 us.  128 rows a workgroup: with 32 every record
-// would be made bf16 four times as often.
+// (600 GFLOP of visible scores and sums, 32 heads) take 475 us, 1260 TFLOP/s
+// (567 under a kernel trace, which holds the clock lower), the matrix units busy
+// 54 % of the time; with a running maximum 656 us traced, with the compiler's
+// own order as well 1171.  128 rows a workgroup: with 32 every record would be
+// made bf16 four times as often.
 constexpr int kPromptRows = 128, kPromptKeys = 64;
 
 struct PromptLds {
@@ -1268,20 +1275,23 @@ struct Kv4Launch {
 struct Kv4Plan {
   Kv4Launch few, many;
 };
-// Sequences of at most kSplitRows rows go to the kernel for few rows: 28 with
-// 64 rows over 4000 keys 53 us there, 71 in the one for many; 8 with 96 over
-// 16000 keys 91 and 75, over 4000 37 and 35.  So do all sequences of a call
-// that cannot have more than kFewScores scores (tokens x keys of a table x query
-// heads), for it starts sooner and is cut finer: one sequence of 512 tokens over
-// 1500 keys (2^24.6 scores) 30 and 40 us, 128 over 4000 (2^24) 28 and 35, 64
-// over 16000 (2^25) 38 and 44; but 300 over 4000 (2^25.2) 51 and 45, two of 64
-// over 16000 (2^26) 55 and 50.
+// (Times of calls replayed in a graph, 8 kv heads of 4.)  Sequences of at most
+// kSplitRows rows go to the kernel for few rows: 28 with 64 rows over 4000 keys
+// 60 us there, 79 in the one for many; 8 with 96 over 16000 keys 98 and 83, over
+// 4000 36 and 37.  So do all sequences of a call that cannot have more than
+// kFewScores scores (tokens x keys of a table x query heads), for it starts
+// sooner and is cut finer: one sequence of 512 tokens over 1500 keys (2^24.6
+// scores) 30 and 42 us, 128 over 4000 (2^24) 27 and 40, 64 over 16000 (2^25) 36
+// and 61; but 300 over 4000 (2^25.2) 51 and 47, two of 64 over 16000 (2^26) 56
+// and 57.  (The host knows the table's width, not the lengths: 300 tokens alone
+// in a table of 8192 keys take 15.6 us there, 13.2 here.)
 constexpr int kSplitRows = 64;
 constexpr double kFewScores = 0x1p25;
 constexpr int kCus = 256;  // of an MI355X
 // Workgroups of a CU (registers), and steps of a part at least.  16 of 32 keys,
-// four a wave: 28 single tokens over 128 to 2048 keys 17 us, with 8 21.8.  8 of
-// 64 keys: 300 tokens alone 14 us, with 4 18.5; over 500 keys 25 and 28.
+// four a wave: 28 single tokens over 128 to 2048 keys 16.3 us, with 8 17.8; four
+// over 300 7.0 and 9.6 (a second launch).  8 of 64 keys: 300 tokens in a table of
+// 8192 keys 15.6 us, with 4 20.8; behind 500 others 27 and 29.5.
 constexpr int kSplit1PerCu = 4, kSplit2PerCu = 2, kPromptPerCu = 2, kSplitSteps = 16, kPromptSteps = 8;
 
 Kv4Launch kv4_launch(int64_t nseq, int64_t T, int G, int hkv, int64_t max_keys, int64_t max_rows, int rb, int ks,

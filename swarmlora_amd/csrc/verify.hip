@@ -11,14 +11,15 @@
 // What decides is held in 64 bits: with 128256 tokens a cumulative sum that is
 // off by 1e-7 of the total picks another token once in about forty draws.  A
 // 64-bit exponential costs fifteen times an fp32 one, though (28 sequences of 1
-// to 5 drafts, 128256 tokens: 77 us with 64 bits throughout, 35 now), and most rows only
-// have to show that their draft is accepted: u q < p is clear in fp32 unless the
-// two are within 2^-14 of each other.  So, in two launches: every row's maximum
-// and sum in fp32, a workgroup per slice of a row (the logits' bytes are its
-// bound); then a workgroup per slice of every sequence's last row: acceptance
-// (each for itself; a comparison that is not clear again in 64 bits over the
-// whole row), the slice's weight in 64 bits, and by the workgroup that ends last
-// the slice and token that the random number falls in.
+// to 5 drafts, 128256 tokens: 77 us with 64 bits throughout, 32 now), and most
+// rows only have to show that their draft is accepted: u q < p is clear in fp32
+// unless the two are within 2^-14 of each other.  So, in two launches: every
+// row's maximum and sum in fp32, a workgroup per slice of a row (the logits'
+// bytes are its bound); then a workgroup per slice of every sequence's last row:
+// acceptance (each for itself; a comparison that is not clear again in 64 bits
+// over the whole row), the weights of the slice's four shares (a wave's each) in
+// 64 bits, and by the workgroup that ends last the share that the random number
+// falls in, and its token.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -177,7 +178,7 @@ __device__ __forceinline__ double block_prefix(double v, double* sh) {
 // (Slices of 2048 for calls of few rows were level at best: one sequence of 4
 // drafts and 32000 tokens 13.6 us for both launches instead of 13.7, 28 rows of
 // 128256 19.3 instead of 17.4, 448 rows 70 instead of 60.)  The logits' bytes
-// bound it: 196 rows of 128256 take 13.4 us, 3.8 TB/s.
+// bound it: 196 rows of 128256 take 12.8 us, 3.9 TB/s.
 constexpr int kStatsSlice = 8192;
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   __shared__ uint32_t shk[4];
@@ -384,12 +385,12 @@ __device__ __forceinline__ double get(const double* p) {
 // Where it could be more than 2^-30 of the residual (rows that are nearly the
 // same) the last workgroup adds the shares up again at the exact ratio.
 //
-// 10.5 us for one sequence of 4 drafts, 22 for 28 of up to 5 (128256 tokens, with
-// a drafter): a chain of loads, sums and one count in memory (5 us until the
-// weights, 6 behind them), and 64-bit arithmetic of some 6 us by its count, spread
-// over the card; every slice is there at once, so that this chain is met once.
-// Sums of whole slices, 4096 logits instead of 1024 to look through at the end:
-// 27 us.
+// 10.5 us for one sequence of 4 drafts (32000 tokens, no drafter): a chain of
+// loads, sums and one count in memory (5 us until the weights, 6 behind them); 22
+// for 28 of up to 5 (128256 tokens, with a drafter): the same chain, met once, for
+// every slice is there at once, and 64-bit arithmetic of some 6 us by its count,
+// spread over the card.  (What the other 6 are has not been found.)  Sums of whole
+// slices, 4096 logits instead of 1024 to look through at the end: 27 us.
 constexpr double kNear = 0x1p-18;  // (the fp32 sums' ratio is nearer than half of it but for rows out of the way)
 constexpr int kPiece = 1024;  // logits of a share that the last workgroup looks at together, four a thread
 

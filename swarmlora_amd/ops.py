@@ -1058,7 +1058,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     gives [nseq, L, hq * 128]; packed q [tokens, hq, 128] with cu_seqlens gives
     [tokens, hq * 128], rows behind the last sequence left as they were in
     `out`.  max_q_len: the most new tokens of a sequence where the host knows
-    it (a hint for speed alone)."""
+    it (a hint for speed alone).  fp32 throughout but for the probabilities,
+    which multiply the values as bf16 (0.0014 of the result, rms)."""
     dev = _device_for(q, "q", BF16)
     qshape, ntok, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
     nseq, nb, hkv, bs, mb = _kv4_cache(pages, block_table, cache_seqlens, "cache_seqlens", qshape[0], cu_seqlens, dev)
