@@ -884,7 +884,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, SETS == 1 ? 4 : 2) void kv4_split
 // running maximum.
 //
 // Matrix and vector work bound it about alike: five prompts up to 8192 tokens
-// (600 GFLOP of visible scores and sums, 32 heads) take 475 us, 1260 TFLOP/s
+// (600 GFLOP of visible scores and sums, 32 heads) take 480 us, 1250 TFLOP/s
 // (567 under a kernel trace, which holds the clock lower), the matrix units busy
 // 54 % of the time; with a running maximum 656 us traced, with the compiler's
 // own order as well 1171.  128 rows a workgroup: with 32 every record would be

@@ -178,7 +178,7 @@ __device__ __forceinline__ double block_prefix(double v, double* sh) {
 // (Slices of 2048 for calls of few rows were level at best: one sequence of 4
 // drafts and 32000 tokens 13.6 us for both launches instead of 13.7, 28 rows of
 // 128256 19.3 instead of 17.4, 448 rows 70 instead of 60.)  The logits' bytes
-// bound it: 196 rows of 128256 take 12.8 us, 3.9 TB/s.
+// bound it: 196 rows of 128256 take 13 us, 3.9 TB/s.
 constexpr int kStatsSlice = 8192;
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   __shared__ uint32_t shk[4];
