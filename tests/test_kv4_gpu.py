@@ -610,3 +610,60 @@ def test_worker_attention_over_a_cache_of_four_bits(dev):
     kv.free_slot(2)
     for p in kv.pages:
         assert not bool(p[blocks].any()) and bool(p[kv.slot_block_tables[0]].any())
+
+
+@pytest.mark.parametrize("ctx,new", [([700, 40], [1, 1]), ([300, 5], [6, 2]), ([60, 0], [150, 90])])
+def test_attention_of_values_and_keys_of_every_scale(dev, ctx, new):
+    """Value groups from 2^-110 to 2^100 beside one another, whole groups of zeros
+    among them, and keys whose groups are up to 2^40 apart under queries that undo
+    it."""
+    ops = _ops()
+    hq, hkv, page = 4, 2, 16
+    total = [c + n for c, n in zip(ctx, new)]
+    T = sum(total)
+    g = torch.Generator().manual_seed(T)
+    bt, nb = _tables(total, page, 17)
+    v = randn((T, hkv, 128), 5).float().unflatten(-1, (4, 32))
+    v = v * torch.exp2(torch.randint(-110, 101, (T, hkv, 4, 1), generator=g).float())
+    v = (v * (torch.rand(T, hkv, 4, 1, generator=g) > 0.2)).flatten(-2).to(BF16)
+    up = torch.exp2(torch.tensor([-20.0, 0.0, 20.0, 7.0])).repeat_interleave(32)
+    k = (randn((T, hkv, 128), 6).float() * up).to(BF16)
+    q = (randn((sum(new), hq, 128), 7).float() / up).to(BF16)
+    pages = ops.kv4_pages(nb, page, hkv, dev)
+    ops.kv4_append(k.to(dev), v.to(dev), pages, bt.to(dev), torch.zeros(2, dtype=torch.int32, device=dev),
+                   cu_seqlens=_prefix(total).to(dev))
+    # q's elements under 2^-13 of their row's largest are rounded by its operands (two fp8 numbers),
+    # and these keys weigh them up again: the definition is taken over q as it is held
+    big = q.double().abs().amax(-1, keepdim=True)
+    s = torch.exp2(torch.floor(torch.log2(big)) - 7)
+    held = _fp8_twice(q.double() / s) * s
+    want, wt = _kv4.attend(held, pages.cpu(), bt, ctx, _prefix(new).tolist(), SCALE)
+    for wide in (False, True):
+        out = ops.kv4_attention(q.to(dev), pages, _wide(bt, wide).to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev),
+                                SCALE, cu_seqlens=_prefix(new).to(dev))
+        _check(out, want, wt, 2.0 ** -7)
+
+
+def _fp8_twice(x):
+    """x as an e4m3 number and what is left of it as another sixteenth of it,
+    ties to even."""
+    def e4m3(y):
+        step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+        return torch.round(y / step) * step
+    hi = e4m3(x)
+    return hi + e4m3((x - hi) * 16) / 16
+
+
+def test_read_of_more_rows_than_the_sequences_have(dev):
+    """Packed rows behind the last sequence hold anything; those before are
+    what they are, empty sequences among them."""
+    ops = _ops()
+    pages, bt = _filled([40, 17, 90], 2, 16, 33)
+    new, starts = [5, 0, 33], [30, 3, 50]
+    k, v = ops.kv4_read(pages, bt.to(dev), torch.tensor(starts, dtype=torch.int32, device=dev), 100,
+                        cu_seqlens=_prefix(new).to(dev))
+    at = 0
+    for s, n in enumerate(new):
+        rk, rv, _ = _kv4.load(pages.cpu(), bt, s, starts[s] + n)
+        assert torch.equal(k[at:at + n].cpu().double(), rk[starts[s]:]) and torch.equal(v[at:at + n].cpu().double(), rv[starts[s]:])
+        at += n

@@ -375,3 +375,42 @@ def test_temperatures_next_to_none(dev, temp, drafter):
         c["u_last"][:] = u
         got = _same(c, dev)
         assert got[1][0] == 2 and got[0][0, 2] == (7 if u < 0.5 else 8)
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+def test_drafts_behind_the_last_sequence_belong_to_none(dev, drafter):
+    """Offsets that end before the drafts do: a captured call of fixed shapes
+    whose offsets, drafts and temperatures change between replays."""
+    ops, V, T, n = _ops(), 3001, 12, 4
+    c = _case(50, [3] * n, V, drafter, [0.8])
+    keys = [k for k in ("tgt", "drf", "ids", "u", "u_last", "temp") if c[k] is not None]
+    d = {k: c[k].to(dev) for k in keys}
+    cu = torch.zeros(n + 1, dtype=torch.int32, device=dev)
+
+    def call():
+        return ops.verify_drafts(d["tgt"], d["ids"], d["u"], d["u_last"], d["temp"], d.get("drf"), cu_drafts=cu, max_drafts=5)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tok, acc = call()
+    for i, new in enumerate([[3, 3, 3, 3], [0, 5, 1, 2], [1, 0, 0, 0], [0, 0, 0, 0], [2, 4, 4, 2]]):
+        c = _case(60 + i, new, V, drafter, [0.8, 0.0, 1.3])
+        used = sum(new)
+        for k, rows in (("tgt", used + n), ("drf", used), ("ids", used), ("u", used)):
+            if k in d:
+                d[k].fill_(math.nan if d[k].is_floating_point() else 7)
+                d[k][:rows].copy_(c[k])
+        d["u_last"].copy_(c["u_last"])
+        d["temp"].copy_(c["temp"])
+        cu.copy_(torch.tensor([0] + new).cumsum(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = rule(c["tgt"], c["ids"], c["u"], c["u_last"], c["temp"], c["drf"], new, 5)
+        assert torch.equal(tok.cpu(), want[0]) and torch.equal(acc.cpu(), want[1])
+        eager = call()
+        assert torch.equal(eager[0], tok) and torch.equal(eager[1], acc)
