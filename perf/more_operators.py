@@ -168,7 +168,7 @@ def _prepare_share(case, gen):
     ang = torch.outer(torch.arange(far, device=DEV, dtype=torch.float64),
                       THETA ** (-torch.arange(0, D, 2, device=DEV, dtype=torch.float64) / D))
     return {"op": "share", "new": new, "ctx": ctx, "pre": pre, "group": group, "kc": kc, "vc": vc, "pt": pt, "bt": bt,
-            "plen": _i32(pre), "lens": _i32(ctx), "cu": _prefix(new), "cg": _prefix(size), "max_new": max(new), "T": T,
+            "plen": _i32(pre), "lens": _i32(ctx), "cu": _prefix(new), "cg": _prefix(size), "T": T,
             "q": qkv[:, :hq * D].view(T, hq, D), "k": qkv[:, hq * D:(hq + hkv) * D].view(T, hkv, D),
             "v": qkv[:, (hq + hkv) * D:].view(T, hkv, D), "pos": pos, "scale": 1.0 / math.sqrt(D),
             "cos_sin": torch.cat([ang.cos(), ang.sin()], -1).to(BF16).contiguous()}
@@ -304,7 +304,7 @@ def run(st):
     if st["op"] == "share":
         out = ops.prefix_attention(st["q"], st["k"], st["v"], st["kc"], st["vc"], st["pt"], st["plen"], st["bt"],
                                    st["lens"], st["pos"], st["cos_sin"], st["scale"], cu_groups=st["cg"],
-                                   cu_seqlens=st["cu"], max_q_len=st["max_new"])
+                                   cu_seqlens=st["cu"])
         return [out, st["kc"], st["vc"]]
     if st["op"] == "sample":
         return ops.sample_tokens(st["x"], st["u"], st["temp"], st["top_k"], st["top_p"], st["min_p"])
