@@ -503,6 +503,50 @@ int swl_verify_drafts_bf16(const void* target, int64_t ld_target, const void* dr
                            int64_t* out_tokens, int32_t* out_accepted, void* workspace, int64_t workspace_bytes,
                            void* stream);
 
+/* ------------------------------------- attention over a shared prefix ----
+ * No counterpart in the reference.  Sequences come in groups: those of group g,
+ * cu_groups[g] .. cu_groups[g + 1] - 1 (device int32 [ngroups + 1], ascending;
+ * NULL with one group: all of them), share prefix_lens[g] tokens held in the pages
+ * prefix_table[g] (int32 [ngroups, max_prefix_blocks]), and go on in pages of their
+ * own, block_table [nseq, max_blocks], where they have cache_seqlens[s] tokens
+ * before the new ones.  A sequence in no group has no prefix.  Prefix and own
+ * tokens begin in a page of their own each; the prefix may end inside one.  Pages
+ * k_cache, v_cache: bf16 [num_blocks, block_size, hkv, 128], any block_size,
+ * num_blocks * block_size under 2^31.  New tokens are packed as above
+ * (cu_seqlens; NULL: ntok / nseq each).
+ *   1. The new keys, rotated (NeoX halves) at positions [ntok] from cos_sin
+ *      [max_pos, 128] (both NULL: no rotation; a position outside 0 .. max_pos - 1:
+ *      that token is not rotated), and the new values are stored as own tokens
+ *      cache_seqlens[s] + i (k and v NULL: they are there already).  A token whose
+ *      page is outside the table, or outside 0 .. num_blocks - 1, is not stored,
+ *      and not attended to.  q, k and v are left as they are: the rotated queries
+ *      (rounded to bf16) are in the workspace.
+ *   2. Query i of sequence s attends to its group's prefix and to its own tokens
+ *      0 .. cache_seqlens[s] + i; query head j reads kv head j / (hq / hkv).  out
+ *      [ntok, hq * 128], not q's memory; rows behind the last sequence are left as
+ *      they were.
+ * Scores, the softmax's statistics and all sums are held in fp32; the
+ * probabilities multiply the values as bf16 (each off by up to 2^-8 of itself; the
+ * row's sum is of them as rounded).  A query that sees no token gets zeros.
+ * Infinities and NaN reach the queries that see their token, nobody else.  Values
+ * must leave room for their sum (under 2^118 / tokens).
+ * nseq + ngroups at most 4096, ntok under 2^25.  workspace:
+ * swl_prefix_attention_workspace(nseq, ntok, ngroups, hq, hkv, max_prefix_blocks *
+ * block_size, max_blocks * block_size, positions != NULL) bytes of device memory,
+ * 16-byte aligned, owned by the call until its kernels have run; its contents do
+ * not matter.  Can be captured into a graph; lengths and tables are read when it
+ * runs. */
+int64_t swl_prefix_attention_workspace(int nseq, int64_t ntok, int ngroups, int hq, int hkv, int64_t max_prefix_keys,
+                                       int64_t max_keys, int rotate);
+int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                              int64_t v_stride, int nseq, int64_t ntok, const int32_t* cu_seqlens, int hq, int hkv,
+                              int d, void* k_cache, void* v_cache, int64_t num_blocks, int block_size,
+                              const int32_t* prefix_table, int64_t max_prefix_blocks, const int32_t* prefix_lens,
+                              const int32_t* cu_groups, int ngroups, const int32_t* block_table, int64_t max_blocks,
+                              const int32_t* cache_seqlens, const int64_t* positions, const void* cos_sin,
+                              int64_t max_pos, float softmax_scale, void* out, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

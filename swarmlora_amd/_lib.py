@@ -139,6 +139,10 @@ _SIGS = {
     "swl_verify_drafts_workspace": (c_i64, [c_int, c_i64, c_i64, c_int]),
     "swl_verify_drafts_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_int, c_vp, c_vp,
                                        c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "swl_prefix_attention_workspace": (c_i64, [c_int, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_int]),
+    "swl_prefix_attention_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_int, c_int,
+                                          c_vp, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_vp,
+                                          c_vp, c_vp, c_i64, c_f32, c_vp, c_vp, c_i64, c_vp]),
 }
 
 _RUNTIME_SIGS = {}

@@ -27,6 +27,7 @@ SOURCES = [
     "kernels.hip",
     "kv4.hip",
     "verify.hip",
+    "prefix.hip",
     "ipc_queue.cpp",
     "aggregator.cpp",
     "worker_slots.cpp",

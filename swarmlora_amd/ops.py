@@ -1088,6 +1088,104 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     return out
 
 
+# --------------------------------------- attention over a shared prefix ---
+@functools.lru_cache(maxsize=1024)
+def _prefix_workspace(nseq: int, ntok: int, ngroups: int, hq: int, hkv: int, pre: int, keys: int, rotate: int) -> int:
+    return _lib.load().swl_prefix_attention_workspace(nseq, ntok, ngroups, hq, hkv, pre, keys, rotate)
+
+
+def prefix_attention(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor], k_cache: torch.Tensor,
+                     v_cache: torch.Tensor, prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+                     block_table: torch.Tensor, cache_seqlens: torch.Tensor, positions: Optional[torch.Tensor],
+                     cos_sin: Optional[torch.Tensor], softmax_scale: float, cu_groups: Optional[torch.Tensor] = None,
+                     cu_seqlens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """paged_attention for sequences that share a prefix, which is read once for
+    all of a group (swl_prefix_attention_bf16).  Group g (sequences cu_groups[g]
+    .. cu_groups[g + 1] - 1, int32; None: all sequences in one group) has
+    prefix_lens[g] tokens in the pages prefix_table[g]; block_table and
+    cache_seqlens tell of the tokens behind it, which begin in pages of their
+    own.  q [nseq, L, hq, 128], k/v [nseq, L, hkv, 128], or packed [tokens,
+    heads, 128] with cu_seqlens int32 [nseq + 1]; tokens may be strided (views of
+    the fused QKV rows).  New keys are rotated at `positions` (int64, one per
+    token, counted from the prefix's start; None: no rotation) and stored with the
+    values behind cache_seqlens; k and v None: they were before.  q, k and v are
+    left as they are.  Returns [nseq, L, hq * 128], packed [tokens, hq * 128];
+    rows behind the last sequence are left as they were in `out`."""
+    dev = _device_for(q, "q", BF16)
+    qshape, ntok, hq, qs = _packed_rows(q, "q", cu_seqlens, dev)
+    _here(k_cache, "k_cache", BF16, dev)
+    _here(v_cache, "v_cache", BF16, dev)
+    cache = k_cache.shape
+    if len(cache) != 4 or cache[3] != 128 or v_cache.shape != cache or not (
+            k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache and v_cache must be contiguous [num_blocks, block_size, hkv, 128]")
+    nb, bs, hkv, _ = cache
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    nseq = qshape[0]
+    if cu_seqlens is not None:
+        _here(cu_seqlens, "cu_seqlens", _I32, dev)
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be contiguous [nseq + 1]")
+        nseq = cu_seqlens.shape[0] - 1
+    for t, nm in ((prefix_table, "prefix_table"), (prefix_lens, "prefix_lens"), (block_table, "block_table"),
+                  (cache_seqlens, "cache_seqlens")):
+        _here(t, nm, _I32, dev)
+        if not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous")
+    pt, bt = prefix_table.shape, block_table.shape
+    if len(pt) != 2 or prefix_lens.shape != pt[:1]:
+        raise ValueError("prefix_table must be [ngroups, max_prefix_blocks], prefix_lens [ngroups]")
+    if len(bt) != 2 or bt[0] < nseq or cache_seqlens.dim() != 1 or cache_seqlens.shape[0] < nseq:
+        raise ValueError("block_table must be [nseq, max_blocks] and cache_seqlens have nseq entries")
+    ng, mp = pt
+    if mp == 0:
+        ng = 0
+    if cu_groups is not None:
+        _here(cu_groups, "cu_groups", _I32, dev)
+        if cu_groups.shape != (pt[0] + 1,) or not cu_groups.is_contiguous():
+            raise ValueError("cu_groups must be contiguous [ngroups + 1]")
+    elif ng > 1:
+        raise ValueError("more than one group needs cu_groups")
+    if (k is None) != (v is None):
+        raise ValueError("k and v go together")
+    ks = vs = 0
+    if k is not None:
+        kshape, _, kh, ks = _packed_rows(k, "k", cu_seqlens, dev)
+        vshape, _, _, vs = _packed_rows(v, "v", cu_seqlens, dev)
+        if kshape != vshape or kshape[:-2] != qshape[:-2]:
+            raise ValueError("q, k and v must have the same tokens")
+        if kh != hkv:
+            raise ValueError("cache geometry mismatch")
+    if (positions is None) != (cos_sin is None):
+        raise ValueError("positions and cos_sin go together")
+    max_pos = 0
+    if positions is not None:
+        _here(positions, "positions", torch.int64, dev)
+        _here(cos_sin, "cos_sin", BF16, dev)
+        if positions.numel() != ntok or not positions.is_contiguous():
+            raise ValueError("positions must be contiguous with one entry per token")
+        table = cos_sin.shape
+        if len(table) != 2 or table[1] != 128 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be contiguous [max_pos, 128]")
+        max_pos = table[0]
+    shape = (*qshape[:-2], hq * 128)
+    if out is None:
+        out = q.new_empty(shape)
+    else:
+        _here(out, "out", BF16, dev)
+        if out.shape != shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous [.., hq * 128] with q's tokens")
+    need = _prefix_workspace(nseq, ntok, ng, hq, hkv, mp * bs if ng else 0, bt[1] * bs, 0 if positions is None else 1)
+    ws = q.new_empty(need, dtype=_U8)
+    _lib.check(_lib.load().swl_prefix_attention_bf16(
+        q.data_ptr(), qs, _addr(k), ks, _addr(v), vs, nseq, ntok, _addr(cu_seqlens), hq, hkv, 128, k_cache.data_ptr(),
+        v_cache.data_ptr(), nb, bs, prefix_table.data_ptr(), mp, prefix_lens.data_ptr(),
+        _addr(cu_groups) if ng else None, ng, block_table.data_ptr(), bt[1], cache_seqlens.data_ptr(), _addr(positions),
+        _addr(cos_sin), max_pos, float(softmax_scale), out.data_ptr(), ws.data_ptr(), need, _stream_of(dev)))
+    return out
+
+
 # -------------------------------------------------------------- timing ---
 def timer_arm(capacity: int):
     """Record HIP events around the next `capacity` decode-projection launches
