@@ -547,6 +547,32 @@ int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const void* k, in
                               int64_t max_pos, float softmax_scale, void* out, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
+/* The next token of every row of logits (bf16 [n, vocab], row stride ld) from
+ * given random numbers; no counterpart in the reference, whose sampler
+ * (swl_sample_bf16) takes its parameters from the host and its numbers from a
+ * generator.  All parameters are device arrays of n entries, read when the call
+ * runs, so that a captured call samples anew each time.
+ * With w_i = e^((x_i - largest) / temperature) and the row's tokens in the order of
+ * falling logits (equal ones, -0 and +0 too, by index), a beginning of that order is
+ * kept, the shortest of: the first top_k; of those, the fewest whose weight reaches
+ * top_p of theirs; those with w_i >= min_p; at least the first token.  The token
+ * drawn is the first, in the order of indexes, whose cumulative weight exceeds u of
+ * all that is kept (u in [0, 1); a u outside draws the first or last token of any
+ * weight).  top_k NULL, <= 0 or >= vocab, top_p NULL or >= 1, min_p NULL or <= 0: no
+ * such filter (a NaN is none).  temperature not above 0: the first largest logit;
+ * so too for rows whose weights are no numbers (a NaN, counted above all, or an
+ * infinity as the largest logit, or nothing but -inf).  Logits of -inf never come.
+ * Weights are 64-bit exponentials in whole multiples of 2^-46 (2^(ceil(log2 vocab)
+ * - 63) for vocabularies over 2^17) of the largest, summed exactly: the result
+ * does not depend on the order of any sum.
+ * n at most 65535, vocab at most 2097152.  workspace:
+ * swl_sample_tokens_workspace(n, vocab) bytes of device memory, 16-byte aligned,
+ * owned by the call until its kernels have run; its contents do not matter. */
+int64_t swl_sample_tokens_workspace(int64_t n, int64_t vocab);
+int swl_sample_tokens_bf16(const void* logits, int64_t ld, int64_t n, int64_t vocab, const float* u,
+                           const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                           int64_t* out_tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

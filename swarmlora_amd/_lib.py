@@ -143,6 +143,9 @@ _SIGS = {
     "swl_prefix_attention_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_int, c_int,
                                           c_vp, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_vp,
                                           c_vp, c_vp, c_i64, c_f32, c_vp, c_vp, c_i64, c_vp]),
+    "swl_sample_tokens_workspace": (c_i64, [c_i64, c_i64]),
+    "swl_sample_tokens_bf16": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
+                                       c_vp]),
 }
 
 _RUNTIME_SIGS = {}

@@ -28,6 +28,7 @@ SOURCES = [
     "kv4.hip",
     "verify.hip",
     "prefix.hip",
+    "sampling.hip",
     "ipc_queue.cpp",
     "aggregator.cpp",
     "worker_slots.cpp",

@@ -726,6 +726,36 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept
     return tok, acc
 
 
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The next token of every row of logits bf16 [n, vocab] (rows may be strided)
+    from given random numbers u fp32 [n] in [0, 1) (swl_sample_tokens_bf16, which
+    states the rule): temperature fp32 [n] (<= 0: greedy), top_k int32 [n] (<= 0:
+    off), top_p fp32 [n] (>= 1: off), min_p fp32 [n] (<= 0: off).  All of them are
+    read on the device when the call runs, so that a captured step samples anew with
+    every replay (sample() takes host values).  Returns int64 [n], in `out` or a new
+    tensor."""
+    dev = _device_for(logits, "logits", BF16)
+    n, vocab, ld = _logit_rows(logits, "logits", True, dev)
+    for t, nm, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32), (top_k, "top_k", _I32),
+                      (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32), (out, "out", torch.int64)):
+        if t is None and nm not in ("u", "temperature"):
+            continue
+        _here(t, nm, dt, dev)
+        if t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous with one entry per row")
+    if out is None:
+        out = logits.new_empty(n, dtype=torch.int64)
+    lib = _lib.load()
+    need = lib.swl_sample_tokens_workspace(n, vocab)
+    ws = logits.new_empty(need, dtype=_U8)
+    _lib.check(lib.swl_sample_tokens_bf16(logits.data_ptr(), ld, n, vocab, u.data_ptr(), temperature.data_ptr(),
+                                          _addr(top_k), _addr(top_p), _addr(min_p), out.data_ptr(), ws.data_ptr(), need,
+                                          _stream_of(dev)))
+    return out
+
+
 def zero_blocks(caches: Sequence[torch.Tensor], block_ids: torch.Tensor):
     """Zero whole pages block_ids of every cache [num_blocks, ...]."""
     _need(block_ids, "block_ids", torch.int64)
