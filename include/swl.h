@@ -573,6 +573,40 @@ int swl_sample_tokens_bf16(const void* logits, int64_t ld, int64_t n, int64_t vo
                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                            int64_t* out_tokens, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------- products in 8-bit integers ----
+ * No counterpart in the reference (its projections are bf16 matmuls,
+ * ext_aggregator.cpp:545-621).  A row is held as codes in -127 .. 127 and one
+ * scale: scale = largest magnitude / 127, code = element * 127 / largest, to the
+ * nearest, halves to even; a row of zeros has scale 0, one with an infinity or a NaN
+ * codes of 0 and a NaN scale.  k at most 131072, so that no sum leaves 32 bits.
+ * All calls can be captured into a graph. */
+
+/* Codes q [m, k] (int8, row stride ldq, a multiple of 16 of at least k rounded up to
+ * 16; the bytes from k up to there become 0; 16-byte aligned) and scales [m] of the
+ * rows x [m, k] (bf16, row stride ldx, any alignment). */
+int swl_int8_rows_bf16(const void* x, int64_t ldx, int64_t m, int64_t k, void* q, int64_t ldq, float* scale,
+                       void* stream);
+
+/* A weight w [n, k] (bf16, row stride ldw) as codes and a scale for each of its n
+ * rows (output channels).  data: swl_int8_weight_bytes(n, k) bytes, 16-byte aligned:
+ * tiles of 16 rows, each whole, as blocks of 64 k (an even number of them), 1 KiB,
+ * 16 (r % 16) + 256 (k % 64 / 16) + k % 16 the byte of row r's column k; rows past n
+ * and columns past k are zeros.  scale: fp32 [n]. */
+int64_t swl_int8_weight_bytes(int64_t n, int64_t k);
+int swl_int8_pack_bf16(const void* w, int64_t ldw, int64_t n, int64_t k, void* data, float* scale, void* stream);
+
+/* y[i][j] = bf16(q_scale[i] * w_scale[j] * sum_k q[i][k] w[j][k] + bias[j]): q int8
+ * [m, k] (row stride ldq, a multiple of 16; of every row, the last too, the bytes up
+ * to k rounded up to 16 are read and may hold anything), w and w_scale as made by
+ * swl_int8_pack_bf16, bias bf16 [n] or NULL, y bf16 [m, n] (row stride ldy, 8-byte
+ * aligned).  The sum is exact (int32); scales, their product and the sum with the
+ * bias are fp32.  workspace: swl_int8_matmul_workspace(m, n, k) bytes (0 for many
+ * sizes), 16-byte aligned, owned by the call until its kernels have run. */
+int64_t swl_int8_matmul_workspace(int64_t m, int64_t n, int64_t k);
+int swl_int8_matmul_bf16(const void* q, int64_t ldq, const float* q_scale, int64_t m, const void* w,
+                         const float* w_scale, int64_t n, int64_t k, const void* bias, void* y, int64_t ldy,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

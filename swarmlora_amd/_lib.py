@@ -143,6 +143,12 @@ _SIGS = {
     "swl_prefix_attention_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_int, c_int,
                                           c_vp, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_vp,
                                           c_vp, c_vp, c_i64, c_f32, c_vp, c_vp, c_i64, c_vp]),
+    "swl_int8_rows_bf16": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "swl_int8_weight_bytes": (c_i64, [c_i64, c_i64]),
+    "swl_int8_pack_bf16": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "swl_int8_matmul_workspace": (c_i64, [c_i64, c_i64, c_i64]),
+    "swl_int8_matmul_bf16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp,
+                                     c_i64, c_vp]),
     "swl_sample_tokens_workspace": (c_i64, [c_i64, c_i64]),
     "swl_sample_tokens_bf16": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                        c_vp]),

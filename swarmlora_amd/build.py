@@ -29,6 +29,7 @@ SOURCES = [
     "verify.hip",
     "prefix.hip",
     "sampling.hip",
+    "int8.hip",
     "ipc_queue.cpp",
     "aggregator.cpp",
     "worker_slots.cpp",

@@ -1118,6 +1118,101 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     return out
 
 
+# ------------------------------------------- products in 8-bit integers ---
+class Int8Weight:
+    """A weight w bf16 [n, k] (rows may be strided) held in 8-bit integers with a
+    scale for each output channel, laid out for int8_matmul (swl_int8_pack_bf16).
+    `data` is flat uint8, `scale` fp32 [n]; w itself is not kept."""
+
+    def __init__(self, w: torch.Tensor):
+        dev = _device_for(w, "w", BF16)
+        _here(w, "w", BF16, dev)
+        if w.dim() != 2 or (w.shape[1] > 1 and w.stride(1) != 1) or w.shape[0] < 1 or w.shape[1] < 1:
+            raise ValueError("w must be an [n, k] matrix with unit column stride")
+        self.n, self.k = w.shape
+        ld = w.stride(0) if self.n > 1 else self.k
+        lib = _lib.load()
+        self.data = w.new_empty(lib.swl_int8_weight_bytes(self.n, self.k), dtype=_U8)
+        self.scale = w.new_empty(self.n, dtype=torch.float32)
+        _lib.check(lib.swl_int8_pack_bf16(w.data_ptr(), ld, self.n, self.k, self.data.data_ptr(), self.scale.data_ptr(),
+                                          _stream_of(dev)))
+
+    @property
+    def shape(self):
+        return (self.n, self.k)
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def int8_rows(x: torch.Tensor):
+    """Rows of x bf16 [m, k] (rows may be strided) as 8-bit integers: (codes int8
+    [m, k], scales fp32 [m]), codes * scale nearest to x (swl_int8_rows_bf16).  The
+    codes' rows are k rounded up to 16 apart."""
+    dev = _device_for(x, "x", BF16)
+    _here(x, "x", BF16, dev)
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.shape[1] < 1:
+        raise ValueError("x must be an [m, k] matrix with unit column stride")
+    m, k = x.shape
+    ld = x.stride(0) if m > 1 else k
+    if ld < k:
+        raise ValueError("x rows must not overlap")
+    ldq = (k + 15) // 16 * 16
+    q = x.new_empty((m, ldq), dtype=torch.int8)
+    scale = x.new_empty(m, dtype=torch.float32)
+    _lib.check(_lib.load().swl_int8_rows_bf16(x.data_ptr(), ld, m, k, q.data_ptr(), ldq, scale.data_ptr(),
+                                              _stream_of(dev)))
+    return q if ldq == k else q[:, :k], scale
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_workspace(m: int, n: int, k: int) -> int:
+    return _lib.load().swl_int8_matmul_workspace(m, n, k)
+
+
+def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: Int8Weight, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gemm in 8-bit integers: bf16 [m, n] = scale[i] * w.scale[j] * (q @ codes of
+    w.T) (+ bias bf16 [n]) for int8 codes q [m, k] and scales fp32 [m] of rows
+    (int8_rows, or made otherwise), sums exact (swl_int8_matmul_bf16).  q's rows must
+    be a multiple of 16 bytes apart and 16-byte aligned, with k rounded up to 16
+    bytes of storage each."""
+    if not isinstance(w, Int8Weight):
+        raise TypeError("w must be an Int8Weight")
+    dev = _device_for(q, "q", torch.int8)
+    _here(q, "q", torch.int8, dev)
+    _here(scale, "scale", torch.float32, dev)
+    _here(w.data, "w", _U8, dev)
+    if q.dim() != 2 or q.shape[1] != w.k or (w.k > 1 and q.stride(1) != 1):
+        raise ValueError("int8_matmul expects q [m, k] with unit column stride and w [n, k]")
+    m, k = q.shape
+    n = w.n
+    room = (k + 15) // 16 * 16
+    ldq = q.stride(0) if m > 1 else room
+    if m and (ldq < room or ldq % 16 or q.data_ptr() % 16 or
+              q.storage_offset() + (m - 1) * ldq + room > q.untyped_storage().nbytes()):
+        raise ValueError("rows of q must be 16-byte aligned, with k rounded up to 16 bytes of storage each")
+    if scale.shape != (m,) or not scale.is_contiguous():
+        raise ValueError("scale must be contiguous with one entry per row")
+    if bias is not None:
+        _here(bias, "bias", BF16, dev)
+        if bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError("bias must be contiguous with n elements")
+    if out is None:
+        out = scale.new_empty((m, n), dtype=BF16)
+    else:
+        _here(out, "out", BF16, dev)
+        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or out.data_ptr() % 8:
+            raise ValueError("out must be [m, n] with unit column stride, rows not overlapping, 8-byte aligned")
+    need = _int8_workspace(m, n, k)
+    ws = q.new_empty(need, dtype=_U8) if need else None
+    _lib.check(_lib.load().swl_int8_matmul_bf16(
+        q.data_ptr(), ldq, scale.data_ptr(), m, w.data.data_ptr(), w.scale.data_ptr(), n, k, _addr(bias), out.data_ptr(),
+        out.stride(0) if m > 1 else n, _addr(ws), need, _stream_of(dev)))
+    return out
+
+
 # --------------------------------------- attention over a shared prefix ---
 @functools.lru_cache(maxsize=1024)
 def _prefix_workspace(nseq: int, ntok: int, ngroups: int, hq: int, hkv: int, pre: int, keys: int, rotate: int) -> int:
