@@ -82,41 +82,51 @@ __device__ __forceinline__ u32x2 codes8(u32x4 q, const RowScale& s) {
   return u32x2{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
 }
 
-// A row of x a workgroup: its largest, then its codes; what is read stays in
-// registers where a row has at most 16384 elements.  Bytes bound it (2325 rows of
-// 4096), the launch and one trip to memory where rows are few.
-constexpr int kRowRegs = 8;  // vectors of 8 a thread
-__global__ __launch_bounds__(256) void int8_rows_kernel(const bf16* x, int64_t ldx, int64_t k, int8_t* q, int64_t ldq,
-                                                        float* scale) {
-  __shared__ uint32_t sh[4];
+// A row of x a workgroup: its largest, then its codes, the row in registers between
+// (rows over 8 NV THREADS, or not in whole 16-byte pieces, are read twice).
+template <int NV, int THREADS>
+__global__ __launch_bounds__(THREADS) void int8_rows_kernel(const bf16* x, int64_t ldx, int64_t k, int8_t* q, int64_t ldq,
+                                                            float* scale) {
+  __shared__ uint32_t sh[THREADS / 64];
   const int64_t row = blockIdx.x;
   const bf16* src = x + row * ldx;
   int8_t* dst = q + row * ldq;
-  const int64_t kp = (k + 15) / 16 * 16;  // (the bytes behind the last code are zeros)
-  u32x4 v[kRowRegs];
+  const bool held = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && k % 8 == 0 && k <= 8 * NV * THREADS;
+  u32x4 v[NV];
   uint32_t top = 0;
+  if (held) {
 #pragma unroll
-  for (int j = 0; j < kRowRegs; ++j) {
-    const int64_t i = (j * 256 + threadIdx.x) * 8;
-    v[j] = u32x4{0u, 0u, 0u, 0u};
-    if (i < k) v[j] = row8(src, i, k);
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * THREADS + threadIdx.x) * 8;
+      v[j] = u32x4{0u, 0u, 0u, 0u};
+      if (i < k) v[j] = ldg16(src + i);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) top = top8(v[j], top);
+  } else {
+#pragma unroll 1
+    for (int64_t i = threadIdx.x * 8; i < k; i += THREADS * 8) top = top8(row8(src, i, k), top);
   }
-#pragma unroll
-  for (int j = 0; j < kRowRegs; ++j) top = top8(v[j], top);
-  for (int64_t i = (kRowRegs * 256 + threadIdx.x) * 8; i < k; i += 2048) top = top8(row8(src, i, k), top);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
   __syncthreads();
-  const RowScale s = row_scale(max(max(sh[0], sh[1]), max(sh[2], sh[3])));
-  if (threadIdx.x == 0) scale[row] = s.scale;
 #pragma unroll
-  for (int j = 0; j < kRowRegs; ++j) {
-    const int64_t i = (j * 256 + threadIdx.x) * 8;
-    if (i < kp) *reinterpret_cast<u32x2*>(dst + i) = codes8(v[j], s);
+  for (int i = 0; i < THREADS / 64; ++i) top = max(top, sh[i]);
+  const RowScale s = row_scale(top);
+  if (threadIdx.x == 0) scale[row] = s.scale;
+  const int64_t kp = (k + 15) / 16 * 16;  // (the bytes behind the last code are zeros)
+  if (held) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * THREADS + threadIdx.x) * 8;
+      if (i < kp) *(__attribute__((address_space(1))) u32x2*)(dst + i) = codes8(v[j], s);
+    }
+  } else {
+#pragma unroll 1
+    for (int64_t i = threadIdx.x * 8; i < kp; i += THREADS * 8)
+      *(__attribute__((address_space(1))) u32x2*)(dst + i) = codes8(row8(src, i, k), s);
   }
-  for (int64_t i = (kRowRegs * 256 + threadIdx.x) * 8; i < kp; i += 2048)
-    *reinterpret_cast<u32x2*>(dst + i) = codes8(row8(src, i, k), s);
 }
 
 // A tile of 16 rows of a weight a workgroup of 16 waves: each wave its row's
@@ -193,9 +203,8 @@ __device__ __forceinline__ void store4(const Int8Args& a, const float (&o)[4], i
 // wave w takes the steps of 128 k w, w + W, ... of all of them, the weight straight
 // into registers past the caches, the rows from L2, and the waves' sums meet in
 // LDS: no partial sums in memory, one launch.
-template <int MT, int TPW, int W>
+template <int MT, int TPW, int W, int D>
 __global__ __launch_bounds__(64 * W) void int8_rows_product_kernel(Int8Args a) {
-  constexpr int D = MT <= 2 ? 4 : 2;  // steps in flight
   __shared__ __attribute__((aligned(16))) i32x4 sh[W][TPW * MT * 64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = blockIdx.x * TPW;
@@ -499,7 +508,18 @@ __global__ __launch_bounds__(256) void int8_fold_kernel(Int8Args a) {
 }
 
 // ---------------------------------------------------------------- launchers ---
-constexpr int kFewRows = 128;  // rows of int8_rows_product_kernel at most
+// Which kernel takes a call (times of MI355X, the weight from memory, n x k by m):
+//   at most 64 rows stream the weight, every workgroup reading all of x from L2; how
+//   many tiles share that is the question: 28672 x 4096 by 28 rows 1 tile 41 us, 2
+//   31, 4 22 (6.3 TB/s at 128256 x 4096), 8 26; by one row 21; but 6144 x 4096 by 28
+//   rows, 2 tiles and 16 waves 8.5, 8 waves 9.1, 4 tiles 12.7, by one row 1 tile 6.1, 2
+//   7.6.  More steps in flight a wave are slower (28672 by 28: one step 22, two 26,
+//   three 27; the registers' cost in waves).
+//   More rows, and 17 to 64 of a long k with few channels, take tiles of 128 x 128
+//   with k split so that there are as many as CUs: 4096 x 14336 by 28 rows streamed
+//   20.3, 8 splits 18.8; by 60 34 and 19.6 (16 splits 25.9); by 107 57 and 22.9; 28672
+//   x 4096 by 60 27.6 and 26.5, 6144 x 4096 by 40 10.0 and 12.1.
+constexpr int kFewRows = 64;
 
 struct Int8Plan {
   bool few, big;
@@ -509,13 +529,13 @@ struct Int8Plan {
 Int8Plan int8_plan(int64_t m, int64_t n, int64_t k) {
   Int8Plan p{};
   p.splits = 1;
-  p.few = m <= kFewRows;
+  p.few = m <= kFewRows && (m <= 16 || k < 8192 || n > 8192);
   if (p.few) return p;
   const int64_t steps = (k + kStep - 1) / kStep;
   p.big = ((m + 255) / 256) * ((n + 255) / 256) >= 160;
   if (!p.big) {
     const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
-    p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)2 * kCus / tiles, steps / 8, (int64_t)16}));
+    p.splits = (int)std::max<int64_t>(1, std::min({(int64_t)kCus / tiles, steps / 6, (int64_t)16}));
   }
   p.bytes = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
   return p;
@@ -534,7 +554,7 @@ int launch_tiles(const Int8Args& a, hipStream_t st) {
     while ((gm + 1) * (gm + 1) <= per_xcd) ++gm;
     gm = std::min(gm, tiles_m);
   }
-  auto kern = int8_tile_kernel<NI, NJ, WM, SLOTS>;
+  auto kern = int8_tile_kernel<NI, NJ, WM, SLOTS>;  // (over the default 64 KiB of LDS: allowed a kernel)
   SWL_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, Geo::LDS));
   hipLaunchKernelGGL(kern, dim3((unsigned)(per_xcd * 8), (unsigned)a.splits), dim3(128 * WM), Geo::LDS, st, a, tiles_m, tiles,
                      per_xcd, gm);
@@ -544,10 +564,15 @@ int launch_tiles(const Int8Args& a, hipStream_t st) {
 
 template <int MT>
 int launch_rows(const Int8Args& a, hipStream_t st) {
-  if (MT <= 4 && a.tiles >= 4 * kCus)
-    hipLaunchKernelGGL((int8_rows_product_kernel<MT, (MT <= 4 ? 2 : 1), 8>), dim3((unsigned)((a.tiles + 1) / 2)), dim3(512), 0, st, a);
+  auto go = [&](auto kern, int tpw, int waves) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)((a.tiles + tpw - 1) / tpw)), dim3(64 * waves), 0, st, a);
+  };
+  if (a.tiles >= 768)
+    go(int8_rows_product_kernel<MT, 4, 4, 1>, 4, 4);
+  else if (MT > 1 && a.tiles >= 192)
+    go(int8_rows_product_kernel<MT, 2, 8, 1>, 2, 8);
   else
-    hipLaunchKernelGGL((int8_rows_product_kernel<MT, 1, 8>), dim3((unsigned)a.tiles), dim3(512), 0, st, a);
+    go(int8_rows_product_kernel<MT, 1, 8, 1>, 1, 8);
   SWL_LAUNCH_CHECK("int8_rows_product_kernel launch");
   return SWL_OK;
 }
@@ -564,8 +589,15 @@ extern "C" int swl_int8_rows_bf16(const void* x, int64_t ldx, int64_t m, int64_t
   SWL_CHECK(x && q && scale, SWL_ERR_INVALID, "swl_int8_rows_bf16: null argument");
   SWL_CHECK(ldx >= k && ldq >= (k + 15) / 16 * 16, SWL_ERR_INVALID, "swl_int8_rows_bf16: row strides smaller than a row");
   SWL_CHECK(aligned(q, 16) && ldq % 16 == 0, SWL_ERR_INVALID, "swl_int8_rows_bf16: rows of q must be 16-byte aligned");
-  hipLaunchKernelGGL(int8_rows_kernel, dim3((unsigned)m), dim3(256), 0, (hipStream_t)stream,
-                     reinterpret_cast<const bf16*>(x), ldx, k, reinterpret_cast<int8_t*>(q), ldq, scale);
+  // (threads with two vectors of 8 each up to 8192; 107 rows of 14336 7.5 us with 256 threads)
+  auto rows = [&](auto kern, int threads) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)m), dim3(threads), 0, (hipStream_t)stream, reinterpret_cast<const bf16*>(x), ldx,
+                       k, reinterpret_cast<int8_t*>(q), ldq, scale);
+  };
+  if (k <= 4096)
+    rows(int8_rows_kernel<2, 256>, 256);
+  else
+    rows(int8_rows_kernel<4, 512>, 512);
   SWL_LAUNCH_CHECK("int8_rows_kernel launch");
   return SWL_OK;
 }
@@ -625,8 +657,7 @@ extern "C" int swl_int8_matmul_bf16(const void* q, int64_t ldq, const float* q_s
   if (p.few) {
     if (m <= 16) return launch_rows<1>(a, st);
     if (m <= 32) return launch_rows<2>(a, st);
-    if (m <= 64) return launch_rows<4>(a, st);
-    return launch_rows<8>(a, st);
+    return launch_rows<4>(a, st);
   }
   if (p.big) return launch_tiles<4, 4, 2, 2>(a, st);
   if (int rc = launch_tiles<2, 2, 2, 4>(a, st)) return rc;
