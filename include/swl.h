@@ -530,7 +530,7 @@ int swl_verify_drafts_bf16(const void* target, int64_t ld_target, const void* dr
  * row's sum is of them as rounded).  A query that sees no token gets zeros.
  * Infinities and NaN reach the queries that see their token, nobody else.  Values
  * must leave room for their sum (under 2^118 / tokens).
- * nseq + ngroups at most 4096, ntok under 2^25.  workspace:
+ * nseq + ngroups at most 1024, ntok under 2^25.  workspace:
  * swl_prefix_attention_workspace(nseq, ntok, ngroups, hq, hkv, max_prefix_blocks *
  * block_size, max_blocks * block_size, positions != NULL) bytes of device memory,
  * 16-byte aligned, owned by the call until its kernels have run; its contents do

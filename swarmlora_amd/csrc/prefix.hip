@@ -33,11 +33,14 @@ constexpr int kD = 128;         // head dim
 constexpr int kRows = 128;      // rows of a block
 constexpr int kKeys = 64;       // keys of a step
 constexpr int kFew = 32;        // rows of a block whose keys its waves share out, 16 each of a step
-constexpr int kMaxEntries = 4096;
+constexpr int kMaxEntries = 1024;
 constexpr int kCus = 256;       // of an MI355X
 constexpr int kPerCu = 2;       // workgroups of a CU (LDS, registers)
 constexpr int kSlots = kCus * kPerCu;
-constexpr int kMinSteps = 4;    // steps of a part at least
+constexpr int kMinSteps = 4;    // steps of a part at least (blocks of many rows: half of it)
+constexpr int kLong = 32;       // steps of a part that is cut once more,
+constexpr int kCuts = 3;        // into so many
+constexpr int kKinds = 8;
 
 // Division by a number that the host knows, for dividends under 2^31.
 struct FastDiv {
@@ -59,17 +62,19 @@ __device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv& f) {
 // What a workgroup of the attention needs to know of its part.
 struct Part {
   int32_t tok0;     // first token, or its place in the list of tokens
-  int32_t listed;   // tokens are in the list
   int32_t n;        // tokens
   int32_t r0;       // first row of the block
   int32_t st0, nst; // steps: the prefix's, then the own tokens'
   int32_t pre;      // steps of the prefix
   int32_t seq, group;
   int32_t len, plen;  // own tokens before the new ones, tokens of the prefix
-  int32_t direct;   // the part is all there is of its rows
+  int32_t flags;    // kListed, kDirect
+  int32_t pad;
   int64_t rec;      // record of row 0 of the block's tokens, kv head 0
   int64_t head;     // records between kv heads
 };
+constexpr int kListed = 1;  // tokens are in the list
+constexpr int kDirect = 2;  // the part is all there is of its rows
 static_assert(sizeof(Part) == 64, "one load of 16 dwords");
 
 // Where the records of a sequence's rows are: parts of its own tokens, and of the
@@ -115,6 +120,7 @@ struct PrefixArgs {
   float* rec_ml;        // [max_rec][2]
   int64_t max_rec;
   int32_t max_parts;
+  int32_t slots, min_steps;  // parts that run at once, steps of a part at least
   int32_t rows_wg;      // rows of a workgroup of the merge
 };
 
@@ -124,37 +130,34 @@ __device__ __forceinline__ void tokens_of(const PrefixArgs& a, int s, int& t0, i
   n = a.cu ? a.cu[s + 1] - t0 : a.L;
   if (t0 < 0 || n < 0 || (int64_t)t0 + n > a.T) t0 = n = 0;
 }
-// Group of sequence s, -1: none.
-__device__ __forceinline__ int group_of(const PrefixArgs& a, int s) {
-  if (!a.cg) return a.ngroups - 1;  // (one group, or none)
-  int lo = 0, hi = a.ngroups;  // the last g with cg[g] <= s
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cg[mid] <= s)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return a.cg[lo] <= s && s < a.cg[lo + 1] ? lo : -1;
-}
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kKeys - 1) / kKeys; }
 
+// A lane's value from a lane below it (DPP; 0 where there is none).
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T below(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+  } else {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)v >> 32), CTRL, ROWS, 0xF, false);
+    return (T)((uint64_t)hi << 32 | lo);
+  }
+}
+// Sums over the lanes up to each: in rows of 16, then across them.
 template <typename T>
-__device__ __forceinline__ T wave_add(T v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ T wave_prefix(T v) {
+  v += below<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += below<0x112, 0xF>(v);
+  v += below<0x114, 0xF>(v);
+  v += below<0x118, 0xF>(v);
+  v += below<0x142, 0xA>(v);  // row_bcast 15, 31
+  return v + below<0x143, 0xC>(v);
 }
 // Exclusive prefix over the 256 threads; `all` the sum.
 template <typename T>
 __device__ __forceinline__ T block_prefix(T v, T* sh, T& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  T inc = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += y;
-  }
+  const T inc = wave_prefix(v);
   __syncthreads();
   if (lane == 63) sh[w] = inc;
   __syncthreads();
@@ -169,15 +172,19 @@ struct PlanLds {  // of E = ngroups + nseq entries: the groups' prefixes, then t
   int32_t* rows;  // [E]
   int32_t* steps; // [E]
   int32_t* pre;   // [E] of them, the prefix's
-  int32_t* few;   // [nseq + 1] tokens before it that share their prefix
   int32_t* first; // [E] first part
+  int32_t* len;   // [E] tokens of the prefix; own tokens before the new ones
+  int32_t* few;   // [nseq + 1] tokens before it that share their prefix
+  int32_t* t0;    // [nseq] first token
+  int32_t* cg;    // [ngroups + 1] first sequence, in range
 };
-constexpr int kPlanEntry = 8 + 5 * 4;
+constexpr int kPlanEntry = 8 + 8 * 4;
 
 __device__ void make_plan(const PrefixArgs& a, char* lds) {
   __shared__ int64_t sh64[4];
   __shared__ int32_t sh32[4];
-  __shared__ float shf[4][2];
+  __shared__ float shf[4];
+  __shared__ int32_t kind[kKinds], at_kind[kKinds];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int ng = a.ngroups, ns = a.nseq, E = ng + ns;
   PlanLds l;
@@ -186,23 +193,45 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
   l.steps = l.rows + E;
   l.pre = l.steps + E;
   l.first = l.pre + E;
-  l.few = l.first + E;
+  l.len = l.first + E;
+  l.few = l.len + E;
+  l.t0 = l.few + ns + 1;
+  l.cg = l.t0 + ns;
 
-  // sequences: rows, steps, and the tokens that walk their prefix in company
+  for (int g = tid; g <= ng; g += 256) {
+    l.cg[g] = a.cg ? min(max(a.cg[g], 0), ns) : g > 0 ? ns : 0;
+    if (g < ng) l.len[g] = min(max(a.plens[g], 0), a.pmax);
+  }
+  for (int s = tid; s < ns; s += 256) {
+    int t0, n;
+    tokens_of(a, s, t0, n);
+    l.t0[s] = t0;
+    l.rows[ng + s] = n * a.G;
+    l.len[ng + s] = min(a.lens[s], 1 << 30);
+  }
+  __syncthreads();
+  auto group_of = [&](int s) {  // -1: none
+    int lo = 0, hi = ng;        // the last g with cg[g] <= s
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (l.cg[mid] <= s)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return ng > 0 && l.cg[lo] <= s && s < l.cg[lo + 1] ? lo : -1;
+  };
+  // sequences: steps, and the tokens that walk their prefix in company
   int run = 0;
   for (int s0 = 0; s0 < ns; s0 += 256) {
     const int s = s0 + tid;
     int share = 0;
     if (s < ns) {
-      int t0, n;
-      tokens_of(a, s, t0, n);
-      const int len = min(a.lens[s], 1 << 30), g = group_of(a, s);
-      const int plen = g >= 0 ? min(max(a.plens[g], 0), a.pmax) : 0;
-      const bool alone = n * a.G >= kRows;
-      const int own = steps_of((int)min<int64_t>(max<int64_t>((int64_t)len + n, 0), a.kmax));
+      const int g = group_of(s), plen = g >= 0 ? l.len[g] : 0, rows = l.rows[ng + s], n = (uint32_t)rows / a.by_g;
+      const bool alone = rows >= kRows;
+      const int own = steps_of((int)min<int64_t>(max<int64_t>((int64_t)l.len[ng + s] + n, 0), a.kmax));
       const int pre = alone ? steps_of(plen) : 0;
       share = plen > 0 && !alone ? n : 0;
-      l.rows[ng + s] = n * a.G;
       l.pre[ng + s] = pre;
       l.steps[ng + s] = max(own + pre, 1);
     }
@@ -214,52 +243,31 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
   if (tid == 0) l.few[ns] = run;
   __syncthreads();
   for (int g = tid; g < ng; g += 256) {
-    const int s0 = a.cg ? min(max(a.cg[g], 0), ns) : 0, s1 = a.cg ? min(max(a.cg[g + 1], s0), ns) : ns;
-    const int n = l.few[s1] - l.few[s0], st = n > 0 ? steps_of(min(max(a.plens[g], 0), a.pmax)) : 0;
+    const int s0 = l.cg[g], s1 = max(l.cg[g + 1], s0);
+    const int n = l.few[s1] - l.few[s0], st = n > 0 ? steps_of(l.len[g]) : 0;
     l.rows[g] = st > 0 ? n * a.G : 0;
     l.steps[g] = l.pre[g] = max(st, 1);
   }
   __syncthreads();
 
-  // Steps of a part: the fewest of eight candidates that let all parts run at
-  // once, at least kMinSteps, and at least all steps / kSlots, so that there are
-  // at most kSlots full parts whatever the lengths are.
-  float sum = 0.f, blocks = 0.f;
+  // Steps of a part: as many as give every place its share of all the work, at
+  // least min_steps; a step of a block of many rows counts twice.  Long shares are
+  // cut into kCuts, as the places do not end together and a step costs much more
+  // than what a part adds.  So there are at most slots, or kCuts * slots, full
+  // parts, whatever the lengths are.
+  float sum = 0.f;
   for (int e = tid; e < E; e += 256) {
-    const float rb = (float)((l.rows[e] + kRows - 1) / kRows);
-    sum += rb * (float)l.steps[e];
-    blocks += rb;
+    const int rows = l.rows[e];
+    sum += (float)((rows + kRows - 1) / kRows) * (float)l.steps[e] * (rows > kFew ? 2.f : 1.f);
   }
-  sum = wave_add(sum);
-  blocks = wave_add(blocks);
-  if (lane == 0) {
-    shf[w][0] = sum;
-    shf[w][1] = blocks;
-  }
+  sum = wave_prefix(sum);
+  if (lane == 63) shf[w] = sum;
   __syncthreads();
   // (rounded up past what the sums' roundings may have lost)
-  sum = ((shf[0][0] + shf[1][0]) + (shf[2][0] + shf[3][0])) * 1.0001f * (float)a.hkv;
-  blocks = ((shf[0][1] + shf[1][1]) + (shf[2][1] + shf[3][1])) * (float)a.hkv;
-  const float slots = (float)kSlots;
-  const int lo = max(kMinSteps, (int)fminf(sum / slots + 1.f, 1073741824.f));
-  const int hi = blocks >= slots ? lo : max(lo, (int)fminf(sum / (slots - blocks) + 1.f, 1073741824.f));
-  int spp = hi;
-  if (hi > lo) {
-    float units[2] = {0.f, 0.f};
-    int cand[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      cand[c] = lo + (int)((float)(hi - lo) * (float)(2 * w + c) * 0.125f);
-      for (int e = lane; e < E; e += 64)
-        units[c] += (float)((l.rows[e] + kRows - 1) / kRows) * (float)((l.steps[e] + cand[c] - 1) / cand[c]);
-      units[c] = wave_add(units[c]) * (float)a.hkv;
-    }
-    const int ok = units[0] <= slots ? cand[0] : units[1] <= slots ? cand[1] : hi;
-    __syncthreads();
-    if (lane == 0) sh32[w] = ok;
-    __syncthreads();
-    spp = min(min(sh32[0], sh32[1]), min(sh32[2], sh32[3]));
-  }
+  sum = ((shf[0] + shf[1]) + (shf[2] + shf[3])) * 1.0001f * (float)a.hkv;
+  const int whole = (int)fminf(sum / (float)a.slots + 1.f, 1073741824.f);
+  const int share = max(a.min_steps, max((whole + kCuts - 1) / kCuts, min(whole, kLong)));
+  auto steps_per_part = [&](int e) { return l.rows[e] > kFew ? (share + 1) >> 1 : share; };
 
   // first parts and records
   int parts_run = 0;
@@ -269,7 +277,7 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
     int units = 0;
     int64_t recs = 0;
     if (e < E) {
-      const int rows = l.rows[e], parts = (l.steps[e] + spp - 1) / spp;
+      const int rows = l.rows[e], spp = steps_per_part(e), parts = (l.steps[e] + spp - 1) / spp;
       units = (rows + kRows - 1) / kRows * parts;
       const bool joined = e < ng || l.few[e - ng + 1] > l.few[e - ng];
       recs = joined || parts > 1 ? (int64_t)rows * parts * a.hkv : 0;
@@ -288,33 +296,36 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
   __syncthreads();
   const int total = min(parts_run, a.max_parts);
   if (tid == 0) a.n_parts[0] = total;
+  if (tid < kKinds) kind[tid] = 0;
   for (int s = tid; s < ns; s += 256) {
     const int e = ng + s;
-    int t0, n;
-    tokens_of(a, s, t0, n);
     SeqRec r{};
-    r.t0 = t0;
-    r.n = n;
+    r.t0 = l.t0[s];
+    r.n = (uint32_t)l.rows[e] / a.by_g;
     if (l.rec[e] >= 0) {
       r.own = l.rec[e];
       r.own_rows = l.rows[e];
+      const int spp = steps_per_part(e);
       r.own_parts = (l.steps[e] + spp - 1) / spp;
       r.own_head = (int64_t)r.own_rows * r.own_parts;
     }
     if (l.few[s + 1] > l.few[s]) {
-      const int g = group_of(a, s), first = a.cg ? max(a.cg[g], 0) : 0;
+      const int g = group_of(s), spp = steps_per_part(g);
       r.pre_rows = l.rows[g];
       r.pre_parts = (l.steps[g] + spp - 1) / spp;
       r.pre_head = (int64_t)r.pre_rows * r.pre_parts;
-      r.pre = l.rec[g] + (int64_t)(l.few[s] - l.few[first]) * a.G;
-      for (int i = 0; i < n && l.few[s] + i < a.T; ++i) a.list[l.few[s] + i] = t0 + i;
+      r.pre = l.rec[g] + (int64_t)(l.few[s] - l.few[l.cg[g]]) * a.G;
+      for (int i = 0; i < r.n && l.few[s] + i < a.T; ++i) a.list[l.few[s] + i] = r.t0 + i;
     }
     // (what lies outside the workspace, by offsets that are none, is left out)
     const int64_t own_end = r.own + r.own_head * a.hkv, pre_end = r.pre + r.pre_head * a.hkv;
     if (r.own < 0 || own_end > a.max_rec || r.pre < 0 || pre_end > a.max_rec) r.own_parts = r.pre_parts = 0;
     a.seq[s] = r;
   }
-  for (int u = tid; u < total; u += 256) {
+  __syncthreads();
+  // The parts, the ones with the most work first: counted by kind (eighths of the
+  // largest), then put where their kind begins.
+  auto part_of = [&](int u, Part& o) {
     int lo_e = 0, hi_e = E;  // the last entry with parts whose first is <= u
     while (hi_e - lo_e > 1) {
       const int mid = (lo_e + hi_e) >> 1;
@@ -323,35 +334,26 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
       else
         hi_e = mid;
     }
-    const int e = lo_e, parts = (l.steps[e] + spp - 1) / spp, rows = l.rows[e];
-    const int local = u - l.first[e], rb = (rows + kRows - 1) / kRows;
-    const int b = rb - 1 - local / parts, p = local - (local / parts) * parts;  // the blocks with the most keys first
-    Part o{};
-    if (local < 0 || b < 0) {  // (counts past 32 bits, by offsets that are none)
-      a.part[u] = o;
-      continue;
-    }
-    o.listed = e < ng;
+    const int e = lo_e, spp = steps_per_part(e), parts = (l.steps[e] + spp - 1) / spp, rows = l.rows[e];
+    const int local = u - l.first[e], b = local / parts, p = local - b * parts;
+    o = Part{};
+    if (local < 0 || (int64_t)b * kRows >= rows) return;  // (counts past 32 bits, by offsets that are none)
     o.r0 = b * kRows;
     o.n = (uint32_t)rows / a.by_g;
     o.st0 = p * spp;
     o.pre = l.pre[e];
     if (e < ng) {
-      const int first = a.cg ? min(max(a.cg[e], 0), ns) : 0;
-      o.tok0 = l.few[first];
+      o.tok0 = l.few[l.cg[e]];
       o.group = e;
-      o.plen = min(max(a.plens[e], 0), a.pmax);
+      o.plen = l.len[e];
       o.nst = min(spp, l.steps[e] - o.st0);
     } else {
-      const int s = e - ng;
-      int t0, n;
-      tokens_of(a, s, t0, n);
-      o.tok0 = t0;
-      o.seq = s;
-      o.len = min(a.lens[s], 1 << 30);
+      o.seq = e - ng;
+      o.tok0 = l.t0[o.seq];
+      o.len = l.len[e];
       if (o.pre > 0) {
-        o.group = group_of(a, s);
-        o.plen = min(max(a.plens[o.group], 0), a.pmax);
+        o.group = group_of(o.seq);
+        o.plen = l.len[o.group];
       }
       // the block's own end: its last row may see fewer keys than the sequence's
       const int last = (uint32_t)(min(o.r0 + kRows, rows) - 1) / a.by_g;
@@ -359,10 +361,29 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
       o.nst = min(spp, o.pre + steps_of(kend) - o.st0);
     }
     o.nst = max(o.nst, 0);
-    o.direct = l.rec[e] < 0;
+    o.flags = (e < ng ? kListed : 0) | (l.rec[e] < 0 ? kDirect : 0);
     o.rec = l.rec[e] + (int64_t)p * rows;
     o.head = (int64_t)rows * parts;
-    a.part[u] = o;
+  };
+  auto kind_of = [&](const Part& o) {
+    const int work = o.n * a.G > kFew ? 2 * o.nst : o.nst;
+    return kKinds - 1 - (int)min<int64_t>((int64_t)work * kKinds / (share + 2), kKinds - 1);
+  };
+  Part o;
+  for (int u = tid; u < total; u += 256) {
+    part_of(u, o);
+    atomicAdd(&kind[kind_of(o)], 1);
+  }
+  __syncthreads();
+  if (tid < kKinds) {
+    int before = 0;
+    for (int i = 0; i < tid; ++i) before += kind[i];
+    at_kind[tid] = before;
+  }
+  __syncthreads();
+  for (int u = tid; u < total; u += 256) {
+    if (total > 256) part_of(u, o);
+    a.part[atomicAdd(&at_kind[kind_of(o)], 1)] = o;
   }
 }
 
@@ -464,7 +485,7 @@ __device__ __forceinline__ f32x4 mfma16k16(u32x2 a, u32x2 b, f32x4 c) {
 }
 
 __device__ __forceinline__ int token_at(const PrefixArgs& a, const Part& u, int i) {
-  return u.listed ? a.list[u.tok0 + i] : u.tok0 + i;
+  return u.flags & kListed ? a.list[u.tok0 + i] : u.tok0 + i;
 }
 
 // Where a block of keys is: the prefix's pages or the sequence's.
@@ -530,30 +551,30 @@ __device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, in
   }
 }
 
-// A row's result: to the output where the part is all there is of it, else its
-// record.  The lane has dims d .. + 8 K - 1 in o.
+// K dims from d of a row's result: to the output where the part is all there is of
+// it, else to its record.
 template <int K>
 __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int h, int r, int d, float m, float L,
-                                        const float* o, bool first) {
-  if (u.direct) {
+                                        const float (&o)[K]) {
+  if (u.flags & kDirect) {
     const int i = (uint32_t)r / a.by_g;
     bf16* dst = a.out + ((int64_t)token_at(a, u, i) * a.hq + h * a.G + r - i * a.G) * kD + d;
     const float inv = L == 0.f ? 0.f : 1.f / L;  // (0: the row sees no key)
+    bf16x2 y[K / 2];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      bf16x8 y;
+    for (int e = 0; e < K / 2; ++e)
+      y[e] = L == 0.f ? bf16x2{f2bf(0.f), f2bf(0.f)} : bf16x2{f2bf(o[2 * e] * inv), f2bf(o[2 * e + 1] * inv)};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = f2bf(L == 0.f ? 0.f : o[8 * k + e] * inv);
-      *(__attribute__((address_space(1))) u32x4*)(dst + 8 * k) = __builtin_bit_cast(u32x4, y);
-    }
+    for (int e = 0; e < K / 4; ++e)
+      stg(dst + 4 * e, u32x2{__builtin_bit_cast(uint32_t, y[2 * e]), __builtin_bit_cast(uint32_t, y[2 * e + 1])});
   } else {
     const int64_t at = u.rec + h * u.head + r;
     if (at < 0 || at >= a.max_rec) return;  // (only where offsets are none)
     float* dst = a.rec_o + at * kD + d;
 #pragma unroll
-    for (int k = 0; k < 2 * K; ++k)
-      *(__attribute__((address_space(1))) f32x4*)(dst + 4 * k) = f32x4{o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]};
-    if (first) {
+    for (int e = 0; e < K; e += 4)
+      *(__attribute__((address_space(1))) f32x4*)(dst + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+    if (d == 0) {
       a.rec_ml[2 * at] = m;
       a.rec_ml[2 * at + 1] = L;
     }
@@ -767,58 +788,60 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
     }
   }
 
-  // the lane's dims 32 g + 4 (d ^ g % 2) .. + 3 in order
-  auto ordered = [&](int e, float (&o)[32]) {
+  // Rows in order by way of LDS: 128 dims (the lane has 32 g + 4 (d ^ g % 2) .. + 3
+  // in acc[d]), maximum, sum.
+  constexpr int F = 132;
+  float* mg = reinterpret_cast<float*>(sh.kv);
+  static_assert(4 * 16 * F * 4 <= (int)sizeof(sh.kv), "the waves' rows");
+  auto leave = [&](int e) {
+    l[e] = sum_groups(l[e]);
+    float* dst = mg + (w * 16 + col) * F;
 #pragma unroll
-    for (int d = 0; d < 8; d += 2)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[4 * d + i] = (g & 1) ? acc[e][d + 1][i] : acc[e][d][i];
-        o[4 * d + 4 + i] = (g & 1) ? acc[e][d][i] : acc[e][d + 1][i];
-      }
+    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(dst + 32 * g + 4 * (d ^ (g & 1))) = acc[e][d];
+    if (g == 0) {
+      dst[128] = m[e];
+      dst[129] = l[e];
+    }
   };
-  if constexpr (MANY) {
+  auto again = [&](int r) {
+    float mx, sm, y[8];
+    slow_row(a, u, h, kend, r, lane, mx, sm, y);
+    if (lane < 16) put_row<8>(a, u, h, r, 8 * lane, mx, sm, y);
+  };
+  if constexpr (MANY) {  // every wave its own, 32 lanes a row
     if (idle) return;
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
-      const int r = wr0 + e * 16 + col;
-      l[e] = sum_groups(l[e]);
-      float o[32];
-      ordered(e, o);
+      const int r0 = wr0 + 16 * e;
       bool bad = not_finite(l[e]);
 #pragma unroll
-      for (int d = 0; d < 32; ++d) bad |= not_finite(o[d]);
-      uint64_t redo = __ballot(bad && r < rows);
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= not_finite(acc[e][d][i]);
+      uint64_t redo = __ballot(bad && r0 + col < rows);
       redo = (redo | redo >> 16 | redo >> 32 | redo >> 48) & 0xffffu;
-      if (r < rows && !(redo >> col & 1)) put_row<4>(a, u, h, r, 32 * g, m[e], l[e], o, g == 0);
-      while (redo) {
-        const int c = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        float mx, sm, x[8];
-        slow_row(a, u, h, kend, wr0 + e * 16 + c, lane, mx, sm, x);
-        if (lane < 16) put_row<1>(a, u, h, wr0 + e * 16 + c, 8 * lane, mx, sm, x, lane == 0);
+      leave(e);
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      asm volatile("" ::: "memory");
+      const int d = 4 * (lane & 31);
+#pragma unroll 4
+      for (int i = lane >> 5; i < 16; i += 2) {
+        const float* src = mg + (w * 16 + i) * F;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + d);
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        if (r0 + i < rows && !(redo >> i & 1)) put_row<4>(a, u, h, r0 + i, d, src[128], src[129], o);
       }
+      for (; redo; redo &= redo - 1) again(r0 + __builtin_ctzll(redo));
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      asm volatile("" ::: "memory");
     }
-  } else {
-    // the waves' results in LDS, rows that there are
-    constexpr int F = 132;  // floats of a row: 128 dims, maximum, sum
-    float* mg = reinterpret_cast<float*>(sh.kv);
-    static_assert(4 * 16 * F * 4 <= (int)sizeof(sh.kv), "merge area");
+  } else {  // the waves' shares of a row merged
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
       const int nr = min(rows - u.r0 - 16 * e, 16);
       if (nr <= 0) return;  // the same for the whole workgroup
       __syncthreads();
-      l[e] = sum_groups(l[e]);
-      if (col < nr) {
-        float* dst = mg + (w * 16 + col) * F;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(dst + 32 * g + 4 * (d ^ (g & 1))) = acc[e][d];
-        if (g == 0) {
-          dst[128] = m[e];
-          dst[129] = l[e];
-        }
-      }
+      leave(e);
       __syncthreads();
       const int row = threadIdx.x >> 4, x8 = 8 * (threadIdx.x & 15);
       float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -839,14 +862,9 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         for (int d = 0; d < 8; ++d) bad |= not_finite(o[d]);
       }
       const uint64_t redo = __ballot(bad);
-      if (row < nr && (redo >> (lane & 48) & 0xffffu) == 0) put_row<1>(a, u, h, u.r0 + 16 * e + row, x8, M, L, o, x8 == 0);
-      for (int i = 0; i < 4; ++i) {  // the wave's four rows
-        if ((redo >> (16 * i) & 0xffffu) == 0) continue;
-        float mx, sm, y[8];
-        const int r = u.r0 + 16 * e + 4 * w + i;
-        slow_row(a, u, h, kend, r, lane, mx, sm, y);
-        if (lane < 16) put_row<1>(a, u, h, r, 8 * lane, mx, sm, y, lane == 0);
-      }
+      if (row < nr && (redo >> (lane & 48) & 0xffffu) == 0) put_row<8>(a, u, h, u.r0 + 16 * e + row, x8, M, L, o);
+      for (int i = 0; i < 4; ++i)  // the wave's four rows
+        if (redo >> (16 * i) & 0xffffu) again(u.r0 + 16 * e + 4 * w + i);
     }
   }
 }
@@ -883,7 +901,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
     float M = -INFINITY, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     auto take = [&](int64_t rec, int64_t step, int parts) {
-      constexpr int B = 4;  // records in flight together
+      constexpr int B = 8;  // records in flight together
       for (int p0 = 0; p0 < parts; p0 += B) {
         float pm[B], pl[B];
         f32x4 po[B];
@@ -929,11 +947,13 @@ PrefixLayout prefix_layout(int64_t nseq, int64_t T, int64_t ngroups, int hq, int
   const int64_t G = hq / hkv;
   const int64_t blocks = nseq + ngroups + T * G / kRows;
   const int64_t steps = (pmax + kKeys - 1) / kKeys + (kmax + kKeys - 1) / kKeys;
-  const int64_t most = std::max<int64_t>(1, (steps + kMinSteps - 1) / kMinSteps);
-  l.parts = std::min<int64_t>(blocks * most, blocks + (kSlots + hkv - 1) / hkv);
+  const int64_t most = std::max<int64_t>(1, (steps + kMinSteps / 2 - 1) / (kMinSteps / 2));
+  // (full parts: kCuts * kSlots only where the work is enough for long ones)
+  const int64_t full = 4 * blocks * hkv * steps > (int64_t)kLong * kSlots ? kCuts * kSlots : kSlots;
+  l.parts = std::min<int64_t>(blocks * most, blocks + (full + hkv - 1) / hkv);
   // rows that share their prefix, twice, and those of blocks that are cut
   const int64_t few = std::min<int64_t>(T, nseq * ((kRows - 1) / G));
-  const int64_t cut = most > 1 ? std::min<int64_t>(2 * kSlots, blocks * most * hkv) * kRows : 0;
+  const int64_t cut = most > 1 ? std::min<int64_t>(2 * full, blocks * most * hkv) * kRows : 0;
   l.recs = 2 * few * hq + cut;
   auto place = [&](int64_t bytes) {
     const int64_t at = l.bytes;
@@ -988,7 +1008,7 @@ extern "C" int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const 
   if (ngroups == 0 && cu_groups) return bad("cu_groups without a group");
   if (ngroups > 0 && (!prefix_table || !prefix_lens || max_prefix_blocks < 1)) return bad("null argument");
   if (!cu_groups && ngroups > 1) return bad("more than one group needs cu_groups");
-  if (nseq + ngroups > kMaxEntries) return bad("at most 4096 sequences and groups");
+  if (nseq + ngroups > kMaxEntries) return bad("at most 1024 sequences and groups");
   if (!cu_seqlens && ntok % nseq) return bad("without cu_seqlens every sequence has as many tokens");
   if (ntok * (int64_t)(hq / hkv) >= ((int64_t)1 << 31)) return bad("too many rows");
   if (q == out) return bad("out must not be q");
@@ -1051,6 +1071,8 @@ extern "C" int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const 
   a.rec_ml = reinterpret_cast<float*>(ws + l.rec_ml);
   a.max_rec = l.recs;
   a.max_parts = (int32_t)l.parts;
+  a.slots = kSlots;
+  a.min_steps = kMinSteps;
   const hipStream_t st = (hipStream_t)stream;
   const int heads = (positions ? hq : 0) + (k ? 2 * hkv : 0), heads_wg = (heads + 31) / 32;
   const int64_t start = 1 + ntok * heads_wg;

@@ -30,7 +30,7 @@ def _call(lib, **kw):
     (dict(maxp=0), "go together"), (dict(k=None), "go together"), (dict(q=None), "null"), (dict(out=None), "null"),
     (dict(kc=None), "null"), (dict(bt=None), "null"), (dict(lens=None), "null"), (dict(pt=None), "null"), (dict(pl=None), "null"),
     (dict(mp=0), "null"), (dict(ng=2), "cu_groups"), (dict(ng=0, cg=P), "cu_groups"), (dict(ng=-1), "count"),
-    (dict(nseq=-1), "count"), (dict(ntok=1 << 25), "count"), (dict(nseq=4096, ntok=4096), "4096"), (dict(ntok=5), "as many"),
+    (dict(nseq=-1), "count"), (dict(ntok=1 << 25), "count"), (dict(nseq=1024, ntok=1024), "1024"), (dict(ntok=5), "as many"),
     (dict(qs=1016), "strides"), (dict(ks=248), "strides"), (dict(vs=260), "aligned"), (dict(q=P + 2), "aligned"),
     (dict(cs=P + 4), "aligned"), (dict(vc=P + 8), "aligned"), (dict(out=P), "must not be q"), (dict(ws=None), "workspace"),
     (dict(wsb=100), "workspace"), (dict(ws=P + 8), "workspace"),
