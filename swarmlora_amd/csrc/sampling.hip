@@ -42,7 +42,7 @@ constexpr int kListed = 4096;   // tokens of a row's list (of more than that, th
 constexpr int kMaxSlices = 256;
 constexpr int kGather = 1024;    // tokens that a slice can list
 constexpr int kShort = 128;      // of rows that keep no more than so many tokens all are listed
-constexpr int kWorkgroups = 512;
+constexpr int kWorkgroups = 1024;
 
 // What the second launch finds of a row.
 struct RowPlan {
