@@ -8,7 +8,7 @@
 // Rows are (new token, query head) pairs of one kv head, row = token * G + head.
 // A prefix is walked once for the rows of all its sequences together, a
 // sequence's own tokens for its rows alone, and what the two leave (a row's
-// maximum, its sum of probabilities and the sum of values under them, fp32) is
+// maximum, its sum of probabilities and the mean of values under them, fp32) is
 // merged.  A sequence with a block of rows to itself (128: a prompt) gains nothing
 // from company: it walks its prefix and its own tokens in one go and is not
 // merged.
@@ -502,8 +502,9 @@ __device__ __forceinline__ Keys keys_of(const PrefixArgs& a, const Part& u, int 
 // One row of a part by a wave, seeing its own keys alone: sixteen lanes a key (8
 // dims each), four keys at a time.  For rows that an infinity or a NaN of a key
 // they do not see may have reached (0 times it is a NaN), and keys without a page.
-__device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float& mx, float& sm,
-                         float (&acc)[8]) {
+// acc: sums of the values times `by`.
+__device__ void slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float by, float& mx,
+                          float& sm, float (&acc)[8]) {
   const int i = (uint32_t)r / a.by_g;
   const bf16* qp = a.q + (int64_t)token_at(a, u, i) * a.qs + (int64_t)(h * a.G + r - i * a.G) * kD + 8 * (lane & 15);
   const float c2 = a.scale * 1.44269504088896340736f;
@@ -534,7 +535,7 @@ __device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, in
       const float nm = fmaxf(mx, sc), corr = merge_factor(mx, nm), p = __builtin_amdgcn_exp2f(sc - (nm == -INFINITY ? 0.f : nm));
       sm = sm * corr + p;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) acc[d] = acc[d] * corr + p * vf[d];
+      for (int d = 0; d < 8; ++d) acc[d] = acc[d] * corr + p * (vf[d] * by);
       mx = nm;
     }
   }
@@ -551,16 +552,40 @@ __device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, in
   }
 }
 
-// K dims from d of a row's result: to the output where the part is all there is of
-// it, else to its record.
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }  // (0: no key)
+
+// mean: the row's result.  Where sums of large values are no 32-bit numbers though
+// their means are (2^31 keys at most), the sums are those of 2^-32 of them.
+__device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float& mx, float& sm,
+                         float (&mean)[8]) {
+  slow_sums(a, u, h, kend, r, lane, 1.f, mx, sm, mean);
+  const float inv = inverse(sm);
+  bool large = false;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    large |= not_finite(mean[d]);
+    mean[d] *= inv;
+  }
+  if (__ballot(large) == 0) return;
+  float of_part[8];
+  slow_sums(a, u, h, kend, r, lane, 0x1p-32f, mx, sm, of_part);
+#pragma unroll
+  for (int d = 0; d < 8; ++d)
+    if (not_finite(mean[d])) mean[d] = of_part[d] * inv * 0x1p32f;
+}
+
+// K dims from d of a row's result, o * inv: to the output where the part is all
+// there is of it, else to its record.  Records hold means: what is merged of them
+// is no larger than they are.
 template <int K>
 __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int h, int r, int d, float m, float L,
-                                        const float (&o)[K]) {
+                                        const float (&o)[K], float inv) {
   if (u.flags & kDirect) {
     const int i = (uint32_t)r / a.by_g;
     bf16* dst = a.out + ((int64_t)token_at(a, u, i) * a.hq + h * a.G + r - i * a.G) * kD + d;
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // (0: the row sees no key)
-    bf16x2 y[K / 2];
+    bf16x2 y[K / 2];  // (L 0: the row sees no key)
 #pragma unroll
     for (int e = 0; e < K / 2; ++e)
       y[e] = L == 0.f ? bf16x2{f2bf(0.f), f2bf(0.f)} : bf16x2{f2bf(o[2 * e] * inv), f2bf(o[2 * e + 1] * inv)};
@@ -573,15 +598,13 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int 
     float* dst = a.rec_o + at * kD + d;
 #pragma unroll
     for (int e = 0; e < K; e += 4)
-      *(__attribute__((address_space(1))) f32x4*)(dst + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+      *(__attribute__((address_space(1))) f32x4*)(dst + e) = f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
     if (d == 0) {
       a.rec_ml[2 * at] = m;
       a.rec_ml[2 * at + 1] = L;
     }
   }
 }
-
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
 // 16 bytes a lane from global memory to LDS at `to` (the same for the wave) + 16
 // lane.  The compiler puts a wait for all of these before every turned read, also
@@ -801,12 +824,13 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
     if (g == 0) {
       dst[128] = m[e];
       dst[129] = l[e];
+      if constexpr (MANY) dst[130] = inverse(l[e]);
     }
   };
   auto again = [&](int r) {
     float mx, sm, y[8];
     slow_row(a, u, h, kend, r, lane, mx, sm, y);
-    if (lane < 16) put_row<8>(a, u, h, r, 8 * lane, mx, sm, y);
+    if (lane < 16) put_row<8>(a, u, h, r, 8 * lane, mx, sm, y, 1.f);
   };
   if constexpr (MANY) {  // every wave its own, 32 lanes a row
     if (idle) return;
@@ -829,7 +853,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         const float* src = mg + (w * 16 + i) * F;
         const f32x4 v = *reinterpret_cast<const f32x4*>(src + d);
         const float o[4] = {v[0], v[1], v[2], v[3]};
-        if (r0 + i < rows && !(redo >> i & 1)) put_row<4>(a, u, h, r0 + i, d, src[128], src[129], o);
+        if (r0 + i < rows && !(redo >> i & 1)) put_row<4>(a, u, h, r0 + i, d, src[128], src[129], o, src[130]);
       }
       for (; redo; redo &= redo - 1) again(r0 + __builtin_ctzll(redo));
       __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -862,7 +886,8 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         for (int d = 0; d < 8; ++d) bad |= not_finite(o[d]);
       }
       const uint64_t redo = __ballot(bad);
-      if (row < nr && (redo >> (lane & 48) & 0xffffu) == 0) put_row<8>(a, u, h, u.r0 + 16 * e + row, x8, M, L, o);
+      if (row < nr && (redo >> (lane & 48) & 0xffffu) == 0)
+        put_row<8>(a, u, h, u.r0 + 16 * e + row, x8, M, L, o, inverse(L));
       for (int i = 0; i < 4; ++i)  // the wave's four rows
         if (redo >> (16 * i) & 0xffffu) again(u.r0 + 16 * e + 4 * w + i);
     }
@@ -917,9 +942,10 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
           if (p0 + b >= parts) break;
           const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
           if (pl[b] != 0.f) {  // (a part without a key counts for nothing)
-            L = L * fa + pl[b] * fb;
+            const float la = L * fa, lb = pl[b] * fb, inv = __builtin_amdgcn_rcpf(la + lb);  // (off by 2^-23)
+            L = la + lb;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = o[e] * fa + po[b][e] * fb;
+            for (int e = 0; e < 4; ++e) o[e] = o[e] * (la * inv) + po[b][e] * (lb * inv);
             M = mn;
           }
         }
@@ -927,10 +953,9 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
     };
     take(r.pre + h * r.pre_head + row, r.pre_rows, r.pre_parts);
     take(r.own + h * r.own_head + row, r.own_rows, r.own_parts);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
     bf16 y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = f2bf(L == 0.f ? 0.f : o[e] * inv);
+    for (int e = 0; e < 4; ++e) y[e] = f2bf(o[e]);  // (without a key 0)
     stg(a.out + ((int64_t)t * a.hq + j) * kD + d, __builtin_bit_cast(u32x2, *reinterpret_cast<bf16(*)[4]>(&y)));
   }
 }

@@ -118,3 +118,238 @@ def _check(c, dev):
 ])
 def test_against_the_definition(dev, name, kw):
     _check(_case(sum(map(ord, name)), **kw), dev)
+
+
+@pytest.mark.parametrize("name,kw", [
+    ("many parts of a prefix", dict(new=[1, 1, 2], ctx=[20, 700, 1], pre=[20011], size=[3], max_pos=32768)),
+    ("many sequences and groups", dict(new=[1] * 523, ctx=[i % 40 for i in range(523)], pre=[i % 70 for i in range(301)],
+                                       size=[3 if i % 2 else 0 for i in range(301)], hq=2, hkv=1)),
+    ("a wide table", dict(new=[1, 1], ctx=[20, 64], pre=[81], size=[2], spare=4000)),
+    ("the longest step of few rows", dict(new=[1] * 8, ctx=[64, 0, 63, 65, 1, 127, 128, 129], pre=[64], size=[8], hq=16, hkv=4)),
+])
+def test_plans_against_the_definition(dev, name, kw):
+    _check(_case(sum(map(ord, name)), **kw), dev)
+
+
+def test_a_prompt_long_enough_to_be_cut_once_more(dev):
+    # 207 blocks of rows x 63 steps, each counted twice, over 512 places: 51 steps
+    # a place, more than the 32 that are cut
+    c = _case(5, new=[3300], ctx=[0], pre=[700], size=[1], hq=8, hkv=1)
+    got, d = _run(c, dev)
+    q, k, v = _views(c, c["qkv"])
+    rows = c["cs"][c["pos"]]
+    qr, kr = (_prefix.rotate(x, rows).float().to(BF16) for x in (q, k))
+    keys, vals = (torch.cat([_prefix.held(x, c["pt"][0], 700)[0], y.double()])[:, 0]
+                  for x, y in ((c["kc"], kr), (c["vc"], v)))
+    see = torch.arange(4000)[None] <= torch.arange(700, 4000)[:, None]
+    for h in range(8):
+        p = torch.softmax((qr[:, h].double() @ keys.T * c["scale"]).masked_fill(~see, -math.inf), -1)
+        want, w = p @ vals, p @ vals.abs()
+        # the tolerance of _check
+        off = (got.cpu().double()[:, h * 128:(h + 1) * 128] - want).abs()
+        assert bool((off <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * w + 1e-30).all()), h
+
+
+MIXED = dict(new=[1, 4, 40, 2, 0, 1], ctx=[5, 0, 40, 9, 3, 130], pre=[260, 77], size=[4, 2])
+
+
+def _seen(c):
+    """Tokens of the cache [num_blocks, page] that some sequence sees or stores."""
+    page = c["kc"].shape[1]
+    m = torch.zeros(c["kc"].shape[:2], dtype=torch.bool)
+
+    def mark(row, n):
+        for p in range(max(n, 0)):
+            if p // page < len(row) and 0 <= row[p // page] < len(m):
+                m[row[p // page], p % page] = True
+
+    for g in range(len(c["plens"])):
+        mark(c["pt"][g].tolist(), int(c["plens"][g]))
+    for s in range(len(c["lens"])):
+        mark(c["bt"][s].tolist(), int(c["lens"][s] + c["cu"][s + 1] - c["cu"][s]))
+    return m
+
+
+@pytest.mark.parametrize("kw", [MIXED, dict(new=[1] * 5, ctx=[0, 5, 16, 63, 64], pre=[100], size=[5]),
+                                dict(new=[140], ctx=[3], pre=[70], size=[1], page=96)])
+def test_what_is_not_seen_does_not_matter(dev, kw):
+    c = _case(31, **kw)
+    want, _ = _run(c, dev)
+    for fill in (math.nan, math.inf, -math.inf):
+        d = dict(c, kc=c["kc"].clone(), vc=c["vc"].clone())
+        d["kc"][~_seen(c)] = fill
+        d["vc"][~_seen(c)] = fill
+        got, _ = _run(d, dev)
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16)), fill
+
+
+@pytest.mark.parametrize("kw", [MIXED, dict(new=[1] * 3, ctx=[40, 5, 16], pre=[100], size=[3])])
+def test_pages_that_are_not_there_are_not_seen(dev, kw):
+    c = _case(32, **kw)
+    c["pt"][0, 1] = -1
+    c["pt"][0, 4] = len(c["kc"])
+    c["bt"][0, 0] = -7
+    c["bt"][1, 0] = 2 ** 31 - 1
+    c["bt"][2, 1] = len(c["kc"])
+    _check(c, dev)
+
+
+def test_a_sequence_none_of_whose_pages_are_there_has_zeros(dev):
+    c = _case(33, new=[1, 3], ctx=[20, 1], pre=[81], size=[2])
+    c["pt"][:] = -1
+    c["bt"][1] = -1
+    got, _ = _check(c, dev)
+    assert not bool(got[1:].any())
+
+
+@pytest.mark.parametrize("where", ["prefix", "own", "new"])
+def test_not_a_number_reaches_those_that_see_it(dev, where):
+    c = _case(34, **MIXED)
+    v = _views(c, c["qkv"])[2]
+    if where == "prefix":
+        c["vc"][c["pt"][1, 1], 3, 0, 5] = math.nan
+    elif where == "own":
+        c["vc"][c["bt"][2, 0], 3, 1, 9] = math.nan
+    else:
+        v[3, 0, 17] = math.nan  # the third of the second sequence's four tokens
+    got, _ = _check(c, dev)
+    assert 0 < int(torch.isnan(got).sum()) < got.numel() // 8
+
+
+def test_sums_that_leave_32_bits_are_done_again(dev):
+    # sums of a few hundred values near 2^127 are no 32-bit numbers, their means are
+    c = _case(35, **MIXED)
+    c["vc"].mul_(0).add_(3e38)
+    _views(c, c["qkv"])[2].mul_(0).add_(3e38)
+    got, _ = _check(c, dev)
+    assert bool(torch.isfinite(got).all())
+
+
+def test_without_new_keys_positions_or_offsets(dev):
+    from swarmlora_amd import ops
+    c = _case(36, new=[3] * 4, ctx=[5, 0, 40, 9], pre=[100], size=[4])
+    d = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    q, k, v = _views(c, d["qkv"])
+    packed = ops.prefix_attention(q, k, v, d["kc"], d["vc"], d["pt"], d["plens"], d["bt"], d["lens"], d["pos"], d["cs"],
+                                  c["scale"], cu_seqlens=d["cu"])
+    # [nseq, L]: the same call
+    kc, vc = c["kc"].to(dev), c["vc"].to(dev)
+    u = [t.view(4, 3, t.shape[1], 128) for t in (q, k, v)]
+    even = ops.prefix_attention(*u, kc, vc, d["pt"], d["plens"], d["bt"], d["lens"], d["pos"], d["cs"], c["scale"])
+    assert even.shape == (4, 3, 8 * 128) and torch.equal(even.flatten(0, 1), packed)
+    assert torch.equal(kc, d["kc"]) and torch.equal(vc, d["vc"])
+    # keys that are there already, queries rotated before
+    qr = _prefix.rotate(_views(c, c["qkv"])[0], c["cs"][c["pos"]]).float().to(BF16)
+    got = ops.prefix_attention(qr.to(dev), None, None, kc, vc, d["pt"], d["plens"], d["bt"], d["lens"], None, None,
+                               c["scale"], cu_seqlens=d["cu"])
+    assert torch.equal(kc, d["kc"]) and torch.equal(vc, d["vc"])
+    o, w = _prefix.attend(qr, kc.cpu(), vc.cpu(), c["pt"], c["plens"], c["cg"], c["bt"], c["lens"], c["cu"], c["scale"])
+    off = (got.cpu().double() - o.flatten(1)).abs()
+    assert bool((off <= 2.0 ** -8 * o.flatten(1).abs() + 2.0 ** -7 * w.flatten(1) + 1e-30).all())
+
+
+def test_no_prefix_at_all_is_paged_attention(dev):
+    from swarmlora_amd import ops
+    c = _case(37, new=[1] * 4, ctx=[5, 0, 140, 9], pre=[], size=[])
+    d = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    q, k, v = (t.view(4, 1, t.shape[1], 128) for t in _views(c, d["qkv"]))
+    kc, vc = c["kc"].to(dev), c["vc"].to(dev)
+    got = ops.prefix_attention(q, k, v, kc, vc, d["bt"][:0, :0], d["plens"], d["bt"], d["lens"], d["pos"], d["cs"], c["scale"])
+    want = ops.paged_attention(q, k, v, d["kc"], d["vc"], d["bt"], d["lens"], d["pos"], d["cs"], c["scale"])
+    assert torch.equal(kc, d["kc"]) and torch.equal(vc, d["vc"])
+    # both are off by half a step and their probabilities' roundings
+    w = _want(c)[1].view(4, 1, -1)
+    assert bool(((got.cpu() - want.cpu()).abs().double() <= 2.0 ** -7 * want.cpu().abs() + 2.0 ** -6 * w).all())
+
+
+def test_sequences_before_the_first_group(dev):
+    c = _case(38, new=[1, 2, 1, 1], ctx=[5, 0, 40, 9], pre=[100], size=[4])
+    c["cg"] = torch.tensor([1, 3], dtype=torch.int32)
+    _check(c, dev)
+
+
+def test_rows_behind_the_last_sequence_are_left(dev):
+    c = _case(39, new=[2, 1, 30], ctx=[20, 1, 0], pre=[81], size=[3], extra=5)
+    out = torch.full((38, 8 * 128), 7.0, dtype=BF16, device=dev)
+    got, d = _run(c, dev, out=out)
+    assert got.data_ptr() == out.data_ptr() and bool((out[33:] == 7).all())
+    assert torch.equal(out[:33], _run(c, dev)[0][:33])
+
+
+def test_caches_past_four_gigabytes(dev):
+    c = _case(40, new=[1, 2, 150], ctx=[30, 0, 17], pre=[100], size=[3])
+    want, d = _run(c, dev)
+    # 16 tokens of 2 heads are 8 KiB: 600000 pages are 4.9 GB a cache
+    far = 600000 - len(c["kc"])
+    big = dict(d)
+    for n in ("kc", "vc"):
+        big[n] = torch.empty(600000, *c["kc"].shape[1:], dtype=BF16, device=dev)
+        big[n][far:] = c[n].to(dev)
+    for n in ("pt", "bt"):
+        big[n] = d[n] + far
+    assert torch.equal(_run_there(big), want)
+    assert torch.equal(big["kc"][far:], d["kc"]) and torch.equal(big["vc"][far:], d["vc"])
+
+
+def _run_there(d, out=None):
+    """The call on what is on the device already, in place."""
+    from swarmlora_amd import ops
+    q, k, v = _views(d, d["qkv"])
+    return ops.prefix_attention(q, k, v, d["kc"], d["vc"], d["pt"], d["plens"], d["bt"], d["lens"], d["pos"], d["cs"],
+                                d["scale"], cu_groups=d["cg"], cu_seqlens=d["cu"], out=out)
+
+
+def test_captured_calls_follow_lengths_and_tables(dev):
+    """Two graphs of calls, each replayed several times with other lengths, tables
+    and groups behind the same addresses, eager calls between them."""
+    cases = [_case(50 + i, new=n, ctx=c, pre=p, size=z) for i, (n, c, p, z) in enumerate([
+        ([1, 1, 1, 1], [5, 0, 40, 9], [100, 0], [3, 1]), ([1, 1, 1, 1], [6, 1, 300, 0], [0, 999], [1, 3]),
+        ([1, 1, 1, 1], [0, 0, 0, 0], [17, 64], [2, 2]), ([4, 0, 0, 0], [3, 1, 1, 1], [64, 640], [4, 0])])]
+    # buffers as large as the largest case's
+    size = {n: [max(c[n].shape[i] for c in cases) for i in range(c0.dim())]
+            for n, c0 in cases[0].items() if isinstance(c0, torch.Tensor)}
+
+    def load(d, c):
+        for n, s in size.items():
+            t = torch.zeros(s, dtype=c[n].dtype)
+            t[tuple(slice(0, x) for x in c[n].shape)] = c[n]
+            d[n].copy_(t)
+
+    state = [dict({n: torch.zeros(s, dtype=cases[0][n].dtype, device=dev) for n, s in size.items()}, hq=8, hkv=2,
+                  scale=cases[0]["scale"]) for _ in range(2)]
+    graphs, outs = [], []
+    for d in state:
+        load(d, cases[0])
+        _run_there(d)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_run_there(d))
+        graphs.append(g)
+    for i in (1, 2, 0, 3, 1):
+        for d, j in zip(state, (i, (i + 1) % 4)):
+            load(d, cases[j])
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for o, j in zip(outs, (i, (i + 1) % 4)):
+            want, _ = _run(cases[j], dev)
+            assert torch.equal(o, want), (i, j)
+
+
+def test_two_streams_at_once(dev):
+    cases = [_case(60 + i, **MIXED) for i in range(2)]
+    want = [_run(c, dev)[0] for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    state = [[{k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()} for _ in range(4)] for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for r in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_run_there(state[i][r]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, want[i])
