@@ -124,11 +124,21 @@ class BatchedDecoder:
     whole-K round (w_layout 2: one launch, no K-slice partials; 206 us
     against 248 for the K-sliced round at 28 workers); the projection rounds
     are K-sliced (whole-K rounds measured slower for them).
+    prefixes (fused step only): [(tokens, workers), ...], consecutive workers
+    whose contexts begin with the same tokens; these are held once and read once a
+    step for all of a group (ops.prefix_attention), and ctx_lens count the tokens
+    behind them.  kv_fill's block_tables then have a row for each prefix behind
+    the workers' rows.
+    sampling: a dict of ops.sample_tokens' u and temperature (top_k, top_p and
+    min_p as wanted), device tensors of W entries that every step reads, also a
+    captured one; the caller writes new random numbers into u between steps.
+    None: greedy.
     """
 
     def __init__(self, shape: DecodeShape, weights: dict, adapters: List[Optional[dict]], ctx_lens: List[int],
                  first_ids: List[int], device, max_new: int = 64, kv_fill=None, fused: bool = True,
-                 packed: bool = True, whole_k: bool = True):
+                 packed: bool = True, whole_k: bool = True, prefixes: Optional[List[tuple]] = None,
+                 sampling: Optional[Dict[str, torch.Tensor]] = None):
         self.shape = s = shape
         self.device = dev = torch.device(device)
         self.W = W = len(ctx_lens)
@@ -136,6 +146,12 @@ class BatchedDecoder:
             raise ValueError(f"1..{ops.RowSet.MAX_ROWS} workers")
         if len(adapters) != W or len(first_ids) != W:
             raise ValueError("one adapter entry and one first token per worker")
+        self.prefixes = list(prefixes or [])
+        if self.prefixes and not fused:
+            raise ValueError("prefixes need the fused step")
+        if any(t < 1 or n < 1 for t, n in self.prefixes) or sum(n for _, n in self.prefixes) > W:
+            raise ValueError("prefixes: at least one token and worker each, no more workers than there are")
+        self.sampling = sampling
         self.max_new = max_new
         self.steps_done = 0
         self.graph = None
@@ -211,20 +227,33 @@ class BatchedDecoder:
 
     def _init_kv(self, ctx_lens, kv_fill):
         s, dev, W = self.shape, self.device, self.W
-        self.kv = PagedKVCache(s.layers, s.kv_heads, s.head_dim, s.block_size, W, max(ctx_lens) + self.max_new, dev,
-                               BF16)
+        P = len(self.prefixes)
+        longest = max([t for t, _ in self.prefixes], default=0)
+        self.kv = PagedKVCache(s.layers, s.kv_heads, s.head_dim, s.block_size, W + P,
+                               max(max(ctx_lens) + self.max_new, longest), dev, BF16)
         for w, c in enumerate(ctx_lens):
             self.kv.ensure_blocks_for_length(w, c + self.max_new)
             self.kv.slot_seq_lens[w] = c
-        self.block_tables = self.kv.get_block_table_tensor(list(range(W)))
+        for i, (t, _) in enumerate(self.prefixes):
+            self.kv.ensure_blocks_for_length(W + i, t)
+            self.kv.slot_seq_lens[W + i] = t
+        tables = self.kv.get_block_table_tensor(list(range(W + P)))
+        self.block_tables, self.prefix_tables = tables[:W], tables[W:]
         if kv_fill is not None:
             for li in range(s.layers):
-                kv_fill(li, self.kv.key_caches[li], self.kv.value_caches[li], self.block_tables)
+                kv_fill(li, self.kv.key_caches[li], self.kv.value_caches[li], tables)
         self.seqlens = self.kv.get_seq_lens_tensor(list(range(W)))
         self.positions = torch.zeros(W, dtype=torch.int64, device=dev)
+        self.prefix_of = None  # tokens before each worker's own
+        if P:
+            groups = [n for _, n in self.prefixes]
+            self.prefix_lens = torch.tensor([t for t, _ in self.prefixes], dtype=torch.int32).to(dev)
+            self.cu_groups = torch.tensor([sum(groups[:i]) for i in range(P + 1)], dtype=torch.int32).to(dev)
+            of = [t for t, n in self.prefixes for _ in range(n)]
+            self.prefix_of = torch.tensor(of + [0] * (W - len(of)), dtype=torch.int64).to(dev)
         from .worker.paged_attention import RotaryInvFreq, build_vllm_cos_sin_cache
-        self.cos_sin = build_vllm_cos_sin_cache(RotaryInvFreq(s.head_dim, s.theta), self.kv.max_blocks_per_seq *
-                                                s.block_size, dev, BF16)
+        self.cos_sin = build_vllm_cos_sin_cache(RotaryInvFreq(s.head_dim, s.theta), longest +
+                                                self.kv.max_blocks_per_seq * s.block_size, dev, BF16)
 
     def _init_fused(self, weights, adapters, ctx_lens, first_ids, kv_fill):
         """In-process step over explicit token rows with the round fusions
@@ -356,21 +385,35 @@ class BatchedDecoder:
     def _body_fused(self):
         s = self.shape
         self.positions.copy_(self.seqlens)
+        if self.prefix_of is not None:
+            self.positions.add_(self.prefix_of)
         ops.embed(self._ids_rows, self.embed, self._h_rows)
         ops.rmsnorm_rows(self.h, self.norms[0][0], s.eps, self.rows_x0)
         for li in range(s.layers):
             qkv, o, gu, down = self._calls[li]
             self._round_ex(qkv)
-            ops.paged_attention_rows(self.rows_qkv, self.rows_attn, 1, s.heads, s.kv_heads, s.head_dim,
-                                     self.kv.key_caches[li], self.kv.value_caches[li], self.block_tables,
-                                     self.seqlens, None, None, self._scale, rope=2)
+            if self.prefix_of is None:
+                ops.paged_attention_rows(self.rows_qkv, self.rows_attn, 1, s.heads, s.kv_heads, s.head_dim,
+                                         self.kv.key_caches[li], self.kv.value_caches[li], self.block_tables,
+                                         self.seqlens, None, None, self._scale, rope=2)
+            else:  # (the round has rotated q and k and stored k and v)
+                q = self.qkv[:, :s.heads * s.head_dim].view(self.W, 1, s.heads, s.head_dim)
+                ops.prefix_attention(q, None, None, self.kv.key_caches[li], self.kv.value_caches[li],
+                                     self.prefix_tables, self.prefix_lens, self.block_tables, self.seqlens, None, None,
+                                     self._scale, cu_groups=self.cu_groups, out=self.attn.view(self.W, 1, -1))
             self._round_ex(o)
             self._round_ex(gu)
             self._round_ex(down)
         self._round_ex(self._lm_call)
-        W = self.W
-        ops.sample(self.logits, self._ids_rows, [False] * W, [1.0] * W, [0] * W, [1.0] * W, 0)
+        self._next_tokens()
         self.seqlens.add_(1)
+
+    def _next_tokens(self):
+        W = self.W
+        if self.sampling is None:
+            ops.sample(self.logits, self._ids_rows, [False] * W, [1.0] * W, [0] * W, [1.0] * W, 0)
+        else:
+            ops.sample_tokens(self.logits, **self.sampling, out=self.ids.view(W))
 
     # ------------------------------------------------------------ one step
     def _round(self, op: int, layer: int):
@@ -396,8 +439,7 @@ class BatchedDecoder:
             self._round(agg.OP_DOWN_PROJ, li)
         ops.rmsnorm_rows(self.h, self.final_norm, s.eps, self.rows_lm, add_rows=self.rows_out_h)
         ops.gemm(self.lm_in, self.lm_head, out=self.logits)
-        W = self.W
-        ops.sample(self.logits, self._ids_rows, [False] * W, [1.0] * W, [0] * W, [1.0] * W, 0)
+        self._next_tokens()
         self.seqlens.add_(1)
 
     def _check_capacity(self):
