@@ -461,10 +461,6 @@ __device__ __forceinline__ float max_groups(float v) {  // over the four lane gr
   auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float sum_groups(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
-}
 
 // e^(m - M) in powers of two; a side without a key (-inf) counts for nothing.
 __device__ __forceinline__ float merge_factor(float m, float M) {
@@ -611,7 +607,7 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int 
 // of the other buffer (it does not for the builtin's plain reads), so they are
 // issued past it: no register is written, wait_dma is the wait, and nothing else
 // in this kernel uses m0.
-__device__ __forceinline__ void dma16(const bf16* from, char* to) {
+__device__ __forceinline__ void dma16(const char* from, char* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"((gbl_ptr)from), "s"(at) : "memory");
 }
@@ -665,13 +661,15 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
     return there ? blk * a.bs + (int)((uint32_t)key - (uint32_t)key / a.by_bs * (uint32_t)a.bs) : 0;
   };
   // (16 bytes of four keys an instruction: lane i of it has place i % 16 of key i / 16)
+  const uint32_t row_bytes = (uint32_t)a.hkv * (kD * 2), lane_at = (uint32_t)h * (kD * 2) + 16 * (col ^ g);
+  const char *kc = reinterpret_cast<const char*>(a.kc), *vc = reinterpret_cast<const char*>(a.vc);
   auto fetch = [&](int row, int buf) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = __shfl(row, 4 * i + g, 64);
-      const int64_t at = (r * a.hkv + h) * kD + 8 * (col ^ (4 * i + g));
-      dma16(a.kc + at, sh.kv[buf][0] + (16 * w + 4 * i) * 256);
-      dma16(a.vc + at, sh.kv[buf][1] + (16 * w + 4 * i) * 256);
+      const uint32_t r = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (4 * i + g), row);
+      const uint64_t at = (uint64_t)r * row_bytes + (lane_at ^ (uint32_t)(64 * i));
+      dma16(kc + at, sh.kv[buf][0] + (16 * w + 4 * i) * 256);
+      dma16(vc + at, sh.kv[buf][1] + (16 * w + 4 * i) * 256);
     }
   };
 
@@ -697,12 +695,12 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
     see[e] = min(max(u.len + i + 1, 0), kend);
   }
   const float c2 = a.scale * 1.44269504088896340736f;  // scores in powers of two
-  float m[SETS], l[SETS];
-  f32x4 acc[SETS][8];
+  float m[SETS];
+  f32x4 l[SETS], acc[SETS][8];  // (l: of a product with ones, four times the same)
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
     m[e] = -INFINITY;
-    l[e] = 0.f;
+    l[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[e][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -719,9 +717,10 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
       fetch(row, buf ^ 1);
       if (MANY && lane == 0) sh.none[buf ^ 1][w] = none_next;
     }
-    const char* kb = sh.kv[buf][0];
-    const char* vb = sh.kv[buf][1];
+    const char* kv = sh.kv[0][0];
     if (!idle) {
+      // K: 16 bytes of key col of a tile, dims 32 k + 8 g ..
+      const uint32_t k_at = buf * 32768 + t0 * 4096 + col * 256 + ((g ^ col) << 4);
       f32x4 s[SETS][T];
 #pragma unroll
       for (int t = 0; t < T; ++t) {
@@ -729,7 +728,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         for (int e = 0; e < SETS; ++e) s[e][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kb + (16 * (t0 + t) + col) * 256 + (((4 * k + g) ^ col) << 4));
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(kv + (k_at ^ (64 * k)) + t * 4096);
 #pragma unroll
           for (int e = 0; e < SETS; ++e) s[e][t] = mfma16(kf, q[e][k], s[e][t]);
         }
@@ -757,11 +756,10 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < T; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[e][t][0], s[e][t][1]), fmaxf(s[e][t][2], s[e][t][3])));
-        mx = c2 * max_groups(mx);
         // the reference the exponents are taken from moves only when the maximum
         // has grown by 2^8 since: any reference gives the same quotient
-        if (__ballot(mx > m[e] + 8.f) != 0) {
-          const float mn = fmaxf(m[e], mx), corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
+        if (__ballot(mx * c2 > m[e] + 8.f) != 0) {
+          const float mn = fmaxf(m[e], c2 * max_groups(mx)), corr = mn == m[e] ? 1.f : __builtin_amdgcn_exp2f(m[e] - mn);
           m[e] = mn;
           l[e] *= corr;
 #pragma unroll
@@ -775,15 +773,28 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
           for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], c2, -mr));
           const bf16x2 lo = {f2bf(x[0]), f2bf(x[1])}, hi = {f2bf(x[2]), f2bf(x[3])};
           p[e][t] = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-          // (summed as rounded: the weights sum to 1)
-          l[e] += (bf2f(lo[0]) + bf2f(lo[1])) + (bf2f(hi[0]) + bf2f(hi[1]));
+        }
+      }
+      // The sums of the probabilities (as rounded: then the weights sum to 1) are
+      // products with ones: the vector units, not the matrix ones, are what a step of
+      // many rows waits for.
+      const uint32_t one = 0x3f803f80u;
+#pragma unroll
+      for (int e = 0; e < SETS; ++e) {
+        if constexpr (MANY) {
+#pragma unroll
+          for (int t = 0; t < 4; t += 2)
+            l[e] = mfma16(u32x4{one, one, one, one}, u32x4{p[e][t][0], p[e][t][1], p[e][t + 1][0], p[e][t + 1][1]}, l[e]);
+        } else {
+          l[e] = mfma16k16(u32x2{one, one}, p[e][0], l[e]);
         }
       }
       // V^T: of four keys 4 g + (lane / 4) % 4 ..., dims 32 c + 4 (d ^ c % 2) .. + 3, c = lane % 4
+      const int c = lane & 3, key = 4 * g + (col >> 2);
+      const uint32_t v_at = buf * 32768 + 16384 + key * 256 + (((4 * c) ^ key) << 4) + 8 * (c & 1);
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        const int c = lane & 3, key = 4 * g + (col >> 2), dd = d ^ (c & 1);
-        const char* vp = vb + key * 256 + (((4 * c + (dd >> 1)) ^ key) << 4) + 8 * (dd & 1);
+        const char* vp = kv + (v_at ^ (8 * d));
         if constexpr (MANY) {
 #pragma unroll
           for (int t = 0; t < 4; t += 2) {
@@ -817,14 +828,13 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
   float* mg = reinterpret_cast<float*>(sh.kv);
   static_assert(4 * 16 * F * 4 <= (int)sizeof(sh.kv), "the waves' rows");
   auto leave = [&](int e) {
-    l[e] = sum_groups(l[e]);
     float* dst = mg + (w * 16 + col) * F;
 #pragma unroll
     for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(dst + 32 * g + 4 * (d ^ (g & 1))) = acc[e][d];
     if (g == 0) {
       dst[128] = m[e];
-      dst[129] = l[e];
-      if constexpr (MANY) dst[130] = inverse(l[e]);
+      dst[129] = l[e][0];
+      if constexpr (MANY) dst[130] = inverse(l[e][0]);
     }
   };
   auto again = [&](int r) {
@@ -837,7 +847,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
       const int r0 = wr0 + 16 * e;
-      bool bad = not_finite(l[e]);
+      bool bad = not_finite(l[e][0]);
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
