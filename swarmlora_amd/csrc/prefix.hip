@@ -173,12 +173,13 @@ struct PlanLds {  // of E = ngroups + nseq entries: the groups' prefixes, then t
   int32_t* steps; // [E]
   int32_t* pre;   // [E] of them, the prefix's
   int32_t* first; // [E] first part
+  int32_t* parts; // [E] of a block of its rows
   int32_t* len;   // [E] tokens of the prefix; own tokens before the new ones
   int32_t* few;   // [nseq + 1] tokens before it that share their prefix
   int32_t* t0;    // [nseq] first token
   int32_t* cg;    // [ngroups + 1] first sequence, in range
 };
-constexpr int kPlanEntry = 8 + 8 * 4;
+constexpr int kPlanEntry = 8 + 9 * 4;
 
 __device__ void make_plan(const PrefixArgs& a, char* lds) {
   __shared__ int64_t sh64[4];
@@ -193,7 +194,8 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
   l.steps = l.rows + E;
   l.pre = l.steps + E;
   l.first = l.pre + E;
-  l.len = l.first + E;
+  l.parts = l.first + E;
+  l.len = l.parts + E;
   l.few = l.len + E;
   l.t0 = l.few + ns + 1;
   l.cg = l.t0 + ns;
@@ -278,6 +280,7 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
     int64_t recs = 0;
     if (e < E) {
       const int rows = l.rows[e], spp = steps_per_part(e), parts = (l.steps[e] + spp - 1) / spp;
+      l.parts[e] = parts;
       units = (rows + kRows - 1) / kRows * parts;
       const bool joined = e < ng || l.few[e - ng + 1] > l.few[e - ng];
       recs = joined || parts > 1 ? (int64_t)rows * parts * a.hkv : 0;
@@ -305,14 +308,13 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
     if (l.rec[e] >= 0) {
       r.own = l.rec[e];
       r.own_rows = l.rows[e];
-      const int spp = steps_per_part(e);
-      r.own_parts = (l.steps[e] + spp - 1) / spp;
+      r.own_parts = l.parts[e];
       r.own_head = (int64_t)r.own_rows * r.own_parts;
     }
     if (l.few[s + 1] > l.few[s]) {
-      const int g = group_of(s), spp = steps_per_part(g);
+      const int g = group_of(s);
       r.pre_rows = l.rows[g];
-      r.pre_parts = (l.steps[g] + spp - 1) / spp;
+      r.pre_parts = l.parts[g];
       r.pre_head = (int64_t)r.pre_rows * r.pre_parts;
       r.pre = l.rec[g] + (int64_t)(l.few[s] - l.few[l.cg[g]]) * a.G;
       for (int i = 0; i < r.n && l.few[s] + i < a.T; ++i) a.list[l.few[s] + i] = r.t0 + i;
@@ -334,7 +336,7 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
       else
         hi_e = mid;
     }
-    const int e = lo_e, spp = steps_per_part(e), parts = (l.steps[e] + spp - 1) / spp, rows = l.rows[e];
+    const int e = lo_e, spp = steps_per_part(e), parts = l.parts[e], rows = l.rows[e];
     const int local = u - l.first[e], b = local / parts, p = local - b * parts;
     o = Part{};
     if (local < 0 || (int64_t)b * kRows >= rows) return;  // (counts past 32 bits, by offsets that are none)
@@ -370,20 +372,24 @@ __device__ void make_plan(const PrefixArgs& a, char* lds) {
     return kKinds - 1 - (int)min<int64_t>((int64_t)work * kKinds / (share + 2), kKinds - 1);
   };
   Part o;
-  for (int u = tid; u < total; u += 256) {
-    part_of(u, o);
-    atomicAdd(&kind[kind_of(o)], 1);
-  }
-  __syncthreads();
-  if (tid < kKinds) {
-    int before = 0;
-    for (int i = 0; i < tid; ++i) before += kind[i];
-    at_kind[tid] = before;
-  }
-  __syncthreads();
-  for (int u = tid; u < total; u += 256) {
-    if (total > 256) part_of(u, o);
-    a.part[atomicAdd(&at_kind[kind_of(o)], 1)] = o;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+    for (int u = tid; u < total; u += 256) {
+      if (pass == 0 || total > 256) part_of(u, o);
+      const int k = kind_of(o);
+      if (pass == 0)
+        atomicAdd(&kind[k], 1);
+      else
+        a.part[atomicAdd(&at_kind[k], 1)] = o;
+    }
+    __syncthreads();
+    if (tid < kKinds) {
+      int before = 0;
+      for (int i = 0; i < tid; ++i) before += kind[i];
+      at_kind[tid] = before;
+    }
+    __syncthreads();
   }
 }
 
@@ -935,34 +941,33 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
     const int h = (uint32_t)j / a.by_g, row = i * a.G + j - h * a.G;
     float M = -INFINITY, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    auto take = [&](int64_t rec, int64_t step, int parts) {
-      constexpr int B = 8;  // records in flight together
-      for (int p0 = 0; p0 < parts; p0 += B) {
-        float pm[B], pl[B];
-        f32x4 po[B];
+    const int64_t pre = r.pre + h * r.pre_head + row, own = r.own + h * r.own_head + row;
+    const int parts = r.pre_parts + r.own_parts;
+    constexpr int B = 8;  // records in flight together
+    for (int p0 = 0; p0 < parts; p0 += B) {
+      float pm[B], pl[B];
+      f32x4 po[B];
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-          const int64_t at = rec + (int64_t)min(p0 + b, parts - 1) * step;
-          pm[b] = a.rec_ml[2 * at];
-          pl[b] = a.rec_ml[2 * at + 1];
-          po[b] = *(const __attribute__((address_space(1))) f32x4*)(a.rec_o + at * kD + d);
-        }
+      for (int b = 0; b < B; ++b) {
+        const int p = min(p0 + b, parts - 1), q = p - r.pre_parts;
+        const int64_t at = q < 0 ? pre + (int64_t)p * r.pre_rows : own + (int64_t)q * r.own_rows;
+        pm[b] = a.rec_ml[2 * at];
+        pl[b] = a.rec_ml[2 * at + 1];
+        po[b] = *(const __attribute__((address_space(1))) f32x4*)(a.rec_o + at * kD + d);
+      }
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-          if (p0 + b >= parts) break;
-          const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
-          if (pl[b] != 0.f) {  // (a part without a key counts for nothing)
-            const float la = L * fa, lb = pl[b] * fb, inv = __builtin_amdgcn_rcpf(la + lb);  // (off by 2^-23)
-            L = la + lb;
+      for (int b = 0; b < B; ++b) {
+        if (p0 + b >= parts) break;
+        const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
+        if (pl[b] != 0.f) {  // (a part without a key counts for nothing)
+          const float la = L * fa, lb = pl[b] * fb, inv = __builtin_amdgcn_rcpf(la + lb);  // (off by 2^-23)
+          L = la + lb;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = o[e] * (la * inv) + po[b][e] * (lb * inv);
-            M = mn;
-          }
+          for (int e = 0; e < 4; ++e) o[e] = o[e] * (la * inv) + po[b][e] * (lb * inv);
+          M = mn;
         }
       }
-    };
-    take(r.pre + h * r.pre_head + row, r.pre_rows, r.pre_parts);
-    take(r.own + h * r.own_head + row, r.own_rows, r.own_parts);
+    }
     bf16 y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = f2bf(o[e]);  // (without a key 0)
