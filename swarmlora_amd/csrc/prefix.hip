@@ -18,6 +18,16 @@
 // once), and for every part (block of 128 rows, kv head, steps of 64 keys) what
 // it needs to know, 64 bytes that a workgroup of the second launch reads with one
 // load.  The host knows none of the lengths, so a captured call follows them.
+//
+// Measured on an MI355X (32 query heads over 8, replayed in a graph), with the bytes
+// or operations that a pass cannot do without at the rates of a large copy (5.2
+// TB/s) and a large bf16 product (1108 TFLOP/s):
+//   4 tokens behind 700                  16.6 us (0.6): three launches, each a chain
+//                                        of loads that wait for one another
+//   32 tokens behind 4096, 0.5 K own     31.3 us (12.7): start 6.7, parts 17, merge 6
+//   48 tokens, 6 prefixes up to 12000    64 us (48): the pages' stream
+//   28 sequences' drafts behind 8191     49 us (20)
+//   12 prompts up to 1024 behind 8000    732-780 us (526): 750-800 TFLOP/s
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -32,15 +42,23 @@ namespace {
 constexpr int kD = 128;         // head dim
 constexpr int kRows = 128;      // rows of a block
 constexpr int kKeys = 64;       // keys of a step
-constexpr int kFew = 32;        // rows of a block whose keys its waves share out, 16 each of a step
+// rows of a block whose keys its waves share out, 16 each of a step (a wave's registers
+// hold the results of two sets of 16 rows)
+constexpr int kFew = 32;
 constexpr int kMaxEntries = 1024;
 constexpr int kCus = 256;       // of an MI355X
 constexpr int kPerCu = 2;       // workgroups of a CU (LDS, registers)
 constexpr int kSlots = kCus * kPerCu;
-constexpr int kMinSteps = 4;    // steps of a part at least (blocks of many rows: half of it)
-constexpr int kLong = 32;       // steps of a part that is cut once more,
-constexpr int kCuts = 3;        // into so many
-constexpr int kKinds = 8;
+// Steps of a part at least (blocks of many rows: half of it).  4 tokens behind 700:
+// 18.0 us at 3, 18.7 at 4, 20.1 at 6, 21.4 at 8; 32 tokens behind 4096: 34.1, 33.5,
+// 33.8, 33.3; 28 sequences' drafts 52.4, 51.5, 50.9, 51.4.
+constexpr int kMinSteps = 4;
+// Shares of more steps than kLong are cut into kCuts: places do not end together.  12
+// prompts over 1, 2, 3, 4 and 5 times the places 867, 844, 773, 782, 785 us; but 48
+// tokens, whose shares are short, 67.8, 72.6, 74.2, 84, 84.
+constexpr int kLong = 32;
+constexpr int kCuts = 3;
+constexpr int kKinds = 8;       // of parts, by their work: the ones with the most start first
 
 // Division by a number that the host knows, for dividends under 2^31.
 struct FastDiv {
@@ -635,6 +653,13 @@ __device__ __forceinline__ void wait_dma() {
 // MANY: a wave takes 32 of the block's 128 rows over all 64 keys.  Otherwise the
 // block has at most 32 rows, which every wave takes over the 16 keys it fetched,
 // without a barrier, and the waves' results meet in LDS.
+//
+// Two workgroups fit a CU, and a SIMD has a wave of each.  Of the busy CUs' time the
+// matrix units take 42 % in a step of many rows and the vector units about as much;
+// the two overlap only as the two waves happen to lie.  Measured against this, 12
+// prompts at 779 us: 256 rows a block by eight waves over a ring of four steps 847,
+// the same with 32 x 32 products 803, the halves of a workgroup of eight waves
+// taking turns at products and exponents, a barrier between, 873.
 constexpr int kStepBytes = kKeys * kD * 2;  // keys, or values, of a step
 
 struct AttnLds {
@@ -943,7 +968,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     const int64_t pre = r.pre + h * r.pre_head + row, own = r.own + h * r.own_head + row;
     const int parts = r.pre_parts + r.own_parts;
-    constexpr int B = 8;  // records in flight together
+    constexpr int B = 8;  // records in flight together (4: a few % slower, 12: 40 %)
     for (int p0 = 0; p0 < parts; p0 += B) {
       float pm[B], pl[B];
       f32x4 po[B];

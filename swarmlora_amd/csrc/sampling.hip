@@ -21,6 +21,12 @@
 //      the random number falls in, and its token.
 // The kernels run once through their code: its fetching is much of their time where
 // rows are few, so loops are kept rolled up.
+//
+// Measured on an MI355X, replayed in a graph (a reading of the logits at the rate of a
+// large copy, 5.2 TB/s): one row of 32000, top-p 19 us (0.01): three launches, 3.5 + 7.8 +
+// 14.6 traced, chains of loads, LDS atomics and prefixes that wait for one another; 28
+// rows of 128256 that ask for different things 38 (1.4): 5 + 12 + 28; 256 rows with all
+// filters 108 (12.7): 18 + 50 + 47, two readings weighed in 64 bits.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -42,6 +48,9 @@ constexpr int kListed = 4096;   // tokens of a row's list (of more than that, th
 constexpr int kMaxSlices = 256;
 constexpr int kGather = 1024;    // tokens that a slice can list
 constexpr int kShort = 128;      // of rows that keep no more than so many tokens all are listed
+// Slices in all, about (a row has at most kMaxSlices): 256 rows of 128256 logits 127 us
+// at 512, 108 at 1024, 119 at 2048, 154 at 4096, where every slice's bins are added to
+// the row's.  Fewer rows have slices of two chunks whatever this is.
 constexpr int kWorkgroups = 1024;
 
 // What the second launch finds of a row.

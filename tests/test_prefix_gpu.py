@@ -353,3 +353,45 @@ def test_two_streams_at_once(dev):
     for i in range(2):
         for o in got[i]:
             assert torch.equal(o, want[i])
+
+
+def test_new_keys_as_they_are_and_queries_alone_rotated(dev):
+    from swarmlora_amd import ops
+    c = _case(41, new=[3, 1, 40], ctx=[5, 0, 9], pre=[100], size=[3])
+    d = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    q, k, v = _views(c, c["qkv"])
+    kc, vc = c["kc"].clone(), c["vc"].clone()
+    _prefix.store(kc, c["bt"], c["lens"], c["cu"], k)
+    _prefix.store(vc, c["bt"], c["lens"], c["cu"], v)
+    dq, dk, dv = _views(c, d["qkv"])
+    call = lambda k, v, pos, cs: ops.prefix_attention(  # noqa: E731
+        dq, k, v, d["kc"], d["vc"], d["pt"], d["plens"], d["bt"], d["lens"], pos, cs, c["scale"], cu_groups=d["cg"],
+        cu_seqlens=d["cu"])
+    for args, qr in (((dk, dv, None, None), q),
+                     ((None, None, d["pos"], d["cs"]), _prefix.rotate(q, c["cs"][c["pos"]]).float().to(BF16))):
+        got = call(*args)
+        assert torch.equal(d["kc"].cpu(), kc) and torch.equal(d["vc"].cpu(), vc)
+        o, w = _prefix.attend(qr, kc, vc, c["pt"], c["plens"], c["cg"], c["bt"], c["lens"], c["cu"], c["scale"])
+        off = (got.cpu().double() - o.flatten(1)).abs()
+        # the tolerance of _check
+        assert bool((off <= 2.0 ** -8 * o.flatten(1).abs() + 2.0 ** -7 * w.flatten(1) + 1e-30).all())
+
+
+def test_refusals_of_the_front_end(dev):
+    from swarmlora_amd import ops
+    c = _case(42, new=[1, 2], ctx=[5, 0], pre=[30, 20], size=[1, 1])
+    d = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    q, k, v = _views(c, d["qkv"])
+    base = dict(q=q, k=k, v=v, k_cache=d["kc"], v_cache=d["vc"], prefix_table=d["pt"], prefix_lens=d["plens"],
+                block_table=d["bt"], cache_seqlens=d["lens"], positions=d["pos"], cos_sin=d["cs"],
+                softmax_scale=c["scale"], cu_groups=d["cg"], cu_seqlens=d["cu"])
+    for kw, text in ((dict(cu_groups=None), "cu_groups"), (dict(k=None), "go together"), (dict(positions=None), "go together"),
+                     (dict(cu_groups=d["cg"][:2]), "ngroups"), (dict(prefix_lens=d["plens"][:1]), "ngroups"),
+                     (dict(block_table=d["bt"][:1]), "nseq"), (dict(k=k[:2]), "same tokens"),
+                     (dict(v_cache=d["vc"][:1]), "contiguous"), (dict(positions=d["pos"][:2]), "positions"),
+                     (dict(block_table=d["bt"].long()), "block_table"), (dict(out=d["qkv"][:, :1024]), "out"),
+                     (dict(q=q[:, :7]), "multiple"), (dict(cache_seqlens=c["lens"]), "cache_seqlens")):
+        with pytest.raises((ValueError, TypeError, RuntimeError), match=text):
+            ops.prefix_attention(**{**base, **kw})
+    with pytest.raises(RuntimeError, match="scale"):
+        ops.prefix_attention(**{**base, "softmax_scale": 0.0})
