@@ -656,10 +656,11 @@ __device__ __forceinline__ void wait_dma() {
 //
 // Two workgroups fit a CU, and a SIMD has a wave of each.  Of the busy CUs' time the
 // matrix units take 42 % in a step of many rows and the vector units about as much;
-// the two overlap only as the two waves happen to lie.  Measured against this, 12
+// the two hardly overlap, and more waves do not make them.  Measured against this, 12
 // prompts at 779 us: 256 rows a block by eight waves over a ring of four steps 847,
 // the same with 32 x 32 products 803, the halves of a workgroup of eight waves
-// taking turns at products and exponents, a barrier between, 873.
+// taking turns at products and exponents, a barrier between, 873; and, at 755, eight
+// waves of 16 rows each, four a SIMD, 776 (48 tokens 64 -> 85).
 constexpr int kStepBytes = kKeys * kD * 2;  // keys, or values, of a step
 
 struct AttnLds {
