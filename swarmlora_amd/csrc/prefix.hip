@@ -504,8 +504,11 @@ __device__ __forceinline__ f32x4 mfma16k16(u32x2 a, u32x2 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
 }
 
+// Token i of a part.  The list holds T tokens: where offsets that overlap make the
+// sequences' tokens more than that (each sequence's lie in 0 .. T - 1 all the same),
+// the last one stands for those that found no place.
 __device__ __forceinline__ int token_at(const PrefixArgs& a, const Part& u, int i) {
-  return u.flags & kListed ? a.list[u.tok0 + i] : u.tok0 + i;
+  return u.flags & kListed ? a.list[min(u.tok0 + i, (int)a.T - 1)] : u.tok0 + i;
 }
 
 // Where a block of keys is: the prefix's pages or the sequence's.

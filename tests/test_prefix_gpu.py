@@ -268,6 +268,20 @@ def test_sequences_before_the_first_group(dev):
     _check(c, dev)
 
 
+def test_offsets_that_overlap_stay_inside_what_is_there(dev):
+    # [0, 4, 0, 4]: 8 tokens share their prefix by these offsets, but there are 4;
+    # what such rows hold is not said, all else is as it was
+    c = _case(44, new=[4, 0, 0], ctx=[20, 0, 20], pre=[81], size=[3])
+    want, _ = _run(c, dev)
+    bad = dict(c, cu=torch.tensor([0, 4, 0, 4], dtype=torch.int32))
+    out = torch.full((8, 8 * 128), 7.0, dtype=BF16, device=dev)
+    _, d = _run(bad, dev, out=out[:4])
+    assert bool((out[4:] == 7).all())
+    for n in ("pt", "bt", "plens", "lens", "cu", "cg", "cs", "pos"):
+        assert torch.equal(d[n].cpu(), bad[n]), n
+    assert torch.equal(_run(c, dev)[0], want)
+
+
 def test_rows_behind_the_last_sequence_are_left(dev):
     c = _case(39, new=[2, 1, 30], ctx=[20, 1, 0], pre=[81], size=[3], extra=5)
     out = torch.full((38, 8 * 128), 7.0, dtype=BF16, device=dev)
