@@ -464,9 +464,10 @@ __global__ __launch_bounds__(256) void prefix_start_kernel(PrefixArgs a, int hea
   if (is_q) {
     dst = a.qrot + (t * a.hq + h) * kD + d;
   } else {
-    const int64_t i = t - (a.cu ? (int64_t)a.cu[s] : (int64_t)s * a.L);
-    const int64_t p = (int64_t)a.lens[s] + i;
-    if (p < 0 || p >= a.kmax) return;
+    int t0, n;
+    tokens_of(a, s, t0, n);
+    const int64_t i = t - t0, p = (int64_t)a.lens[s] + i;
+    if (i < 0 || i >= n || p < 0 || p >= a.kmax) return;
     const uint32_t bi = (uint32_t)p / a.by_bs;
     const int32_t blk = a.bt[(int64_t)s * a.max_blocks + bi];
     if (blk < 0 || blk >= a.num_blocks) return;

@@ -282,6 +282,21 @@ def test_offsets_that_overlap_stay_inside_what_is_there(dev):
     assert torch.equal(_run(c, dev)[0], want)
 
 
+def test_rows_before_the_first_sequence_are_left(dev):
+    # rows 0 and 1 belong to nobody: stored, they would be the two tokens before those of
+    # the first sequence
+    c = _case(45, new=[5, 1], ctx=[20, 40], pre=[81], size=[2])
+    c["cu"] = torch.tensor([2, 5, 6], dtype=torch.int32)
+    out = torch.full((6, 8 * 128), 7.0, dtype=BF16, device=dev)
+    got, d = _run(c, dev, out=out)
+    want, w, kc, vc = _want(c)
+    assert bool((got[:2] == 7).all())
+    assert torch.equal(d["vc"].cpu().view(torch.int16), vc.view(torch.int16))
+    off = (got.cpu().double() - want).abs()[2:]
+    # the tolerance of _check
+    assert bool((off <= 2.0 ** -8 * want[2:].abs() + 2.0 ** -7 * w[2:] + 1e-30).all())
+
+
 def test_rows_behind_the_last_sequence_are_left(dev):
     c = _case(39, new=[2, 1, 30], ctx=[20, 1, 0], pre=[81], size=[3], extra=5)
     out = torch.full((38, 8 * 128), 7.0, dtype=BF16, device=dev)
