@@ -633,11 +633,16 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int 
 // 16 bytes a lane from global memory to LDS at `to` (the same for the wave) + 16
 // lane.  The compiler puts a wait for all of these before every turned read, also
 // of the other buffer (it does not for the builtin's plain reads), so they are
-// issued past it: no register is written, wait_dma is the wait, and nothing else
-// in this kernel uses m0.
+// issued past it: no register is written, wait_dma is the wait.  m0 is left as it was:
+// the compiler does not know that it is written (it takes it for reserved, and warns of
+// it as a clobber).
 __device__ __forceinline__ void dma16(const char* from, char* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"((gbl_ptr)from), "s"(at) : "memory");
+  uint32_t was;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(was)
+               : "v"((gbl_ptr)from), "s"(at)
+               : "memory");
 }
 // (the builtin, so that the compiler knows its own loads to be there as well)
 __device__ __forceinline__ void wait_dma() {
