@@ -555,7 +555,10 @@ __device__ void slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, i
       for (int d = 0; d < 8; ++d) sc += q[d] * kf[d];
 #pragma unroll
       for (int o = 8; o >= 1; o >>= 1) sc += __shfl_xor(sc, o, 16);
-      sc *= c2;
+      {  // rounded before the largest is subtracted of it, as that is (not one fma with it)
+#pragma clang fp contract(off)
+        sc *= c2;
+      }
       const float nm = fmaxf(mx, sc), corr = merge_factor(mx, nm), p = __builtin_amdgcn_exp2f(sc - (nm == -INFINITY ? 0.f : nm));
       sm = sm * corr + p;
 #pragma unroll
@@ -686,6 +689,14 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
   const int kend = (int)min<int64_t>(max<int64_t>((int64_t)u.len + last + 1, 0), a.kmax);  // of the own tokens
   const int all_see = max(min(u.len + (int)((uint32_t)u.r0 / a.by_g) + 1, kend), 0);       // those that every row sees
   const bool idle = wr0 >= rows;  // the wave has no row
+  // Keys of the part that a row with `see` own ones sees (those without a page among
+  // them), and whether the sum l of such a row's probabilities is not to be trusted:
+  // the key of the largest score has a probability of about 1, unless scores are past
+  // 2^31 and what is subtracted of them is rounded so far from theirs that it has none.
+  auto no_sum = [&](float l, int see) {
+    const int own0 = max(u.st0 - u.pre, 0) * kKeys;
+    return l < 0x1p-60f && u.nst > 0 && (u.st0 < u.pre || (u.st0 + u.nst > u.pre && see > own0));
+  };
 
   // Row of the pages that holds the lane's key of a step (key 16 w + col), and
   // the wave's keys that have none.  Keys past the last are the last one.
@@ -716,6 +727,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
 
   const int st_end = u.st0 + u.nst;
   uint32_t none = 0, none_next = 0;
+  bool there = false;  // some key of the part has a page
   int32_t blk = 0;
   if (u.nst > 0) {
     blk = block_of(u.st0);
@@ -778,6 +790,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
       uint64_t gone = none;
       if (MANY)
         gone = (uint64_t)(sh.none[buf][3] << 16 | sh.none[buf][2]) << 32 | (sh.none[buf][1] << 16 | sh.none[buf][0]);
+      there |= gone != (MANY ? ~(uint64_t)0 : 0xffffu);
       const bool pre = st < u.pre;
       const int first = (pre ? st : st - u.pre) * kKeys;
       if (first + kKeys > (pre ? u.plen : all_see) || gone != 0) {
@@ -875,7 +888,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
     if (g == 0) {
       dst[128] = m[e];
       dst[129] = l[e][0];
-      if constexpr (MANY) dst[130] = inverse(l[e][0]);
+      dst[130] = MANY ? inverse(l[e][0]) : there ? 1.f : 0.f;
     }
   };
   auto again = [&](int r) {
@@ -888,7 +901,7 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
       const int r0 = wr0 + 16 * e;
-      bool bad = not_finite(l[e][0]);
+      bool bad = not_finite(l[e][0]) || (there && no_sum(l[e][0], see[e]));
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
@@ -935,6 +948,13 @@ __device__ __forceinline__ void attend_part(const PrefixArgs& a, const Part& u, 
         bad = not_finite(L);
 #pragma unroll
         for (int d = 0; d < 8; ++d) bad |= not_finite(o[d]);
+        if (L < 0x1p-60f) {
+          float some = 0.f;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) some += mg[(v * 16 + row) * F + 130];
+          const int i = (uint32_t)(u.r0 + 16 * e + row) / a.by_g;
+          bad |= some != 0.f && no_sum(L, min(max(u.len + i + 1, 0), kend));
+        }
       }
       const uint64_t redo = __ballot(bad);
       if (row < nr && (redo >> (lane & 48) & 0xffffu) == 0)

@@ -225,6 +225,59 @@ def test_sums_that_leave_32_bits_are_done_again(dev):
     assert bool(torch.isfinite(got).all())
 
 
+def _check_unrotated(c, dev):
+    """_check of a call without positions, whose queries and keys are what is given:
+    fp32 and 64 bits see the same scores."""
+    from swarmlora_amd import ops
+    d = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    q, k, v = _views(c, c["qkv"])
+    got = ops.prefix_attention(*_views(c, d["qkv"]), d["kc"], d["vc"], d["pt"], d["plens"], d["bt"], d["lens"], None, None,
+                               c["scale"], cu_groups=d["cg"], cu_seqlens=d["cu"]).cpu()
+    kc, vc = c["kc"].clone(), c["vc"].clone()
+    _prefix.store(kc, c["bt"], c["lens"], c["cu"], k)
+    _prefix.store(vc, c["bt"], c["lens"], c["cu"], v)
+    o, w = _prefix.attend(q, kc, vc, c["pt"], c["plens"], c["cg"], c["bt"], c["lens"], c["cu"], c["scale"])
+    o, w = o.flatten(1), w.flatten(1)
+    ok = (got.double() - o).abs() <= 2.0 ** -8 * o.abs() + 2.0 ** -7 * w + 1e-30
+    assert bool((ok | (torch.isnan(got) & torch.isnan(o))).all())
+    return got, o
+
+
+LARGE = [dict(new=[1, 1, 2, 1], ctx=[0, 1, 30, 5], pre=[0, 90], size=[2, 2]),
+         dict(new=[1, 40, 33], ctx=[0, 2, 100], pre=[70], size=[3]),
+         dict(new=[1, 1], ctx=[70, 3], pre=[1531], size=[2]),
+         dict(new=[140], ctx=[3], pre=[70], size=[1], page=96)]
+
+
+@pytest.mark.parametrize("kw", LARGE)
+def test_scores_past_32_bits_of_an_exponent(dev, kw):
+    # Scores near 2^40: a step of 32 bits there is thousands of powers of two.  The key of
+    # the largest score is all of a row's result: the next one of any row is further
+    # from it than 128 products' roundings, 128 * 2^-24 of the sum of their magnitudes.
+    c = _case(46, **kw)
+    hq, hkv = c["hq"], c["hkv"]
+    c["qkv"][:, :(hq + hkv) * 128] *= 2.0 ** 18
+    c["kc"] *= 2.0 ** 18
+    q, k, _ = _views(c, c["qkv"])
+    kc = c["kc"].clone()
+    _prefix.store(kc, c["bt"], c["lens"], c["cu"], k)
+    n = 0
+    for s in range(len(kw["new"])):
+        g = sum(s >= int(x) for x in c["cg"][1:])
+        P, last = int(c["plens"][g]), int(c["lens"][s] + kw["new"][s])
+        keys = torch.cat([_prefix.held(kc, c["pt"][g], P)[0], _prefix.held(kc, c["bt"][s], last)[0]])
+        for i in range(kw["new"][s]):
+            for h in range(hq):
+                x = keys[:P + int(c["lens"][s]) + i + 1, h // (hq // hkv)]
+                y = q[n + i, h].double()
+                sc = (x @ y).sort(descending=True).values
+                near = 128 * 2.0 ** -24 * float((x.abs() @ y.abs()).max())
+                assert len(sc) == 1 or float(sc[0] - sc[1]) > 2 * near
+        n += kw["new"][s]
+    got, _ = _check_unrotated(c, dev)
+    assert bool((got != 0).any(1).all())
+
+
 def test_without_new_keys_positions_or_offsets(dev):
     from swarmlora_amd import ops
     c = _case(36, new=[3] * 4, ctx=[5, 0, 40, 9], pre=[100], size=[4])
