@@ -527,10 +527,11 @@ int swl_verify_drafts_bf16(const void* target, int64_t ld_target, const void* dr
  *      they were.
  * Scores, the softmax's statistics and all sums are held in fp32; the
  * probabilities multiply the values as bf16 (each off by up to 2^-8 of itself; the
- * row's sum is of them as rounded).  A query that sees no token gets zeros.
- * Infinities and NaN reach the queries that see their token, nobody else.  Rows
- * whose sums leave fp32 (an infinity, a NaN, values near the largest number) are
- * done again one by one, seeing their own tokens alone: right, but slow.
+ * row's sum is of them as rounded).  A query that sees no token gets zeros, one
+ * that sees some, all with a score of -inf, NaN (0 / 0).  Infinities and NaN reach
+ * the queries that see their token, nobody else.  Rows whose sums leave fp32 (an
+ * infinity, a NaN, values near the largest number, scores past 2^31) are done again
+ * one by one, seeing their own tokens alone: right, but slow.
  * nseq + ngroups at most 1024, ntok under 2^25.  workspace:
  * swl_prefix_attention_workspace(nseq, ntok, ngroups, hq, hkv, max_prefix_blocks *
  * block_size, max_blocks * block_size, positions != NULL) bytes of device memory,

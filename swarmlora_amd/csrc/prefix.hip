@@ -526,9 +526,10 @@ __device__ __forceinline__ Keys keys_of(const PrefixArgs& a, const Part& u, int 
 // One row of a part by a wave, seeing its own keys alone: sixteen lanes a key (8
 // dims each), four keys at a time.  For rows that an infinity or a NaN of a key
 // they do not see may have reached (0 times it is a NaN), and keys without a page.
-// acc: sums of the values times `by`.
-__device__ void slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float by, float& mx,
+// acc: sums of the values times `by`.  Whether it sees a key.
+__device__ bool slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float by, float& mx,
                           float& sm, float (&acc)[8]) {
+  bool seen = false;
   const int i = (uint32_t)r / a.by_g;
   const bf16* qp = a.q + (int64_t)token_at(a, u, i) * a.qs + (int64_t)(h * a.G + r - i * a.G) * kD + 8 * (lane & 15);
   const float c2 = a.scale * 1.44269504088896340736f;
@@ -547,6 +548,7 @@ __device__ void slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, i
       const uint32_t bi = (uint32_t)key / a.by_bs;
       const int32_t blk = ks.table[bi];
       if (blk < 0 || blk >= a.num_blocks) continue;
+      seen = true;
       const int64_t at = (((int64_t)blk * a.bs + (key - bi * a.bs)) * a.hkv + h) * kD + 8 * (lane & 15);
       float kf[8], vf[8], sc = 0.f;
       unpack8(ldg16(a.kc + at), kf);
@@ -570,13 +572,11 @@ __device__ void slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, i
     const float mo = __shfl_xor(mx, o, 64), so = __shfl_xor(sm, o, 64), nm = fmaxf(mx, mo);
     const float ca = merge_factor(mx, nm), cb = merge_factor(mo, nm);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const float ao = __shfl_xor(acc[d], o, 64);
-      acc[d] = (sm == 0.f ? 0.f : acc[d] * ca) + (so == 0.f ? 0.f : ao * cb);
-    }
+    for (int d = 0; d < 8; ++d) acc[d] = acc[d] * ca + __shfl_xor(acc[d], o, 64) * cb;
     sm = sm * ca + so * cb;
     mx = nm;
   }
+  return __ballot(seen) != 0;
 }
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
@@ -584,20 +584,24 @@ __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x)
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }  // (0: no key)
 
 // mean: the row's result.  Where sums of large values are no 32-bit numbers though
-// their means are (2^31 keys at most), the sums are those of 2^-32 of them.
+// their means are (2^31 keys at most), the sums are those of 2^-32 of them.  A row
+// whose keys all have the score -inf has no weight (sm 0) and, which tells it from one
+// without a key, a NaN as its maximum: what it sees elsewhere is its result, or else
+// a NaN.
 __device__ void slow_row(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float& mx, float& sm,
                          float (&mean)[8]) {
-  slow_sums(a, u, h, kend, r, lane, 1.f, mx, sm, mean);
-  const float inv = inverse(sm);
+  const bool seen = slow_sums(a, u, h, kend, r, lane, 1.f, mx, sm, mean);
+  const float inv = inverse(sm), max_or_nan = sm == 0.f && seen ? NAN : mx;
   bool large = false;
 #pragma unroll
   for (int d = 0; d < 8; ++d) {
     large |= not_finite(mean[d]);
     mean[d] *= inv;
   }
+  mx = max_or_nan;
   if (__ballot(large) == 0) return;
-  float of_part[8];
-  slow_sums(a, u, h, kend, r, lane, 0x1p-32f, mx, sm, of_part);
+  float of_part[8], mx_again;
+  slow_sums(a, u, h, kend, r, lane, 0x1p-32f, mx_again, sm, of_part);
 #pragma unroll
   for (int d = 0; d < 8; ++d)
     if (not_finite(mean[d])) mean[d] = of_part[d] * inv * 0x1p32f;
@@ -612,10 +616,10 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, const Part& u, int 
   if (u.flags & kDirect) {
     const int i = (uint32_t)r / a.by_g;
     bf16* dst = a.out + ((int64_t)token_at(a, u, i) * a.hq + h * a.G + r - i * a.G) * kD + d;
-    bf16x2 y[K / 2];  // (L 0: the row sees no key)
+    bf16x2 y[K / 2];  // (m a NaN: keys, but none of any weight; a row without a key has zeros)
 #pragma unroll
     for (int e = 0; e < K / 2; ++e)
-      y[e] = L == 0.f ? bf16x2{f2bf(0.f), f2bf(0.f)} : bf16x2{f2bf(o[2 * e] * inv), f2bf(o[2 * e + 1] * inv)};
+      y[e] = m != m ? bf16x2{f2bf(m), f2bf(m)} : bf16x2{f2bf(o[2 * e] * inv), f2bf(o[2 * e + 1] * inv)};
 #pragma unroll
     for (int e = 0; e < K / 4; ++e)
       stg(dst + 4 * e, u32x2{__builtin_bit_cast(uint32_t, y[2 * e]), __builtin_bit_cast(uint32_t, y[2 * e + 1])});
@@ -996,6 +1000,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
     const int h = (uint32_t)j / a.by_g, row = i * a.G + j - h * a.G;
     float M = -INFINITY, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    bool weightless = false;
     const int64_t pre = r.pre + h * r.pre_head + row, own = r.own + h * r.own_head + row;
     const int parts = r.pre_parts + r.own_parts;
     constexpr int B = 8;  // records in flight together (4: a few % slower, 12: 40 %)
@@ -1014,6 +1019,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
       for (int b = 0; b < B; ++b) {
         if (p0 + b >= parts) break;
         const float mn = fmaxf(M, pm[b]), fa = merge_factor(M, mn), fb = merge_factor(pm[b], mn);
+        weightless |= pm[b] != pm[b];
         if (pl[b] != 0.f) {  // (a part without a key counts for nothing)
           const float la = L * fa, lb = pl[b] * fb, inv = __builtin_amdgcn_rcpf(la + lb);  // (off by 2^-23)
           L = la + lb;
@@ -1022,6 +1028,14 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a, int wgs
           M = mn;
         }
       }
+    }
+    if (weightless) {  // 0 times the values of keys without weight: 0 or a NaN, all NaN where there are no others
+      for (int p = 0; p < parts; ++p) {
+        const int q = p - r.pre_parts;
+        const int64_t at = q < 0 ? pre + (int64_t)p * r.pre_rows : own + (int64_t)q * r.own_rows;
+        if (a.rec_ml[2 * at + 1] == 0.f) o += *(const __attribute__((address_space(1))) f32x4*)(a.rec_o + at * kD + d);
+      }
+      if (L == 0.f) o = f32x4{NAN, NAN, NAN, NAN};
     }
     bf16 y[4];
 #pragma unroll

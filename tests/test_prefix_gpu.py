@@ -278,6 +278,30 @@ def test_scores_past_32_bits_of_an_exponent(dev, kw):
     assert bool((got != 0).any(1).all())
 
 
+@pytest.mark.parametrize("where", ["all", "prefix", "own", "first own", "prefix of values"])
+@pytest.mark.parametrize("kw", LARGE)
+def test_scores_of_minus_infinity(dev, kw, where):
+    # q and k of dim 0 are 1 and, of some keys, -inf: rows that see no other keys have
+    # 0 / 0, the others are as without these
+    c = _case(47, **kw)
+    q, k, v = _views(c, c["qkv"])
+    q[..., 0] = 1
+    if where in ("all", "prefix", "prefix of values"):
+        for g in range(len(c["plens"])):
+            for p in range(int(c["plens"][g])):
+                c["kc"][c["pt"][g, p // c["kc"].shape[1]], p % c["kc"].shape[1], :, 0] = -math.inf
+    if where == "prefix of values":  # 0 times an infinity is a NaN, whatever else the row sees
+        c["vc"][c["pt"][-1, 0], 0, :, 7] = math.inf
+    if where in ("all", "own", "first own"):
+        for s in range(len(kw["new"])):
+            for p in range(int(c["lens"][s])):
+                c["kc"][c["bt"][s, p // c["kc"].shape[1]], p % c["kc"].shape[1], :, 0] = -math.inf
+        (k if where != "first own" else k[:1])[..., 0] = -math.inf
+    got, o = _check_unrotated(c, dev)
+    assert torch.equal(torch.isnan(got), torch.isnan(o))
+    assert where != "all" or bool(torch.isnan(got).all())
+
+
 def test_without_new_keys_positions_or_offsets(dev):
     from swarmlora_amd import ops
     c = _case(36, new=[3] * 4, ctx=[5, 0, 40, 9], pre=[100], size=[4])
