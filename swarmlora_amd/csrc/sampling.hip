@@ -120,18 +120,19 @@ __device__ __forceinline__ float value_of(uint32_t bits) { return __uint_as_floa
 // What a row's weights and bins are taken by.
 struct Row {
   float mx;      // the largest logit
-  float by_bin;  // bins of a unit of logits
+  float by_bin;  // bins of two units of logits
   double rate;   // 256ths of a power of two of a unit
 };
 __device__ __forceinline__ Row row_of(float mx, float temp) {
   Row r;
   r.mx = mx;
   r.rate = 256.0 * 1.44269504088896340735992468100 / (double)temp;
-  r.by_bin = fminf((float)(r.rate * (kPerPower / 256)), 1e30f);
+  r.by_bin = fminf((float)(r.rate * (kPerPower / 128)), 1e30f);
   return r;
 }
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
-  return (int)fminf((r.mx - x) * r.by_bin, (float)kOut);  // (-inf, and the NaN of a rate of 0 times it: kOut)
+  // (by halves: two finite logits can be more than the largest number apart)
+  return (int)fminf((0.5f * r.mx - 0.5f * x) * r.by_bin, (float)kOut);  // (-inf, and the NaN of a rate of 0 times it: kOut)
 }
 // unit 2^(k / 256), k = 0 .. 255, a thread each: the series of 2^f for |f| <= 1/2
 // (the next term is under 2e-16 of it), times 2^(1/2)

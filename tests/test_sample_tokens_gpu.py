@@ -128,6 +128,28 @@ def test_temperatures(dev, t):
     _check(dev, x, u, [t] * 12, [0, 50, 0, 0, 900, 3] * 2, [1.0, 1.0, 0.9, 1.0, 0.99, 0.5] * 2, [0.0, 0.0, 0.0, 0.3, 0.0, 0.1] * 2)
 
 
+@pytest.mark.parametrize("t", [1e37, 1e38, 3e38, float("inf")])
+def test_logits_further_apart_than_the_largest_number(dev, t):
+    # from -3.4e38 to 3.4e38: at these temperatures tokens of the lower half weigh
+    # something too
+    from swarmlora_amd import ops
+    g = torch.Generator().manual_seed(13)
+    big = torch.finfo(BF16).max
+    x = ((2 * torch.rand(12, 9000, generator=g, dtype=torch.float64) - 1) * big).to(BF16)
+    x[:, 100] = big
+    x[6:, ::7] = -big
+    x[9:, 1:8000] = float("-inf")
+    u = ((torch.arange(12) + 0.5) / 12).tolist()
+    k, p, m = [0, 8000, 0, 0, 5000, 30] * 2, [1.0, 1.0, 0.9, 1.0, 0.99, 0.5] * 2, [0.0, 0.0, 0.0, 0.3, 0.0, 0.1] * 2
+    got = ops.sample_tokens(x.to(dev), *[_f32(a).to(dev) for a in (u, [t] * 12)], torch.tensor(k, dtype=torch.int32, device=dev),
+                            _f32(p).to(dev), _f32(m).to(dev)).cpu()
+    # an infinite temperature by 1e300: e^(-7e38 / 1e300) is 1 in 64 bits and e^(-inf /
+    # 1e300) is 0, where -inf / inf is no number
+    f = lambda a: float(_f32([a]))  # noqa: E731
+    assert got.tolist() == [want_token(x[i].double().numpy(), f(u[i]), min(f(t), 1e300), k[i], f(p[i]), f(m[i]))
+                            for i in range(12)]
+
+
 def test_list_longer_than_its_room(dev):
     """A border among more tokens than are listed: all near one logit."""
     g = torch.Generator().manual_seed(2)
