@@ -228,9 +228,13 @@ class BatchedDecoder:
     def _init_kv(self, ctx_lens, kv_fill):
         s, dev, W = self.shape, self.device, self.W
         P = len(self.prefixes)
-        longest = max([t for t, _ in self.prefixes], default=0)
-        self.kv = PagedKVCache(s.layers, s.kv_heads, s.head_dim, s.block_size, W + P,
-                               max(max(ctx_lens) + self.max_new, longest), dev, BF16)
+        longest, own = max([t for t, _ in self.prefixes], default=0), max(ctx_lens) + self.max_new
+        blocks = lambda n: (n + s.block_size - 1) // s.block_size  # noqa: E731
+        # with prefixes, the pages that there are tokens for: a prefix's are not reserved
+        # for every worker
+        need = sum(blocks(c + self.max_new) for c in ctx_lens) + sum(blocks(t) for t, _ in self.prefixes)
+        self.kv = PagedKVCache(s.layers, s.kv_heads, s.head_dim, s.block_size, W + P, max(own, longest), dev, BF16,
+                               need if P else None)
         for w, c in enumerate(ctx_lens):
             self.kv.ensure_blocks_for_length(w, c + self.max_new)
             self.kv.slot_seq_lens[w] = c
@@ -238,7 +242,7 @@ class BatchedDecoder:
             self.kv.ensure_blocks_for_length(W + i, t)
             self.kv.slot_seq_lens[W + i] = t
         tables = self.kv.get_block_table_tensor(list(range(W + P)))
-        self.block_tables, self.prefix_tables = tables[:W], tables[W:]
+        self.block_tables, self.prefix_tables = tables[:W, :blocks(own)].contiguous(), tables[W:, :blocks(longest)].contiguous()
         if kv_fill is not None:
             for li in range(s.layers):
                 kv_fill(li, self.kv.key_caches[li], self.kv.value_caches[li], tables)
@@ -252,8 +256,8 @@ class BatchedDecoder:
             of = [t for t, n in self.prefixes for _ in range(n)]
             self.prefix_of = torch.tensor(of + [0] * (W - len(of)), dtype=torch.int64).to(dev)
         from .worker.paged_attention import RotaryInvFreq, build_vllm_cos_sin_cache
-        self.cos_sin = build_vllm_cos_sin_cache(RotaryInvFreq(s.head_dim, s.theta), longest +
-                                                self.kv.max_blocks_per_seq * s.block_size, dev, BF16)
+        self.cos_sin = build_vllm_cos_sin_cache(RotaryInvFreq(s.head_dim, s.theta), longest + blocks(own) * s.block_size,
+                                                dev, BF16)
 
     def _init_fused(self, weights, adapters, ctx_lens, first_ids, kv_fill):
         """In-process step over explicit token rows with the round fusions

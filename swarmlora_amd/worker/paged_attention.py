@@ -19,10 +19,11 @@ from .. import ops
 class PagedKVCache:
     """Per-layer K and V page pools with a LIFO free list (the first
     allocations get blocks 0, 1, 2, ...), per-slot block tables and
-    sequence lengths."""
+    sequence lengths.  num_blocks (an addition): pages of a pool; None: as many as
+    let every slot have max_seq_len tokens."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int, max_slots: int,
-                 max_seq_len: int, device, dtype: torch.dtype):
+                 max_seq_len: int, device, dtype: torch.dtype, num_blocks: Optional[int] = None):
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
@@ -30,7 +31,7 @@ class PagedKVCache:
         self.device = device
         self.dtype = dtype
         self.max_blocks_per_seq = (max_seq_len + block_size - 1) // block_size
-        self.num_blocks = max_slots * self.max_blocks_per_seq
+        self.num_blocks = max_slots * self.max_blocks_per_seq if num_blocks is None else num_blocks
         self._make_pools()
         self.free_blocks = list(range(self.num_blocks - 1, -1, -1))
         self.slot_block_tables: Dict[int, List[int]] = {}
@@ -103,10 +104,11 @@ class PagedKVCache4(PagedKVCache):
     it in place of the bf16 cache.  head_dim 128, block_size a multiple of 16."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int, max_slots: int,
-                 max_seq_len: int, device, dtype: torch.dtype = torch.bfloat16):
+                 max_seq_len: int, device, dtype: torch.dtype = torch.bfloat16, num_blocks: Optional[int] = None):
         if head_dim != 128 or dtype != torch.bfloat16:
             raise ValueError("the 4-bit cache takes bf16 heads of 128 dims")
-        super().__init__(num_layers, num_kv_heads, head_dim, block_size, max_slots, max_seq_len, device, dtype)
+        super().__init__(num_layers, num_kv_heads, head_dim, block_size, max_slots, max_seq_len, device, dtype,
+                         num_blocks)
 
     def _make_pools(self):
         self.pages = [ops.kv4_pages(self.num_blocks, self.block_size, self.num_kv_heads, self.device)

@@ -76,6 +76,23 @@ def test_shared_prompts_and_sampling(dev):
         dec.close()
 
 
+def test_a_prefix_takes_its_pages_once(dev):
+    prefixes = [(3000, 3), (161, 1)]
+    dec = _decoder(dev, prefixes=prefixes)[0]
+    try:
+        # 8 tokens to come; pages of 16
+        assert dec.kv.num_blocks == sum((c + 8 + 15) // 16 for c in CTX) + 188 + 11
+        assert all(t.shape[0] == dec.kv.num_blocks for t in dec.kv.key_caches + dec.kv.value_caches)
+        assert dec.block_tables.shape == (5, 7) and dec.prefix_tables.shape == (2, 188)
+        assert not dec.kv.free_blocks
+        for _ in range(8):
+            dec.step()
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(dec.logits).all())
+    finally:
+        dec.close()
+
+
 @pytest.mark.parametrize("fused", [False, True])
 def test_sampling_at_no_temperature_is_the_greedy_step(dev, fused):
     told = []

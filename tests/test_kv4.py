@@ -150,3 +150,15 @@ def test_cache_of_four_bits_allocates_as_the_bf16_one():
         PagedKVCache4(1, 2, 128, 24, 1, 64, "cpu")
     with pytest.raises(ValueError, match="outside"):
         c4.read(0, 0, 3, 3)
+
+
+def test_pool_of_fewer_pages_than_slots_could_have():
+    from swarmlora_amd.worker.paged_attention import PagedKVCache, PagedKVCache4
+    for c in (PagedKVCache(1, 2, 128, 16, 3, 100, "cpu", torch.bfloat16, num_blocks=5),
+              PagedKVCache4(1, 2, 128, 16, 3, 100, "cpu", num_blocks=5)):
+        assert c.num_blocks == 5 and c.max_blocks_per_seq == 7 and all(p.shape[0] == 5 for p in c._pools())
+        c.ensure_blocks_for_length(0, 64)
+        c.ensure_blocks_for_length(1, 16)
+        assert c.slot_block_tables == {0: [0, 1, 2, 3], 1: [4]}
+        with pytest.raises(RuntimeError, match="only 0 free"):
+            c.ensure_blocks_for_length(2, 1)
