@@ -151,6 +151,10 @@ class BatchedDecoder:
             raise ValueError("prefixes need the fused step")
         if any(t < 1 or n < 1 for t, n in self.prefixes) or sum(n for _, n in self.prefixes) > W:
             raise ValueError("prefixes: at least one token and worker each, no more workers than there are")
+        if sampling is not None:
+            if not {"u", "temperature"} <= set(sampling) <= {"u", "temperature", "top_k", "top_p", "min_p"}:
+                raise ValueError("sampling: u and temperature, and those of top_k, top_p and min_p that are wanted")
+            ops.check_sampling(W, torch.cuda.current_device(), **sampling)
         self.sampling = sampling
         self.max_new = max_new
         self.steps_done = 0

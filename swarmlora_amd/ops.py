@@ -726,6 +726,18 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, u_accept
     return tok, acc
 
 
+def check_sampling(n: int, dev: int, u, temperature, top_k=None, top_p=None, min_p=None, out=None):
+    """Raises what sample_tokens does for parameters that are none of n rows on the
+    current device (index `dev`)."""
+    for t, nm, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32), (top_k, "top_k", _I32),
+                      (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32), (out, "out", torch.int64)):
+        if t is None and nm not in ("u", "temperature"):
+            continue
+        _here(t, nm, dt, dev)
+        if t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous with one entry per row")
+
+
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
                   top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
                   min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -738,13 +750,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tens
     tensor."""
     dev = _device_for(logits, "logits", BF16)
     n, vocab, ld = _logit_rows(logits, "logits", True, dev)
-    for t, nm, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32), (top_k, "top_k", _I32),
-                      (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32), (out, "out", torch.int64)):
-        if t is None and nm not in ("u", "temperature"):
-            continue
-        _here(t, nm, dt, dev)
-        if t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{nm} must be contiguous with one entry per row")
+    check_sampling(n, dev, u, temperature, top_k, top_p, min_p, out)
     if out is None:
         out = logits.new_empty(n, dtype=torch.int64)
     lib = _lib.load()

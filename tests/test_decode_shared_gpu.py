@@ -105,6 +105,18 @@ def test_sampling_at_no_temperature_is_the_greedy_step(dev, fused):
     assert told[0] == told[1]
 
 
+def test_sampling_is_looked_at_when_the_decoder_is_made(dev):
+    u, t = torch.zeros(5, device=dev), torch.ones(5, device=dev)
+    for kw, error, text in ((dict(u=u), ValueError, "u and temperature"), (dict(temperature=t), ValueError, "u and temperature"),
+                            (dict(u=u, temperature=t, topk=t), ValueError, "u and temperature"),
+                            (dict(u=u, temperature=t[:4]), ValueError, "temperature must be contiguous"),
+                            (dict(u=u, temperature=t, top_k=t), TypeError, "top_k"),
+                            (dict(u=u, temperature=t, top_p=t.cpu()), (ValueError, RuntimeError), "top_p"),
+                            (dict(u=u, temperature=t, out=t.long()), ValueError, "u and temperature")):
+        with pytest.raises(error, match=text):
+            _decoder(dev, sampling=kw)
+
+
 def test_refusals(dev):
     for kw, text in ((dict(prefixes=[(16, 2)], fused=False), "fused"), (dict(prefixes=[(0, 2)]), "at least one"),
                      (dict(prefixes=[(16, 4), (16, 2)]), "at least one")):
