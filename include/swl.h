@@ -532,7 +532,9 @@ int swl_verify_drafts_bf16(const void* target, int64_t ld_target, const void* dr
  * the queries that see their token, nobody else.  Rows whose sums leave fp32 (an
  * infinity, a NaN, values near the largest number, scores past 2^31) are done again
  * one by one, seeing their own tokens alone: right, but slow.
- * nseq + ngroups at most 1024, ntok under 2^25.  workspace:
+ * nseq + ngroups at most 1024; ntok, times the heads to rotate and to store (hq
+ * where positions are given, 2 hkv where k is) over 32, rounded up, under 2^24 - 1.
+ * workspace:
  * swl_prefix_attention_workspace(nseq, ntok, ngroups, hq, hkv, max_prefix_blocks *
  * block_size, max_blocks * block_size, positions != NULL) bytes of device memory,
  * 16-byte aligned, owned by the call until its kernels have run; its contents do
@@ -580,7 +582,8 @@ int swl_sample_tokens_bf16(const void* logits, int64_t ld, int64_t n, int64_t vo
  * ext_aggregator.cpp:545-621).  A row is held as codes in -127 .. 127 and one
  * scale: scale = largest magnitude / 127, code = element * 127 / largest, to the
  * nearest, halves to even; a row of zeros has scale 0, one with an infinity or a NaN
- * codes of 0 and a NaN scale.  k at most 131072, so that no sum leaves 32 bits.
+ * codes of 0 and a NaN scale.  k at most 131072, so that no sum leaves 32 bits; a
+ * weight has under 2^26 rows.
  * All calls can be captured into a graph. */
 
 /* Codes q [m, k] (int8, row stride ldq, a multiple of 16 of at least k rounded up to

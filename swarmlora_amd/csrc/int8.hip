@@ -25,6 +25,8 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kStep = 128;   // k of a step (two blocks)
 constexpr int kCus = 256;    // of an MI355X
+constexpr int64_t kMaxChannels = (int64_t)1 << 26;  // (packed by 64 threads each)
+static_assert(swl::grid_fits((kMaxChannels - 1) / 16, 1024), "");
 
 __device__ __forceinline__ i32x4 mfma_i8(u32x4 a, u32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
@@ -546,7 +548,7 @@ int launch_tiles(const Int8Args& a, hipStream_t st) {
   using Geo = TileGeom<NI, NJ, WM, SLOTS>;
   const int tiles_m = (int)((a.m + Geo::MT - 1) / Geo::MT);
   const int64_t all = tiles_m * ((a.n + Geo::NT - 1) / Geo::NT);
-  SWL_CHECK(all < ((int64_t)1 << 28), SWL_ERR_INVALID, "swl_int8_matmul_bf16: too many rows");
+  SWL_CHECK(swl::grid_fits(all + 8, 128 * WM), SWL_ERR_INVALID, "swl_int8_matmul_bf16: too many rows");
   const int tiles = (int)all, per_xcd = (tiles + 7) / 8;
   int gm = tiles_m;
   if (tiles <= kCus) {
@@ -590,9 +592,13 @@ extern "C" int swl_int8_rows_bf16(const void* x, int64_t ldx, int64_t m, int64_t
   SWL_CHECK(ldx >= k && ldq >= (k + 15) / 16 * 16, SWL_ERR_INVALID, "swl_int8_rows_bf16: row strides smaller than a row");
   SWL_CHECK(aligned(q, 16) && ldq % 16 == 0, SWL_ERR_INVALID, "swl_int8_rows_bf16: rows of q must be 16-byte aligned");
   // (threads with two vectors of 8 each up to 8192; 107 rows of 14336 7.5 us with 256 threads)
+  constexpr int64_t kRowsLaunch = 1 << 22;
+  static_assert(swl::grid_fits(kRowsLaunch, 512), "");
   auto rows = [&](auto kern, int threads) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)m), dim3(threads), 0, (hipStream_t)stream, reinterpret_cast<const bf16*>(x), ldx,
-                       k, reinterpret_cast<int8_t*>(q), ldq, scale);
+    for (int64_t r = 0; r < m; r += kRowsLaunch)
+      hipLaunchKernelGGL(kern, dim3((unsigned)std::min(m - r, kRowsLaunch)), dim3(threads), 0, (hipStream_t)stream,
+                         reinterpret_cast<const bf16*>(x) + r * ldx, ldx, k, reinterpret_cast<int8_t*>(q) + r * ldq, ldq,
+                         scale + r);
   };
   if (k <= 4096)
     rows(int8_rows_kernel<2, 256>, 256);
@@ -608,7 +614,7 @@ extern "C" int64_t swl_int8_weight_bytes(int64_t n, int64_t k) {
 }
 
 extern "C" int swl_int8_pack_bf16(const void* w, int64_t ldw, int64_t n, int64_t k, void* data, float* scale, void* stream) {
-  SWL_CHECK(n > 0 && n < ((int64_t)1 << 31) && k > 0 && k <= (1 << 17), SWL_ERR_INVALID,
+  SWL_CHECK(n > 0 && n < kMaxChannels && k > 0 && k <= (1 << 17), SWL_ERR_INVALID,
             "swl_int8_pack_bf16: bad channel count, or more than 131072 columns");
   SWL_CHECK(w && data && scale, SWL_ERR_INVALID, "swl_int8_pack_bf16: null argument");
   SWL_CHECK(ldw >= k, SWL_ERR_INVALID, "swl_int8_pack_bf16: row stride smaller than a row");
@@ -627,7 +633,7 @@ extern "C" int64_t swl_int8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
 extern "C" int swl_int8_matmul_bf16(const void* q, int64_t ldq, const float* q_scale, int64_t m, const void* w,
                                     const float* w_scale, int64_t n, int64_t k, const void* bias, void* y, int64_t ldy,
                                     void* workspace, int64_t workspace_bytes, void* stream) {
-  SWL_CHECK(m >= 0 && m < ((int64_t)1 << 31) && n > 0 && n < ((int64_t)1 << 31) && k > 0 && k <= (1 << 17), SWL_ERR_INVALID,
+  SWL_CHECK(m >= 0 && m < ((int64_t)1 << 31) && n > 0 && n < kMaxChannels && k > 0 && k <= (1 << 17), SWL_ERR_INVALID,
             "swl_int8_matmul_bf16: bad sizes, or k over 131072");
   if (m == 0) return SWL_OK;
   SWL_CHECK(q && q_scale && w && w_scale && y, SWL_ERR_INVALID, "swl_int8_matmul_bf16: null argument");

@@ -1128,7 +1128,12 @@ extern "C" int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const 
     return bad("q, k, v, out rows, the caches and cos_sin must be 16-byte aligned");
   const int64_t pmax = ngroups > 0 ? max_prefix_blocks * block_size : 0, kmax = max_blocks * block_size;
   const PrefixLayout l = prefix_layout(nseq, ntok, ngroups, hq, hkv, pmax, kmax, positions != nullptr);
-  if (l.parts * hkv >= ((int64_t)1 << 31) || l.recs >= ((int64_t)1 << 40)) return bad("too many rows");
+  const int heads = (positions ? hq : 0) + (k ? 2 * hkv : 0), heads_wg = (heads + 31) / 32;
+  const int64_t start = 1 + ntok * heads_wg;  // workgroups of the first launch
+  const int rows_wg = ntok * hq > 32768 ? hq : 8, wgs = (hq + rows_wg - 1) / rows_wg;  // of the merge
+  if (!swl::grid_fits(start, 256) || !swl::grid_fits(l.parts * hkv, 256) || !swl::grid_fits(ntok * wgs, 256) ||
+      l.recs >= ((int64_t)1 << 40))
+    return bad("too many rows");
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < l.bytes)
     return bad("workspace smaller than swl_prefix_attention_workspace");
   PrefixArgs a{};
@@ -1182,18 +1187,14 @@ extern "C" int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const 
   a.max_parts = (int32_t)l.parts;
   a.slots = kSlots;
   a.min_steps = kMinSteps;
+  a.rows_wg = rows_wg;
   const hipStream_t st = (hipStream_t)stream;
-  const int heads = (positions ? hq : 0) + (k ? 2 * hkv : 0), heads_wg = (heads + 31) / 32;
-  const int64_t start = 1 + ntok * heads_wg;
-  if (start >= ((int64_t)1 << 31)) return bad("too many rows");
   const size_t lds = (size_t)(nseq + ngroups + 1) * kPlanEntry;
   hipLaunchKernelGGL(prefix_start_kernel, dim3((unsigned)start), dim3(256), lds, st, a, std::max(heads_wg, 1));
   SWL_LAUNCH_CHECK("prefix_start_kernel launch");
   hipLaunchKernelGGL(prefix_attention_kernel, dim3((unsigned)(l.parts * hkv)), dim3(256), 0, st, a);
   SWL_LAUNCH_CHECK("prefix_attention_kernel launch");
   if (l.recs == 0) return SWL_OK;
-  a.rows_wg = ntok * hq > 32768 ? hq : 8;
-  const int wgs = (hq + a.rows_wg - 1) / a.rows_wg;
   hipLaunchKernelGGL(prefix_merge_kernel, dim3((unsigned)(ntok * wgs)), dim3(256), 0, st, a, wgs);
   SWL_LAUNCH_CHECK("prefix_merge_kernel launch");
   return SWL_OK;

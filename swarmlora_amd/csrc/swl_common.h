@@ -93,6 +93,11 @@ int combine_silu_rows_launch(void* dst, void* dst2, const void* src, int64_t row
 int wait_copy_launch(const uint64_t* flag, uint64_t want, int32_t tag, uint32_t* timed_out, uint32_t limit_us,
                      void* dst, const void* src, size_t bytes, hipStream_t stream);
 
+// Whether a launch can have so many workgroups along a dimension: their threads are
+// counted in 32 bits.  Past that the count wraps around without an error, and a few of
+// the workgroups run.
+constexpr bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
+
 }  // namespace swl
 
 #define SWL_HIP(call)                                   \

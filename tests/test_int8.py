@@ -51,6 +51,17 @@ def test_matmul_refusals(kw, text):
     assert text in _lib().last_error()
 
 
+def test_more_workgroups_than_a_launch_has():
+    # 2^22 of 1024 threads for a weight, 2^24 of 256 for a product: their threads are
+    # counted in 32 bits
+    lib = _lib().load()
+    assert lib.swl_int8_pack_bf16(P, 1, 1 << 26, 1, P, P, None) and "channel count" in _lib().last_error()
+    assert lib.swl_int8_matmul_bf16(P, 16, P, 1, P, P, 1 << 26, 1, None, P, 1 << 26, None, 0, None)
+    assert "sizes" in _lib().last_error()
+    assert lib.swl_int8_matmul_bf16(P, 16, P, 1 << 30, P, P, 1 << 20, 1, None, P, 1 << 20, None, 0, None)
+    assert "too many rows" in _lib().last_error()
+
+
 def test_nothing_to_do_and_sizes():
     lib = _lib().load()
     assert lib.swl_int8_rows_bf16(None, 100, 0, 100, None, 112, None, None) == 0

@@ -70,6 +70,16 @@ def test_rows(dev, k):
     assert bool((off <= 2.0 ** -24 * ws.nan_to_num() + 2.0 ** -150).all())
 
 
+@pytest.mark.parametrize("m", [2 ** 22, 2 ** 22 + 5, 2 ** 24 + 5])
+def test_more_rows_than_a_launch_has(dev, m):
+    from swarmlora_amd import ops
+    x = torch.randn(m, 1, generator=torch.Generator(dev).manual_seed(1), device=dev).to(BF16)
+    q, s = ops.int8_rows(x)
+    # (one division in fp32 on either side, exact to half a step)
+    assert torch.equal(q, (127 * x.sign()).to(torch.int8))
+    assert bool(((s.double() * 127 - x[:, 0].double().abs()).abs() <= 2.0 ** -24 * x[:, 0].double().abs()).all())
+
+
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 129), (100, 1000), (130, 64)])
 def test_weight(dev, n, k):
     from swarmlora_amd import ops

@@ -42,6 +42,16 @@ def test_refusals(kw, text):
     assert text in _lib().last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(ntok=1 << 24), dict(ntok=(1 << 24) + 5, pos=None, cs=None, k=None, v=None), dict(ntok=1 << 23, hq=16, hkv=16, ks=2048, vs=2048),
+])
+def test_more_workgroups_than_a_launch_has(kw):
+    # 2^24 of 256 threads: their threads are counted in 32 bits
+    lib = _lib().load()
+    assert _call(lib, **{**dict(nseq=1, hq=1, hkv=1, qs=2048, ks=128, vs=128, wsb=1 << 60), **kw}) != 0
+    assert "too many rows" in _lib().last_error()
+
+
 def test_nothing_to_do_and_workspace():
     lib = _lib().load()
     assert _call(lib, nseq=0, ntok=0) == 0
