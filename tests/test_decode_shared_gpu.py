@@ -76,6 +76,44 @@ def test_shared_prompts_and_sampling(dev):
         dec.close()
 
 
+def test_prefixes_that_end_inside_a_page(dev):
+    # 37 and 161 tokens in pages of 16; the oracle has pages of its own, with every
+    # worker's tokens one after another
+    prefixes, before, of = [(37, 2), (161, 2)], [37, 37, 161, 161, 0], [0, 0, 1, 1, None]
+    dec, shape, wts, ads, pages = _decoder(dev, prefixes=prefixes)
+    try:
+        own, pre = dec.block_tables.cpu(), dec.prefix_tables.cpu()
+        width = max((b + c + 8 + 15) // 16 for b, c in zip(before, CTX))
+        bt = torch.arange(5 * width, dtype=torch.int32).view(5, width)
+        at = lambda row, p: (row[p // 16].long(), p % 16)  # noqa: E731
+        held = [[torch.zeros(5 * width, 16, *p.shape[2:], dtype=p.dtype) for p in ps] for ps in pages]
+        for w in range(5):
+            t = torch.arange(before[w] + CTX[w])
+            ctx = t >= before[w]
+            for ps, hs in zip(pages, held):
+                for p, x in zip(ps, hs):
+                    if of[w] is not None:
+                        x[at(bt[w], t[~ctx])] = p[at(pre[of[w]], t[~ctx])]
+                    x[at(bt[w], t[ctx])] = p[at(own[w], t[ctx] - before[w])]
+        cs = ref.cos_sin_cache(ref.rope_inv_freq(shape.head_dim, shape.theta), dec.cos_sin.shape[0])
+        for step in range(4):
+            if step == 2:
+                dec.capture()
+            ids = dec.ids.reshape(-1).cpu()
+            dec.step()
+            torch.cuda.synchronize()
+            seq = torch.tensor([c + b + step for c, b in zip(CTX, before)], dtype=torch.int32)
+            _, lg = ref.decode_step(shape, wts, ads, *held, bt, seq, ids, cs)
+            assert rel_err(dec.logits.cpu(), lg) <= TOL, step
+        for li in range(shape.layers):  # the new tokens' keys and values
+            for mine, want in ((dec.kv.key_caches[li].cpu(), held[0][li]), (dec.kv.value_caches[li].cpu(), held[1][li])):
+                for w in range(5):
+                    new = torch.arange(4) + CTX[w]
+                    assert rel_err(mine[at(own[w], new)], want[at(bt[w], new + before[w])]) <= TOL
+    finally:
+        dec.close()
+
+
 def test_a_prefix_takes_its_pages_once(dev):
     prefixes = [(3000, 3), (161, 1)]
     dec = _decoder(dev, prefixes=prefixes)[0]

@@ -80,6 +80,17 @@ def test_more_rows_than_a_launch_has(dev, m):
     assert bool(((s.double() * 127 - x[:, 0].double().abs()).abs() <= 2.0 ** -24 * x[:, 0].double().abs()).all())
 
 
+@pytest.mark.parametrize("n,k", [(130, 14336), (17, 40001), (28672, 130)])
+def test_large_weight(dev, n, k):
+    from swarmlora_amd import ops
+    w = _randn((n, k), n + k)
+    w[3] = 0
+    p = ops.Int8Weight(w.to(dev))
+    wq, ws = codes(w)
+    assert torch.equal(unpacked(p), wq)
+    assert bool(((p.scale.cpu().double() - ws).abs() <= 2.0 ** -24 * ws).all())
+
+
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 129), (100, 1000), (130, 64)])
 def test_weight(dev, n, k):
     from swarmlora_amd import ops
@@ -107,6 +118,45 @@ def test_product(dev, m, n, k, with_bias):
     y = ops.int8_matmul(q, s, p, None if bias is None else bias.to(dev))
     assert y.shape == (m, n) and y.dtype == BF16
     check(y, q.cpu().double(), s.cpu().double(), unpacked(p), p.scale.cpu().double(), bias)
+
+
+# Every kernel that a call can take, over more steps of k than it has places for: 16, 32
+# and 64 rows by one, two and four tiles of 16 channels a workgroup (waves of several
+# steps each), tiles of 128 x 128 whole and with k split, tiles of 256 x 256.
+LONG = [(16, 1000, 3000), (1, 12300, 1200), (28, 1031, 5000), (17, 6144, 2100), (28, 12300, 1200), (50, 700, 5000),
+        (60, 4000, 3000), (64, 16400, 1200), (200, 3100, 1900), (1700, 1500, 1100), (2325, 4864, 1100), (2305, 4700, 3333)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+def test_product_of_many_steps(dev, m, n, k):
+    """Codes that differ in every step, row and channel: a stage read too early or left
+    from another one, or a swapped tile, has other sums."""
+    from swarmlora_amd import ops
+    p = ops.Int8Weight(_randn((n, k), n).to(dev))
+    q, s = ops.int8_rows(_randn((m, k), m + k).to(dev))
+    y = ops.int8_matmul(q, s, p)
+    check(y, q.cpu().double(), s.cpu().double(), unpacked(p), p.scale.cpu().double(), None)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 12300, 14336), (40, 12300, 8100), (40, 500, 14336), (300, 700, 14336), (2325, 4864, 4096)])
+def test_largest_codes_by_channel_and_step(dev, m, n, k):
+    """Codes of +-127 alone whose signs differ by channel, row and step of 64 k, so that
+    sums lie between -k 127^2 and k 127^2, each another."""
+    from swarmlora_amd import ops
+    g = torch.Generator().manual_seed(m + n)
+    sign = lambda *shape: 1 - 2 * torch.randint(0, 2, shape, generator=g)  # noqa: E731
+    steps = (k + 63) // 64
+    flip = torch.where(torch.rand(n, steps, generator=g) < torch.linspace(0, 1, n)[:, None], -1, 1)
+    base = sign(k)
+    wq = 127 * base * flip.repeat_interleave(64, 1)[:, :k]
+    q = 127 * base * torch.where(torch.rand(m, steps, generator=g) < 0.1, -1, 1).repeat_interleave(64, 1)[:, :k]
+    w = ops.Int8Weight((wq / 127).to(BF16).to(dev))
+    assert torch.equal(unpacked(w), wq.double())
+    room = torch.zeros(m, (k + 15) // 16 * 16, dtype=torch.int8)
+    room[:, :k] = q
+    s = torch.ones(m, device=dev)
+    y = ops.int8_matmul(room.to(dev)[:, :k], s, w)
+    check(y, q.double(), s.cpu().double(), wq.double(), w.scale.cpu().double(), None)
 
 
 @pytest.mark.parametrize("m", [5, 40, 100, 300, 3000])
