@@ -174,6 +174,20 @@ def test_largest_sums_are_exact(dev, m):
     assert bool(((y - t).abs() <= (2.0 ** -8 + 2.0 ** -22) * t.abs()).all())
 
 
+@pytest.mark.parametrize("m", [3, 20, 70, 600])
+def test_longest_rows(dev, m):
+    """131072 codes of -128 (made otherwise: rows have -127 at least) by 127, and of 127:
+    sums within 32 bits by less than 1 %."""
+    from swarmlora_amd import ops
+    k, n = 131072, 40
+    q = torch.full((m, k), -128, dtype=torch.int8)
+    q[1::2] = 127
+    w = ops.Int8Weight(torch.ones(n, k, dtype=BF16, device=dev))
+    s = torch.ones(m, device=dev)
+    check(ops.int8_matmul(q.to(dev), s, w), q.double(), s.cpu().double(), torch.full((n, k), 127.0).double(),
+          w.scale.cpu().double(), None)
+
+
 def test_views_and_strides(dev):
     from swarmlora_amd import ops
     m, n, k = 50, 70, 333

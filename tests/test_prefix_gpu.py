@@ -121,6 +121,16 @@ def test_against_the_definition(dev, name, kw):
 
 
 @pytest.mark.parametrize("name,kw", [
+    ("129 heads", dict(new=[1, 2], ctx=[20, 1], pre=[81], size=[2], hq=129, hkv=1)),
+    ("200 heads of two", dict(new=[1, 2, 1], ctx=[20, 1, 300], pre=[700, 0], size=[2, 1], hq=400, hkv=2)),
+    ("127 heads", dict(new=[1, 2, 0], ctx=[20, 1, 5], pre=[81], size=[3], hq=127, hkv=1)),
+    ("128 heads behind nothing", dict(new=[1, 1], ctx=[20, 1], pre=[], size=[], hq=128, hkv=1)),
+])
+def test_more_heads_than_a_block_has_rows(dev, name, kw):
+    _check(_case(sum(map(ord, name)), **kw), dev)
+
+
+@pytest.mark.parametrize("name,kw", [
     ("many parts of a prefix", dict(new=[1, 1, 2], ctx=[20, 700, 1], pre=[20011], size=[3], max_pos=32768)),
     ("many sequences and groups", dict(new=[1] * 523, ctx=[i % 40 for i in range(523)], pre=[i % 70 for i in range(301)],
                                        size=[3 if i % 2 else 0 for i in range(301)], hq=2, hkv=1)),

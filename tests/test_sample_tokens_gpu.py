@@ -159,6 +159,29 @@ def test_list_longer_than_its_room(dev):
            [1.0, 0.6, 0.5, 1.0, 0.31, 0.77])
 
 
+def test_largest_vocabulary(dev):
+    V = 1 << 21
+    g = torch.Generator().manual_seed(21)
+    x = torch.zeros(6, V, dtype=BF16)  # equal logits: all sums are whole numbers on either side
+    x[3:, ::3] = float("-inf")
+    _check(dev, x, torch.rand(6, generator=g).tolist(), [1.0] * 6, [0, 1000003, 0, 0, 700001, 5], [1.0, 1.0, 0.5, 1.0, 1.0, 1.0])
+
+
+def test_most_rows(dev):
+    from swarmlora_amd import ops
+    n, V = 65535, 37
+    g = torch.Generator(dev).manual_seed(22)
+    x = torch.randn(n, V, generator=g, device=dev).to(BF16)
+    u, t = torch.rand(n, generator=g, device=dev), 0.5 + torch.rand(n, generator=g, device=dev)
+    k = torch.randint(0, V, (n,), generator=g, device=dev, dtype=torch.int32)
+    got = ops.sample_tokens(x, u, t, k)
+    for i in range(0, n, 8000):
+        j = min(i + 8000, n)
+        assert torch.equal(got[i:j], ops.sample_tokens(x[i:j], u[i:j].clone(), t[i:j].clone(), k[i:j].clone()))
+    for i in (0, 1, 32767, 32768, 65533, 65534):
+        assert int(got[i]) == want_token(x[i].cpu().double().numpy(), float(u[i]), float(t[i]), int(k[i]))
+
+
 def test_strided_and_unaligned_rows(dev):
     x, u, t = _logits(9, 9001, 7)
     for pad in (1, 3, 8):
