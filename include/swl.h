@@ -568,7 +568,9 @@ int swl_prefix_attention_bf16(const void* q, int64_t q_stride, const void* k, in
  * infinity as the largest logit, or nothing but -inf).  Logits of -inf never come.
  * Weights are 64-bit exponentials in whole multiples of 2^-46 (2^(ceil(log2 vocab)
  * - 63) for vocabularies over 2^17) of the largest, summed exactly: the result
- * does not depend on the order of any sum.
+ * does not depend on the order of any sum.  A row whose filter's border falls among
+ * thousands of equal or nearly equal logits takes long: 128256 equal ones 1.7 ms a
+ * filter.
  * n at most 65535, vocab at most 2097152.  workspace:
  * swl_sample_tokens_workspace(n, vocab) bytes of device memory, 16-byte aligned,
  * owned by the call until its kernels have run; its contents do not matter. */

@@ -518,9 +518,26 @@ __global__ __launch_bounds__(256) void int8_fold_kernel(Int8Args a) {
 //   7.6.  More steps in flight a wave are slower (28672 by 28: one step 22, two 26,
 //   three 27; the registers' cost in waves).
 //   More rows, and 17 to 64 of a long k with few channels, take tiles of 128 x 128
-//   with k split so that there are as many as CUs: 4096 x 14336 by 28 rows streamed
-//   20.3, 8 splits 18.8; by 60 34 and 19.6 (16 splits 25.9); by 107 57 and 22.9; 28672
-//   x 4096 by 60 27.6 and 26.5, 6144 x 4096 by 40 10.0 and 12.1.
+//   with k split so that there are as many as CUs: 4096 x 14336 by 107 rows streamed 57,
+//   8 splits 22.9 (by 60 16 splits 25.9).  17 to 64 rows streamed | by tiles:
+//     k      n      17 rows      28           40           64
+//     4096   4096   7.7 | 11.7   8.5 | 12.2   10.0 | 12.2  12.2 | 13.3
+//            9216   12.2 | 14.4  13.6 | 14.6  17.6 | 15.0  22.2 | 16.2
+//            12288  11.8 | 16.9  11.6 | 16.7  19.0 | 17.0  20.7 | 18.6
+//            28672  21.3 | 26.3  22.1 | 26.6  26.0 | 26.9  28.6 | 27.5
+//     8192   4096   13.0 | 15.0  14.6 | 14.9  16.4 | 15.3  21.5 | 16.2
+//            8192   15.1 | 19.7  16.3 | 20.0  17.7 | 20.3  22.9 | 21.1
+//            9216   21.1 | 20.5  24.3 | 20.7  31.6 | 21.1  41.0 | 22.5
+//            12288  19.8 | 24.1  20.6 | 24.7  34.3 | 25.5  37.2 | 27.6
+//            28672  41.3 | 45.5  41.9 | 46.0  48.3 | 46.5  52.3 | 48.1
+//     14336  4096   22.1 | 20.2  24.2 | 20.0  28.6 | 19.7  36.4 | 20.4
+//            8192   25.2 | 27.7  26.4 | 27.8  30.5 | 28.1  38.5 | 29.2
+//            9216   36.0 | 29.3  41.4 | 29.5  54.4 | 30.4  71.4 | 32.3
+//            12288  32.7 | 40.6  33.5 | 38.3  57.5 | 39.9  62.9 | 43.6
+//            28672  69.4 | 78.4  74.0 | 72.9  79.0 | 73.4  88.5 | 77.2
+//   The rule takes the slower side of 17 to 32 rows at k = 8192 with n of 6144 to 8192 (by
+//   up to 1.3) and at n of 9216 and 10240 with k from 8192 (1.4), and of 33 to 64 rows by n
+//   over 8192 (1.1 to 2.2).
 constexpr int kFewRows = 64;
 
 struct Int8Plan {

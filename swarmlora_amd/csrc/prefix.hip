@@ -22,12 +22,13 @@
 // Measured on an MI355X (32 query heads over 8, replayed in a graph), with the bytes
 // or operations that a pass cannot do without at the rates of a large copy (5.2
 // TB/s) and a large bf16 product (1108 TFLOP/s):
-//   4 tokens behind 700                  16.6 us (0.6): three launches, each a chain
+//   4 tokens behind 700                  17.0 us (0.6): three launches, each a chain
 //                                        of loads that wait for one another
-//   32 tokens behind 4096, 0.5 K own     31.3 us (12.7): start 6.7, parts 17, merge 6
-//   48 tokens, 6 prefixes up to 12000    64 us (48): the pages' stream
-//   28 sequences' drafts behind 8191     49 us (20)
-//   12 prompts up to 1024 behind 8000    732-780 us (526): 750-800 TFLOP/s
+//   32 tokens behind 4096, 0.5 K own     31.7 us (12.7): traced start 7.2, parts 18.6,
+//                                        merge 6.2
+//   48 tokens, 6 prefixes up to 12000    65 us (48): the pages' stream
+//   28 sequences' drafts behind 8191     48.5 us (20)
+//   12 prompts up to 1024 behind 8000    712-732 us (526): 796-818 TFLOP/s
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -524,8 +525,9 @@ __device__ __forceinline__ Keys keys_of(const PrefixArgs& a, const Part& u, int 
 }
 
 // One row of a part by a wave, seeing its own keys alone: sixteen lanes a key (8
-// dims each), four keys at a time.  For rows that an infinity or a NaN of a key
-// they do not see may have reached (0 times it is a NaN), and keys without a page.
+// dims each), four keys at a time.  For rows that an infinity or a NaN of a key they
+// do not see may have reached (0 times it is a NaN), and those whose scores are past
+// what is subtracted of them.
 // acc: sums of the values times `by`.  Whether it sees a key.
 __device__ bool slow_sums(const PrefixArgs& a, const Part& u, int h, int kend, int r, int lane, float by, float& mx,
                           float& sm, float (&acc)[8]) {

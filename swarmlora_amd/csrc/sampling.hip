@@ -23,10 +23,16 @@
 // rows are few, so loops are kept rolled up.
 //
 // Measured on an MI355X, replayed in a graph (a reading of the logits at the rate of a
-// large copy, 5.2 TB/s): one row of 32000, top-p 19 us (0.01): three launches, 3.5 + 7.8 +
-// 14.6 traced, chains of loads, LDS atomics and prefixes that wait for one another; 28
-// rows of 128256 that ask for different things 38 (1.4): 5 + 12 + 28; 256 rows with all
-// filters 108 (12.7): 18 + 50 + 47, two readings weighed in 64 bits.
+// large copy, 5.2 TB/s): one row of 32000, top-p 27.8 us (0.01): three launches, 3.7 + 7.6 +
+// 14.0 traced, chains of loads, LDS atomics and prefixes that wait for one another; 28
+// rows of 128256 that ask for different things 43.5 (1.4): 5 + 12 + 28; 256 rows with all
+// filters 109 (12.7): 18 + 49 + 47, two readings weighed in 64 bits.
+//
+// Flat rows are slow: where more tokens are in the borders' bins than the list holds, the
+// row's last workgroup goes through the whole row for every digit of a border.  A row of
+// 128256 logits, top-p 0.9: normal ones of deviation 2 at a temperature of 1 36 us, 5 49,
+// 20 469; three values 709, all equal 1695 (as much for top-k, both filters twice).
+// 28 such rows 52, 70, 679, 1273, 3254; 256 164, 213, 1464, 2858, 6893.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
